@@ -120,6 +120,17 @@ def lib():
             L.ck_batch_last_error.argtypes = [P]
             L.ck_batch_last_error.restype = ctypes.c_char_p
             L.ck_batch_destroy.argtypes = [P]
+            B = ctypes.c_char_p   # packed argument structs (kv_cache.py)
+            L.ck_kv_create.argtypes = [pp(ctypes.c_int32), I, pp(P)]
+            L.ck_kv_destroy.argtypes = [P]
+            L.ck_kv_bytes.argtypes = [P, pp(S)]
+            L.ck_kv_store.argtypes = [P, B, P]
+            L.ck_kv_load.argtypes = [P, B, P]
+            L.ck_kv_attend.argtypes = [P, B, P]
+            L.ck_kv_attend_prompt.argtypes = [P, B, P, I, P]
+            L.ck_kv_check.argtypes = [P, P]
+            L.ck_kv_last_error.argtypes = [P]
+            L.ck_kv_last_error.restype = ctypes.c_char_p
             _lib = L
     return _lib
 

@@ -111,8 +111,6 @@ struct BAttn {
 // the predecessor grid has completed and its writes are visible) before it
 // reads or writes anything the step's kernels share, then lets its own
 // successor launch.  Without the launch attribute both are no-ops.
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
 // Embedding of every active entry's token (GGUF_*_EMBEDDING_WGSL, :2615-2866).
@@ -169,10 +167,6 @@ __device__ __forceinline__ uint32_t kmaj_off(int row, int k) {
 __device__ __forceinline__ size_t tc_index(int r, int e, int nch, int part) {
   const size_t tile = ((size_t)(r >> 7) * nch + (e >> 6)) * 2 + part;
   return tile * (TC_TILE / 2) + kmaj_off(r & 127, e & 63) / 2;
-}
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);   // version 1, no swizzle
 }
 __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, int* err) {
   unsigned spins = 0;

@@ -18,6 +18,7 @@
 #include "ck_ops.cuh"
 #include "ck_step.cuh"
 #include "ck_gemv.cuh"
+#include "ck_kv.h"
 
 namespace {
 
@@ -32,6 +33,12 @@ int set_global(int code, const char* fmt, ...) {
   g_err = buf;
   return code;
 }
+
+}  // namespace
+
+int ck_global_message(int code, const char* msg) { return set_global(code, "%s", msg); }
+
+namespace {
 
 struct Weight {
   Lay L;

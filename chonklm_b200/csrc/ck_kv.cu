@@ -1,0 +1,368 @@
+// Quantised paged key-value cache: handles, argument checks and the C ABI.
+#include <cuda_runtime.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <new>
+
+#include "../../include/chonk_b200.h"
+#include "ck_kv.h"
+#include "ck_kv.cuh"
+#include "ck_kv_attn.cuh"
+
+// ---------------------------------------------------------------------------
+// Launches
+
+namespace {
+
+template <typename... KArgs, typename... Args>
+cudaError_t kv_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl, Args... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+}  // namespace
+
+size_t kv_pool_bytes(const KvPool& p) {
+  return (size_t)p.n_blocks * p.kvh * (p.block / KV_TILE) * kv_record_bytes(p.hd, p.vbits);
+}
+
+int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes) {
+  *part_bytes = *ml_bytes = 16;
+  return 0;
+}
+
+cudaError_t kv_setup(const KvPool& p) { return cudaSuccess; }
+
+cudaError_t kv_store_launch(const KvStore& a, cudaStream_t s, bool pdl) {
+  if (a.n == 0) return cudaSuccess;
+  const int vec = (kv_vec4(a.q) ? 1 : 0) | (kv_vec4(a.k) ? 2 : 0) | (kv_vec4(a.v) ? 4 : 0) | (kv_vec4(a.qo) ? 8 : 0);
+  const dim3 grid(a.n, 1);
+  switch (a.pool.hd) {
+    case 64: return kv_launch(k_kv_store<64>, grid, dim3(KV_STORE_THREADS), 0, s, pdl, a, vec);
+    case 128: return kv_launch(k_kv_store<128>, grid, dim3(KV_STORE_THREADS), 0, s, pdl, a, vec);
+    default: return kv_launch(k_kv_store<256>, grid, dim3(KV_STORE_THREADS), 0, s, pdl, a, vec);
+  }
+}
+
+cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
+  if (a.n == 0) return cudaSuccess;
+  const int vec = (kv_vec4(a.k) ? 1 : 0) | (kv_vec4(a.v) ? 2 : 0);
+  const long long lanes = (long long)a.n * a.pool.kvh * (a.pool.hd / 4);
+  const dim3 grid((unsigned)((lanes + KV_LOAD_THREADS - 1) / KV_LOAD_THREADS)), block(KV_LOAD_THREADS);
+#define KV_CASE(HD, VB) \
+  if (a.pool.hd == HD && a.pool.vbits == VB) return kv_launch(k_kv_load<HD, VB>, grid, block, 0, s, false, a, vec);
+  KV_CASE(64, 8) KV_CASE(64, 4) KV_CASE(128, 8) KV_CASE(128, 4) KV_CASE(256, 8) KV_CASE(256, 4)
+#undef KV_CASE
+  return cudaErrorInvalidValue;
+}
+
+static cudaError_t kv_attn_simple(const KvAttn& a, int rows, cudaStream_t s, bool pdl) {
+  if (rows == 0) return cudaSuccess;
+  const dim3 grid((unsigned)(((long long)rows * a.heads + 3) / 4)), block(128);
+#define KV_CASE(HD, VB) \
+  if (a.pool.hd == HD && a.pool.vbits == VB) return kv_launch(k_kv_attn_simple<HD, VB>, grid, block, 0, s, pdl, a);
+  KV_CASE(64, 8) KV_CASE(64, 4) KV_CASE(128, 8) KV_CASE(128, 4) KV_CASE(256, 8) KV_CASE(256, 4)
+#undef KV_CASE
+  return cudaErrorInvalidValue;
+}
+cudaError_t kv_attend_launch(const KvAttn& a, int sms, cudaStream_t s, bool pdl) {
+  return kv_attn_simple(a, a.n, s, pdl);
+}
+cudaError_t kv_prompt_launch(const KvAttn& a, int sms, cudaStream_t s) { return kv_attn_simple(a, a.rows, s, false); }
+
+// ---------------------------------------------------------------------------
+// Handles
+
+struct ck_kv {
+  ck_kv_cfg cfg;
+  int device, sms;
+  KvPool pool;
+  float *part, *ml;
+  char err[256];
+
+  int fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(err, sizeof err, fmt, ap);
+    va_end(ap);
+    return code;
+  }
+};
+
+namespace {
+
+// The caller's current device is put back when a call ends.
+struct OnDevice {
+  int was = -1;
+  cudaError_t rc;
+  explicit OnDevice(int dev) {
+    rc = cudaGetDevice(&was);
+    if (rc == cudaSuccess && was != dev) rc = cudaSetDevice(dev);
+    else if (rc == cudaSuccess) was = -1;
+  }
+  ~OnDevice() { if (was >= 0) cudaSetDevice(was); }
+};
+
+int kv_global(int code, const char* fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return ck_global_message(code, buf);
+}
+
+int type_bytes(int t) { return t == CK_DT_F32 ? 4 : 2; }
+
+// token rows: present, of a known type, aligned to their elements
+int check_rows(ck_kv* h, const char* call, const char* name, const ck_kv_rows& r, int n, int heads, bool f32, KvRows* out) {
+  if (!r.dev && n > 0) return h->fail(CK_EINVAL, "%s: %s is null", call, name);
+  if (r.dtype != CK_DT_F16 && r.dtype != CK_DT_BF16 && !(f32 && r.dtype == CK_DT_F32))
+    return h->fail(CK_EINVAL, "%s: %s has type %d, expected %s", call, name, r.dtype, f32 ? "f32, f16 or bf16" : "f16 or bf16");
+  if ((uintptr_t)r.dev % type_bytes(r.dtype)) return h->fail(CK_EINVAL, "%s: %s is not aligned to its elements", call, name);
+  if (r.token_stride < 0 || r.head_stride < 0) return h->fail(CK_EINVAL, "%s: %s has a negative stride", call, name);
+  out->p = r.dev;
+  out->st = r.token_stride;
+  out->sh = r.head_stride;
+  out->type = r.dtype;
+  return CK_OK;
+}
+
+// rows that are written: no two of them may overlap
+int check_out(ck_kv* h, const char* call, const char* name, const ck_kv_rows& r, int n, int heads) {
+  const int64_t hd = h->cfg.head_dim;
+  const bool token_major = r.head_stride >= hd && (n < 2 || r.token_stride >= (heads - 1) * r.head_stride + hd);
+  const bool head_major = r.token_stride >= hd && (heads < 2 || r.head_stride >= (n - 1) * r.token_stride + hd);
+  if (n > 0 && !(heads == 1 && n == 1) && !token_major && !head_major)
+    return h->fail(CK_EINVAL, "%s: rows of %s overlap (strides %lld, %lld)", call, name, (long long)r.token_stride,
+                   (long long)r.head_stride);
+  return CK_OK;
+}
+
+int check_table(ck_kv* h, const char* call, const ck_kv_table& t, KvTable* out) {
+  if (t.n_seqs < 0 || t.max_blocks < 0 || (!t.dev && (int64_t)t.n_seqs * t.max_blocks > 0))
+    return h->fail(CK_EINVAL, "%s: bad block table", call);
+  if ((int64_t)t.max_blocks * h->cfg.block > INT32_MAX - KV_TILE)
+    return h->fail(CK_EINVAL, "%s: %d blocks of %d positions pass the largest position", call, t.max_blocks, h->cfg.block);
+  out->dev = t.dev;
+  out->n_seqs = t.n_seqs;
+  out->max_blocks = t.max_blocks;
+  return CK_OK;
+}
+
+#define KVC(call)                                                                                            \
+  do {                                                                                                       \
+    cudaError_t e_ = (call);                                                                                 \
+    if (e_ != cudaSuccess) return h->fail(CK_ECUDA, "%s: %s", #call, cudaGetErrorString(e_));                \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int ck_kv_create(const ck_kv_cfg* cfg, int device, ck_kv** out) {
+  if (!cfg || !out) return kv_global(CK_EINVAL, "ck_kv_create: bad argument");
+  *out = nullptr;
+  if (cfg->head_dim != 64 && cfg->head_dim != 128 && cfg->head_dim != 256)
+    return kv_global(CK_EINVAL, "ck_kv_create: head_dim %d, expected 64, 128 or 256", cfg->head_dim);
+  if (cfg->kv_heads < 1 || cfg->heads < cfg->kv_heads || cfg->heads > 1024 || cfg->heads % cfg->kv_heads)
+    return kv_global(CK_EINVAL, "ck_kv_create: %d heads over %d kv heads", cfg->heads, cfg->kv_heads);
+  if (cfg->block != 16 && cfg->block != 32 && cfg->block != 64 && cfg->block != 128)
+    return kv_global(CK_EINVAL, "ck_kv_create: blocks of %d positions, expected 16, 32, 64 or 128", cfg->block);
+  if (cfg->v_bits != 8 && cfg->v_bits != 4)
+    return kv_global(CK_EINVAL, "ck_kv_create: values of %d bits, expected 8 or 4", cfg->v_bits);
+  if (cfg->n_blocks < 1) return kv_global(CK_EINVAL, "ck_kv_create: %d blocks", cfg->n_blocks);
+  ck_kv* h = new (std::nothrow) ck_kv();
+  if (!h) return kv_global(CK_ENOMEM, "ck_kv_create: out of host memory");
+  h->cfg = *cfg;
+  h->device = device;
+  KvPool& p = h->pool;
+  p.n_blocks = cfg->n_blocks;
+  p.kvh = cfg->kv_heads;
+  p.block = cfg->block;
+  p.hd = cfg->head_dim;
+  p.vbits = cfg->v_bits;
+  OnDevice on(device);
+  auto bail = [&](int code, const char* what, cudaError_t e) {
+    cudaGetLastError();
+    cudaFree(p.base);
+    cudaFree(p.err);
+    cudaFree(h->part);
+    cudaFree(h->ml);
+    delete h;
+    return kv_global(code, "ck_kv_create: %s: %s", what, cudaGetErrorString(e));
+  };
+  if (on.rc != cudaSuccess) return bail(CK_ECUDA, "device", on.rc);
+  cudaError_t e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device);
+  if (e != cudaSuccess) return bail(CK_ECUDA, "device", e);
+  size_t pb = 0, mb = 0;
+  kv_workspace(p, cfg->heads, h->sms, &pb, &mb);
+  if ((e = cudaMalloc(&p.base, kv_pool_bytes(p))) != cudaSuccess || (e = cudaMalloc(&p.err, 16)) != cudaSuccess ||
+      (e = cudaMalloc(&h->part, pb)) != cudaSuccess || (e = cudaMalloc(&h->ml, mb)) != cudaSuccess)
+    return bail(CK_ENOMEM, "cudaMalloc", e);
+  if ((e = cudaMemset(p.err, 0, 16)) != cudaSuccess || (e = kv_setup(p)) != cudaSuccess ||
+      (e = cudaDeviceSynchronize()) != cudaSuccess)
+    return bail(CK_ECUDA, "set-up", e);
+  *out = h;
+  return CK_OK;
+}
+
+int ck_kv_destroy(ck_kv* h) {
+  if (!h) return CK_OK;
+  OnDevice on(h->device);
+  cudaFree(h->pool.base);   // waits for the device's work
+  cudaFree(h->pool.err);
+  cudaFree(h->part);
+  cudaFree(h->ml);
+  delete h;
+  return CK_OK;
+}
+
+const char* ck_kv_last_error(ck_kv* h) { return h ? h->err : ck_global_error(); }
+
+int ck_kv_bytes(ck_kv* h, size_t* pool_bytes) {
+  if (!h || !pool_bytes) return kv_global(CK_EINVAL, "ck_kv_bytes: bad argument");
+  *pool_bytes = kv_pool_bytes(h->pool);
+  return CK_OK;
+}
+
+int ck_kv_store(ck_kv* h, const ck_kv_store_args* a, void* stream) {
+  if (!h || !a) return kv_global(CK_EINVAL, "ck_kv_store: bad argument");
+  if (a->n < 0 || (a->n > 0 && (!a->seq || !a->pos))) return h->fail(CK_EINVAL, "ck_kv_store: bad token list");
+  KvStore p;
+  memset(&p, 0, sizeof p);
+  const int H = h->cfg.heads, K = h->cfg.kv_heads;
+  int rc;
+  if ((rc = check_rows(h, "ck_kv_store", "k", a->k, a->n, K, true, &p.k)) ||
+      (rc = check_rows(h, "ck_kv_store", "v", a->v, a->n, K, true, &p.v)) ||
+      (rc = check_table(h, "ck_kv_store", a->table, &p.tab)))
+    return rc;
+  if (a->q.dev) {
+    if ((rc = check_rows(h, "ck_kv_store", "q", a->q, a->n, H, true, &p.q)) ||
+        (rc = check_rows(h, "ck_kv_store", "q_out", a->q_out, a->n, H, false, &p.qo)) ||
+        (rc = check_out(h, "ck_kv_store", "q_out", a->q_out, a->n, H)))
+      return rc;
+    p.heads = H;
+  } else if (a->q_out.dev) {
+    return h->fail(CK_EINVAL, "ck_kv_store: q_out without q");
+  }
+  if (!(a->eps >= 0.f) && (a->q_norm || a->k_norm)) return h->fail(CK_EINVAL, "ck_kv_store: eps %g", a->eps);
+  p.pool = h->pool;
+  p.seq = a->seq;
+  p.pos = a->pos;
+  p.n = a->n;
+  p.qw = a->q_norm;
+  p.kw = a->k_norm;
+  p.inv_freq = a->inv_freq;
+  p.eps = a->eps;
+  p.interleaved = a->interleaved ? 1 : 0;
+  OnDevice on(h->device);
+  KVC(on.rc);
+  KVC(kv_store_launch(p, (cudaStream_t)stream, false));
+  return CK_OK;
+}
+
+int ck_kv_load(ck_kv* h, const ck_kv_load_args* a, void* stream) {
+  if (!h || !a) return kv_global(CK_EINVAL, "ck_kv_load: bad argument");
+  if (a->n < 0 || (a->n > 0 && (!a->seq || !a->pos))) return h->fail(CK_EINVAL, "ck_kv_load: bad token list");
+  KvLoad p;
+  memset(&p, 0, sizeof p);
+  const int K = h->cfg.kv_heads;
+  int rc;
+  if ((rc = check_rows(h, "ck_kv_load", "k", a->k, a->n, K, true, &p.k)) ||
+      (rc = check_rows(h, "ck_kv_load", "v", a->v, a->n, K, true, &p.v)) ||
+      (rc = check_out(h, "ck_kv_load", "k", a->k, a->n, K)) || (rc = check_out(h, "ck_kv_load", "v", a->v, a->n, K)) ||
+      (rc = check_table(h, "ck_kv_load", a->table, &p.tab)))
+    return rc;
+  p.pool = h->pool;
+  p.seq = a->seq;
+  p.pos = a->pos;
+  p.n = a->n;
+  OnDevice on(h->device);
+  KVC(on.rc);
+  KVC(kv_load_launch(p, (cudaStream_t)stream));
+  return CK_OK;
+}
+
+static int attn_args(ck_kv* h, const char* call, const ck_kv_attend_args* a, int rows, KvAttn* p) {
+  memset(p, 0, sizeof *p);
+  if (a->n < 0 || rows < 0 || (a->n > 0 && !a->len)) return h->fail(CK_EINVAL, "%s: bad length list", call);
+  if (a->window < 0) return h->fail(CK_EINVAL, "%s: window %d", call, a->window);
+  if (!(a->scale > -INFINITY && a->scale < INFINITY)) return h->fail(CK_EINVAL, "%s: scale is not finite", call);
+  int rc;
+  if ((rc = check_rows(h, call, "q", a->q, rows, h->cfg.heads, false, &p->q)) ||
+      (rc = check_rows(h, call, "out", a->out, rows, h->cfg.heads, false, &p->o)) ||
+      (rc = check_out(h, call, "out", a->out, rows, h->cfg.heads)) || (rc = check_table(h, call, a->table, &p->tab)))
+    return rc;
+  p->pool = h->pool;
+  p->seq = a->seq;
+  p->len = a->len;
+  p->n = a->n;
+  p->rows = rows;
+  p->heads = h->cfg.heads;
+  p->window = a->window;
+  p->scale = a->scale;
+  p->part = h->part;
+  p->ml = h->ml;
+  return CK_OK;
+}
+
+int ck_kv_attend(ck_kv* h, const ck_kv_attend_args* a, void* stream) {
+  if (!h || !a) return kv_global(CK_EINVAL, "ck_kv_attend: bad argument");
+  KvAttn p;
+  int rc = attn_args(h, "ck_kv_attend", a, a->n, &p);
+  if (rc) return rc;
+  if (!a->seq && a->n > a->table.n_seqs)
+    return h->fail(CK_EINVAL, "ck_kv_attend: %d queries for %d rows of the block table", a->n, a->table.n_seqs);
+  OnDevice on(h->device);
+  KVC(on.rc);
+  KVC(kv_attend_launch(p, h->sms, (cudaStream_t)stream, false));
+  return CK_OK;
+}
+
+int ck_kv_attend_prompt(ck_kv* h, const ck_kv_attend_args* a, const int32_t* cu, int rows, void* stream) {
+  if (!h || !a) return kv_global(CK_EINVAL, "ck_kv_attend_prompt: bad argument");
+  KvAttn p;
+  int rc = attn_args(h, "ck_kv_attend_prompt", a, rows, &p);
+  if (rc) return rc;
+  if (a->seq) return h->fail(CK_EINVAL, "ck_kv_attend_prompt: sequence i reads row i of the block table");
+  if (a->n > a->table.n_seqs)
+    return h->fail(CK_EINVAL, "ck_kv_attend_prompt: %d sequences for %d rows of the block table", a->n, a->table.n_seqs);
+  if (rows > 0 && (!cu || a->n < 1)) return h->fail(CK_EINVAL, "ck_kv_attend_prompt: bad row list");
+  p.cu = cu;
+  OnDevice on(h->device);
+  KVC(on.rc);
+  KVC(kv_prompt_launch(p, h->sms, (cudaStream_t)stream));
+  return CK_OK;
+}
+
+int ck_kv_check(ck_kv* h, void* stream) {
+  if (!h) return kv_global(CK_EINVAL, "ck_kv_check: null cache");
+  OnDevice on(h->device);
+  KVC(on.rc);
+  int bits = 0;
+  cudaStream_t s = (cudaStream_t)stream;
+  KVC(cudaMemcpyAsync(&bits, h->pool.err, sizeof bits, cudaMemcpyDeviceToHost, s));
+  KVC(cudaStreamSynchronize(s));
+  if (!bits) return CK_OK;
+  KVC(cudaMemsetAsync(h->pool.err, 0, sizeof bits, s));
+  KVC(cudaStreamSynchronize(s));
+  return h->fail(CK_EDEVICE, "%s%s%s%s", bits & KV_ERR_SEQ ? "sequence outside the block table; " : "",
+                 bits & KV_ERR_POS ? "position or length outside the block table; " : "",
+                 bits & KV_ERR_BLOCK ? "block table entry outside the pool; " : "",
+                 bits & KV_ERR_WAIT ? "device wait timed out; " : "");
+}
+
+}  // extern "C"

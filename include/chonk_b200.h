@@ -236,6 +236,105 @@ int ck_batch_stats(ck_batch* b, uint64_t* steps, uint64_t* tokens_fed, uint64_t*
 const char* ck_batch_last_error(ck_batch* b);
 int ck_batch_destroy(ck_batch* b);
 
+/* ---- quantised paged key-value cache ----
+ * No counterpart in the reference, whose cache is one fp32 (here also fp16)
+ * buffer per engine (llama-wgsl-runtime.ts:619-919).  One handle holds one
+ * layer's pages: keys in 8 bits, values in 8 or 4, an fp16 scale for each 32
+ * values of a head.  Sequences own blocks of `block` positions through a
+ * block table in device memory ([n_seqs][max_blocks] int32) that the caller
+ * keeps; entries past a sequence's last block are not read.
+ *
+ * The four calls that work on the cache only enqueue their kernels on
+ * `stream` (a cudaStream_t; NULL = the default stream) and allocate nothing,
+ * so they may be captured into a CUDA graph.  All pointers in their arguments
+ * are device pointers, read when the kernels run; calls on one handle have to
+ * be ordered on one stream or by events (ck_kv_attend shares the handle's
+ * workspace).  What only the device can see (a sequence, position or block
+ * out of range) is skipped there and reported by ck_kv_check. */
+typedef struct ck_kv ck_kv;
+
+#define CK_DT_F32 0
+#define CK_DT_F16 1
+#define CK_DT_BF16 2
+
+typedef struct ck_kv_cfg {
+  int32_t heads, kv_heads;         /* heads: a multiple of kv_heads, up to 1024       */
+  int32_t head_dim;                /* 64, 128 or 256                                  */
+  int32_t block;                   /* positions of a block: 16, 32, 64 or 128         */
+  int32_t v_bits;                  /* 8 or 4                                          */
+  int32_t n_blocks;                /* blocks of the pool                              */
+} ck_kv_cfg;
+
+typedef struct ck_kv_rows {        /* [n][heads or kv_heads][head_dim], head_dim contiguous */
+  void* dev;
+  int64_t token_stride, head_stride;   /* in elements */
+  int32_t dtype;                   /* CK_DT_*                                         */
+  int32_t reserved;
+} ck_kv_rows;
+
+typedef struct ck_kv_table {
+  const int32_t* dev;              /* [n_seqs][max_blocks] blocks of the pool         */
+  int32_t n_seqs, max_blocks;
+} ck_kv_table;
+
+typedef struct ck_kv_store_args {
+  ck_kv_rows q, k, v;              /* f32, f16 or bf16; q.dev NULL: only k and v      */
+  ck_kv_rows q_out;                /* f16 or bf16                                     */
+  ck_kv_table table;
+  const int32_t *seq, *pos;        /* [n] row of the table and position; seq < 0: padding, not stored */
+  const float *q_norm, *k_norm;    /* [head_dim] RMS norm weights, or NULL            */
+  const float* inv_freq;           /* [head_dim / 2]; NULL: no rotation               */
+  float eps;
+  int32_t interleaved;             /* rotate (2i, 2i+1) instead of (i, i + head_dim/2) */
+  int32_t n;
+  int32_t reserved;
+} ck_kv_store_args;
+
+typedef struct ck_kv_load_args {
+  ck_kv_rows k, v;                 /* written: f32, f16 or bf16                       */
+  ck_kv_table table;
+  const int32_t *seq, *pos;
+  int32_t n;
+  int32_t reserved;
+} ck_kv_load_args;
+
+typedef struct ck_kv_attend_args {
+  ck_kv_rows q, out;               /* f16 or bf16                                     */
+  ck_kv_table table;
+  const int32_t* len;              /* [n] cached positions, the new ones among them   */
+  const int32_t* seq;              /* ck_kv_attend: [n] row of the table of each query; NULL: query i reads row i */
+  int32_t n;                       /* queries (ck_kv_attend) or sequences (ck_kv_attend_prompt) */
+  int32_t window;                  /* positions seen, the own one among them; 0: all  */
+  float scale;
+  int32_t reserved;
+} ck_kv_attend_args;
+
+int ck_kv_create(const ck_kv_cfg* cfg, int device, ck_kv** out);
+/* Waits for the device's work, then frees the pages. */
+int ck_kv_destroy(ck_kv* h);
+int ck_kv_bytes(ck_kv* h, size_t* pool_bytes);
+/* Norm (where weights are given) and rotate every head of q and k, write q to
+ * q_out, quantise k and v into their pages.  Two tokens of one call must not
+ * name the same place. */
+int ck_kv_store(ck_kv* h, const ck_kv_store_args* a, void* stream);
+/* Keys and values of n tokens as the cache holds them (zero where seq < 0 or
+ * the place does not exist). */
+int ck_kv_load(ck_kv* h, const ck_kv_load_args* a, void* stream);
+/* One new token per query, whose own key and value are stored already:
+ * out = softmax(scale q k) v over the last `window` of its len positions, zero
+ * where len is 0.  The cached length is split over the device and joined.
+ * Products run on 16-bit operands with 32-bit sums: cached values of more
+ * than 65504 in magnitude are out of range. */
+int ck_kv_attend(ck_kv* h, const ck_kv_attend_args* a, void* stream);
+/* Several new tokens per sequence: rows cu[i] .. cu[i + 1] of q ([rows] in
+ * all) are the last tokens of sequence i's len[i] cached positions, each
+ * seeing the positions up to its own. */
+int ck_kv_attend_prompt(ck_kv* h, const ck_kv_attend_args* a, const int32_t* cu, int rows, void* stream);
+/* Waits for `stream`; CK_EDEVICE when a kernel since the last check met a
+ * sequence, position or block out of range. */
+int ck_kv_check(ck_kv* h, void* stream);
+const char* ck_kv_last_error(ck_kv* h);
+
 /* sizeof(ck_model_cfg) and sizeof(ck_sampling) as compiled, so bindings can
  * check their struct mirrors; needs no GPU. */
 void ck_abi_info(int* sizeof_cfg, int* sizeof_sampling);
