@@ -10,6 +10,7 @@
 #include "ck_kv.h"
 #include "ck_kv.cuh"
 #include "ck_kv_attn.cuh"
+#include "ck_kv_prompt.cuh"
 
 // ---------------------------------------------------------------------------
 // Launches
@@ -38,12 +39,28 @@ size_t kv_pool_bytes(const KvPool& p) {
   return (size_t)p.n_blocks * p.kvh * (p.block / KV_TILE) * kv_record_bytes(p.hd, p.vbits);
 }
 
+#define KV_EACH(X) X(64, 8) X(64, 4) X(128, 8) X(128, 4) X(256, 8) X(256, 4)
+
+static int kv_token_warps(int hd) { return hd == 256 ? KvTok<256, 8>::WARPS : KvTok<128, 8>::WARPS; }
+static_assert(KvTok<64, 8>::WARPS == KvTok<128, 8>::WARPS, "kv_token_warps");
+
+// two partial outputs of 8 heads per share (one per warp of the device); the
+// prefix sums of a launch's queries and the partials' (m, l)
 int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes) {
-  *part_bytes = *ml_bytes = 16;
+  const size_t slots = (size_t)2 * sms * kv_token_warps(p.hd);
+  *part_bytes = slots * 8 * p.hd * sizeof(float);
+  *ml_bytes = (KV_MAXQ + 1) * sizeof(long long) + slots * 8 * sizeof(float2);
   return 0;
 }
 
-cudaError_t kv_setup(const KvPool& p) { return cudaSuccess; }
+cudaError_t kv_setup(const KvPool& p) {
+#define KV_CASE(HD, VB)                                                                                   \
+  if (p.hd == HD && p.vbits == VB)                                                                        \
+    return cudaFuncSetAttribute(k_kv_token<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvTok<HD, VB>::SMEM);
+  KV_EACH(KV_CASE)
+#undef KV_CASE
+  return cudaErrorInvalidValue;
+}
 
 cudaError_t kv_store_launch(const KvStore& a, cudaStream_t s, bool pdl) {
   if (a.n == 0) return cudaSuccess;
@@ -63,7 +80,7 @@ cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
   const dim3 grid((unsigned)((lanes + KV_LOAD_THREADS - 1) / KV_LOAD_THREADS)), block(KV_LOAD_THREADS);
 #define KV_CASE(HD, VB) \
   if (a.pool.hd == HD && a.pool.vbits == VB) return kv_launch(k_kv_load<HD, VB>, grid, block, 0, s, false, a, vec);
-  KV_CASE(64, 8) KV_CASE(64, 4) KV_CASE(128, 8) KV_CASE(128, 4) KV_CASE(256, 8) KV_CASE(256, 4)
+  KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
 }
@@ -73,12 +90,37 @@ static cudaError_t kv_attn_simple(const KvAttn& a, int rows, cudaStream_t s, boo
   const dim3 grid((unsigned)(((long long)rows * a.heads + 3) / 4)), block(128);
 #define KV_CASE(HD, VB) \
   if (a.pool.hd == HD && a.pool.vbits == VB) return kv_launch(k_kv_attn_simple<HD, VB>, grid, block, 0, s, pdl, a);
-  KV_CASE(64, 8) KV_CASE(64, 4) KV_CASE(128, 8) KV_CASE(128, 4) KV_CASE(256, 8) KV_CASE(256, 4)
+  KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
 }
-cudaError_t kv_attend_launch(const KvAttn& a, int sms, cudaStream_t s, bool pdl) {
-  return kv_attn_simple(a, a.n, s, pdl);
+cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pdl) {
+  const int warps = sms * kv_token_warps(all.pool.hd), units = kv_units(all.heads, all.pool.kvh);
+  for (int i0 = 0; i0 < all.n; i0 += KV_MAXQ) {
+    KvAttn a = all;
+    a.n = all.n - i0 < KV_MAXQ ? all.n - i0 : KV_MAXQ;
+    a.len += i0;
+    if (a.seq) a.seq += i0;
+    else if (i0) { a.tab.dev += (size_t)i0 * a.tab.max_blocks; a.tab.n_seqs -= i0; }
+    a.q.p = (char*)a.q.p + (size_t)i0 * a.q.st * 2;
+    a.o.p = (char*)a.o.p + (size_t)i0 * a.o.st * 2;
+    cudaError_t e = cudaErrorInvalidValue;
+#define KV_CASE(HD, VB)                                                                                             \
+  if (a.pool.hd == HD && a.pool.vbits == VB)                                                                        \
+    e = kv_launch(k_kv_token<HD, VB>, dim3(sms), dim3(KvTok<HD, VB>::WARPS * 32), KvTok<HD, VB>::SMEM, s, pdl, a);
+    KV_EACH(KV_CASE)
+#undef KV_CASE
+    if (e != cudaSuccess) return e;
+    // thread groups of the join: about half the partials that a unit has when all are alike
+    int rows = 1;
+    while (rows < KV_JOIN_ROWS && 2 * rows * a.n * units < warps) rows *= 2;
+    const dim3 grid(a.n, a.heads);
+    if (a.pool.hd == 64) e = kv_launch(k_kv_join<64>, grid, dim3(rows < 2 ? 32 : rows * 16), 0, s, true, a, warps);
+    else if (a.pool.hd == 128) e = kv_launch(k_kv_join<128>, grid, dim3(rows * 32), 0, s, true, a, warps);
+    else e = kv_launch(k_kv_join<256>, grid, dim3(rows * 64), 0, s, true, a, warps);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 cudaError_t kv_prompt_launch(const KvAttn& a, int sms, cudaStream_t s) { return kv_attn_simple(a, a.rows, s, false); }
 
