@@ -44,8 +44,12 @@ size_t kv_pool_bytes(const KvPool& p) {
 static int kv_token_warps(int hd) { return hd == 256 ? KvTok<256, 8>::WARPS : KvTok<128, 8>::WARPS; }
 static_assert(KvTok<64, 8>::WARPS == KvTok<128, 8>::WARPS, "kv_token_warps");
 
-// two partial outputs of 8 heads per share (one per warp of the device); the
-// prefix sums of a launch's queries and the partials' (m, l)
+// Workspace.  One token: two partial outputs of 8 heads per share (one per
+// warp of the device), the prefix sums of a launch's queries and the partials'
+// (m, l).  Prompts take no more: a split launch has at most one CTA per SM, of
+// as many rows (16 x sms x 128 for 128 and 256 wide heads, twice that at 64 of
+// which a CTA needs 256), a descriptor of 16 bytes a CTA in the place of the
+// prefix sums.
 int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes) {
   const size_t slots = (size_t)2 * sms * kv_token_warps(p.hd);
   *part_bytes = slots * 8 * p.hd * sizeof(float);
@@ -55,8 +59,13 @@ int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t
 
 cudaError_t kv_setup(const KvPool& p) {
 #define KV_CASE(HD, VB)                                                                                   \
-  if (p.hd == HD && p.vbits == VB)                                                                        \
-    return cudaFuncSetAttribute(k_kv_token<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvTok<HD, VB>::SMEM);
+  if (p.hd == HD && p.vbits == VB) {                                                                      \
+    cudaError_t e = cudaFuncSetAttribute(k_kv_token<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize,  \
+                                         KvTok<HD, VB>::SMEM);                                            \
+    return e != cudaSuccess ? e                                                                           \
+                            : cudaFuncSetAttribute(k_kv_prompt<HD, VB>,                                   \
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB>::SMEM); \
+  }
   KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
@@ -85,15 +94,6 @@ cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-static cudaError_t kv_attn_simple(const KvAttn& a, int rows, cudaStream_t s, bool pdl) {
-  if (rows == 0) return cudaSuccess;
-  const dim3 grid((unsigned)(((long long)rows * a.heads + 3) / 4)), block(128);
-#define KV_CASE(HD, VB) \
-  if (a.pool.hd == HD && a.pool.vbits == VB) return kv_launch(k_kv_attn_simple<HD, VB>, grid, block, 0, s, pdl, a);
-  KV_EACH(KV_CASE)
-#undef KV_CASE
-  return cudaErrorInvalidValue;
-}
 cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pdl) {
   const int warps = sms * kv_token_warps(all.pool.hd), units = kv_units(all.heads, all.pool.kvh);
   for (int i0 = 0; i0 < all.n; i0 += KV_MAXQ) {
@@ -122,7 +122,46 @@ cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pd
   }
   return cudaSuccess;
 }
-cudaError_t kv_prompt_launch(const KvAttn& a, int sms, cudaStream_t s) { return kv_attn_simple(a, a.rows, s, false); }
+cudaError_t kv_prompt_launch(const KvAttn& all, int sms, cudaStream_t s) {
+  if (all.rows == 0) return cudaSuccess;
+  const int gsz = all.heads / all.pool.kvh, hb = (gsz + 127) / 128, gs = (gsz + hb - 1) / hb;   // heads of a unit
+  const int units = all.pool.kvh * hb, bt = (all.pool.hd == 256 ? 128 : 256) / gs, pt = all.pool.hd == 256 ? 64 : 128;
+  for (int i0 = 0; i0 < all.n; i0 += KVP_MAXS) {
+    KvAttn a = all;
+    a.n = all.n - i0 < KVP_MAXS ? all.n - i0 : KVP_MAXS;
+    a.len += i0;
+    a.cu += i0;
+    a.tab.dev += (size_t)i0 * a.tab.max_blocks;
+    a.tab.n_seqs -= i0;
+    // tiles: at most a partial one per sequence.  The cached length is split
+    // when they leave more than half of the SMs idle: what can be split (the
+    // block table's width) into at least 4 position tiles a CTA, as joining
+    // costs about as much as 3 of them
+    const long long ctas = ((long long)a.rows / bt + a.n) * units;
+    const long long tiles = ((long long)a.tab.max_blocks * a.pool.block + pt - 1) / pt;
+    long long splits = ctas ? sms / ctas : 1;
+    if (splits > tiles / 4) splits = tiles / 4;
+    if (splits < 1) splits = 1;
+    if (ctas * splits > 0x7fffffffLL) return cudaErrorInvalidValue;
+    const dim3 grid((unsigned)(ctas * splits));
+    cudaError_t e = cudaErrorInvalidValue;
+#define KV_CASE(HD, VB)                                                                                            \
+  if (a.pool.hd == HD && a.pool.vbits == VB)                                                                       \
+    e = kv_launch(k_kv_prompt<HD, VB>, grid, dim3(KvPr<HD, VB>::THREADS), KvPr<HD, VB>::SMEM, s, false, a, units, gs, \
+                  (int)splits);
+    KV_EACH(KV_CASE)
+#undef KV_CASE
+    if (e != cudaSuccess) return e;
+    if (splits > 1) {
+      const dim3 jg((unsigned)ctas, bt * gs / 8 + (bt * gs % 8 != 0));
+      if (a.pool.hd == 64) e = kv_launch(k_kv_prompt_join<64>, jg, dim3(256), 0, s, true, a, units, gs, (int)splits);
+      else if (a.pool.hd == 128) e = kv_launch(k_kv_prompt_join<128>, jg, dim3(256), 0, s, true, a, units, gs, (int)splits);
+      else e = kv_launch(k_kv_prompt_join<256>, jg, dim3(256), 0, s, true, a, units, gs, (int)splits);
+      if (e != cudaSuccess) return e;
+    }
+  }
+  return cudaSuccess;
+}
 
 // ---------------------------------------------------------------------------
 // Handles

@@ -1,85 +1,618 @@
+// Causal attention of several new tokens per sequence over the quantised
+// paged cache, on tcgen05.
+//
+//   S = scale Q K^T,  P = exp(S - m) under the causal and window mask,
+//   O = P V / sum P;  K and V = code * scale, rounded to 16 bits (an fp16
+//   cache's values), sums in 32 bits in tensor memory.
+//
+// Bound by arithmetic once a sequence has some hundred tokens: per 128 x 128
+// tile of scores at head_dim 128 the two products take 1024 cycles of an SM's
+// tensor pipe, the exponentials 1024 of its special-function units, making K
+// and V from codes about 440 issue slots of each scheduler.  So all four run
+// side by side, on warps of their own:
+//   1 warp    copies records (16 positions of a kv head, one bulk copy each)
+//             through KvPr::STAGES staging buffers
+//   4 or 8    turn codes into fp16 operand tiles (the same arithmetic for both:
+//             V is fed to the second product as it lies, its dims contiguous)
+//   1 thread  issues the products
+//   4 or 8    softmax: a thread owns a query row; it reads S from tensor
+//             memory twice (maximum, then exponentials) and writes P over it
+//             as the second product's operand
+// A CTA holds 256 query rows (two tiles, whose products and softmaxes take
+// turns; the K and V tiles serve both) or, at head_dim 256, 128 rows with two
+// score buffers (the next scores are computed under the present softmax).  A
+// query row is a (token, head of the kv head's group) pair, so the group
+// shares K and V.  O is rescaled only when a row's maximum passes the
+// reference by 2^8.  CTAs are numbered by depth (position of the tile within
+// its sequence), the deepest first: they take longest.
+//
+// Long caches with few rows would leave SMs idle: the cached positions are
+// then split over several CTAs, which leave unnormalised partial rows for
+// k_kv_prompt_join.
 #pragma once
-#include "ck_kv.cuh"
-// Attention over the quantised paged cache, first form: one warp per (query
-// row, head), the cached positions one after another with an online softmax
-// (running maximum and sum, o rescaled when the maximum grows), all in 32
-// bits.  Serves one-token and prompt queries alike.
+#include "ck_kv_attn.cuh"
 
+#define KVP_MAXS 1024        // sequences of one launch
+#define KVP_SLACK 8.f
 
-
-// position and sequence of query row i; false when the row sees nothing
 template <int HD, int VB>
-__global__ void __launch_bounds__(128) k_kv_attn_simple(KvAttn A) {
+struct KvPr {
   using R = KvRec<HD, VB>;
-  constexpr int E = HD / 32;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const int i = (int)(w / A.heads), h = (int)(w % A.heads);
-  pdl_wait();
-  pdl_launch();
-  const int n_rows = A.cu ? A.rows : A.n_dev ? *A.n_dev : A.n;
-  if (i >= n_rows) return;
-  int seq = i, len;
-  if (A.cu) {
-    int lo = 0, hi = A.n;                     // last sequence whose first row is at most i
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (A.cu[mid] <= i) lo = mid; else hi = mid;
+  static constexpr int NQ = HD == 256 ? 1 : 2;            // 128-row query tiles
+  static constexpr int PT = HD == 256 ? 64 : 128;         // positions of a K / V tile
+  static constexpr int SB = NQ == 1 ? 2 : 1;              // score buffers of a query tile
+  static constexpr int SOFT = 4 * NQ, DEQ = 12 - SOFT;    // warps
+  static constexpr int THREADS = (SOFT + DEQ + 2) * 32;
+  static constexpr int RECS = PT / KV_TILE;
+  static constexpr int STAGES = HD == 64 ? 4 : 2;
+  static constexpr int STAGE_BYTES = RECS * R::BYTES;
+  static constexpr int QB = 128 * HD * 2, KB = PT * HD * 2;
+  static constexpr int SQ = 0, SK = NQ * QB, SV = SK + KB, SST = SV + KB;
+  // at least 120 KB, so that an SM holds one CTA (each takes all of its tensor memory)
+  static constexpr int NEED = SST + STAGES * STAGE_BYTES;
+  static constexpr int SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;
+  static constexpr int TO = NQ * SB * PT;                 // tensor memory: score buffers, then O
+  static_assert(TO + NQ * HD <= 512, "tensor memory");
+  static_assert(SMEM <= 227 * 1024 - 1024, "shared memory");
+};
+
+// operand tile of ROWS rows, the contraction running along a row (K-major):
+// core matrices of 8 rows x 16 bytes, the two halves of a 16-wide step 128
+// bytes apart, 8-row groups 256, steps ROWS * 32
+template <int ROWS>
+__device__ __forceinline__ int kvp_kmajor(int row, int k) {
+  return (k >> 4) * (ROWS * 32) + (row >> 3) * 256 + ((k >> 3) & 1) * 128 + (row & 7) * 16 + (k & 7) * 2;
+}
+// V: 16 bytes are 8 dims of a position; core matrices of 8 positions x 16
+// bytes, 8-dim groups 128 bytes apart, 8-position groups HD * 16
+template <int HD>
+__device__ __forceinline__ int kvp_vmajor(int pos, int dim) {
+  return (pos >> 3) * (HD * 16) + (dim >> 3) * 128 + (pos & 7) * 16 + (dim & 7) * 2;
+}
+
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem, uint32_t a, uint64_t db, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+               " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem),
+               "r"(a), "l"(db), "r"(idesc), "r"(acc));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+}
+
+// A value scale that is NaN, or so large that code * scale would pass fp16,
+// must not meet a masked p = 0 in the second product (0 * inf): its values
+// count as zero there, and the position's key becomes NaN, so that exactly the
+// rows that see the position are NaN.
+template <int VB>
+__device__ __forceinline__ bool kvp_bad(uint32_t d) {
+  return (d & 0x7fffu) > (VB == 8 ? 0x6007u : 0x6fffu);      // 515.5 (x 127) and 8188 (x 8)
+}
+
+// Waits for a phase of bar; gives up (false) after a bounded number of polls
+// or when another role of the CTA has given up.  WARP: called by a whole warp,
+// whose lanes get the same answer.
+template <bool WARP>
+__device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* err) {
+  unsigned spins = 0;
+  bool ok = true;
+  while (!mbar_try_wait(bar, parity)) {
+    if (++spins > (1u << 20)) {
+      atomicOr(err, KV_ERR_WAIT);
+      *fail = 1;
+      ok = false;
+      break;
     }
-    seq = lo;
-    len = A.len[seq] - (A.cu[seq + 1] - 1 - i);
-    if (i >= A.cu[A.n]) len = 0;
-  } else {
-    len = A.len[i] + A.len_add;
-    if (A.seq) seq = A.seq[i];
+    if ((spins & 63u) == 0 && *fail) {
+      ok = false;
+      break;
+    }
   }
-  if (len > (long long)A.tab.max_blocks * A.pool.block) {
-    atomicOr(A.pool.err, KV_ERR_POS);
-    len = 0;
-  }
-  const int start = A.window > 0 && len > A.window ? len - A.window : 0;
-  const int kvh = h / (A.heads / A.pool.kvh);
-  float q[E], o[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
-    const size_t off = (size_t)i * A.q.st + (size_t)h * A.q.sh + 32 * e + lane;
-    q[e] = A.q.type == KV_F16 ? __half2float(((const __half*)A.q.p)[off])
-                              : __bfloat162float(((const __nv_bfloat16*)A.q.p)[off]);
-    o[e] = 0.f;
-  }
-  for (int pos = start; pos < len; pos++) {
-    const uint8_t* rec = kv_record(A.pool, A.tab, seq, pos, R::BYTES, kvh);
-    if (!rec) continue;
-    const int p = pos & (KV_TILE - 1);
-    float s = 0.f, v[E];
-#pragma unroll
-    for (int g = 0; g < E; g++) {
-      const float kd = __half2float(*(const __half*)(rec + R::KS + (p * R::G + g) * 2));
-      const float vd = __half2float(*(const __half*)(rec + R::VS + (p * R::G + g) * 2));
-      s += q[g] * (((float)rec[kv_kchunk<HD>(p, g) + lane] - 128.f) * kd);
-      if (VB == 8) {
-        v[g] = ((float)rec[R::V + kv_vchunk<R::VROW>(p, g) + lane] - 128.f) * vd;
-      } else {
-        const uint32_t c = rec[R::V + kv_vchunk<R::VROW>(p, g >> 1) + lane];
-        v[g] = ((float)((c >> (4 * (g & 1))) & 15u) - 8.f) * vd;
+  return WARP ? __all_sync(0xffffffffu, ok) : ok;
+}
+
+template <int HD, int VB>
+__global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A, int units, int gs, int splits) {
+  using C = KvPr<HD, VB>;
+  using R = KvRec<HD, VB>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  __shared__ uint32_t s_tmem;
+  __shared__ volatile int s_fail;
+  __shared__ int s_seq, s_tile;
+  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_k, b_kfree, b_v, b_vfree, b_s[2], b_p[2],
+      b_o, b_pv, b_end;
+  __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 4 ahead)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bt = 128 * C::NQ / gs;             // tokens of a CTA
+  const int unit = blockIdx.x % units, zb = blockIdx.x / units, z = zb % splits, b = zb / splits;
+
+  if (warp == 0) {
+    // tile b, deepest first: D with f(D + 1) <= b < f(D), f(D) = tiles at depth >= D
+    auto depth = [&](int s) {
+      const int r = A.cu[s + 1] - A.cu[s];
+      return r > 0 ? (r + bt - 1) / bt : 0;
+    };
+    auto above = [&](int d) {
+      int c = 0;
+      for (int s = lane; s < A.n; s += 32) c += max(0, depth(s) - d);
+      return __reduce_add_sync(0xffffffffu, c);
+    };
+    int lo = -1, hi = A.rows / bt + 1;         // f(lo) > b >= f(hi)
+    if (above(0) <= b) {
+      hi = -1;
+    } else {
+      lo = 0;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (above(mid) > b) lo = mid; else hi = mid;
       }
     }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    s *= A.scale;
-    const float mn = fmaxf(m, s);
-    const float base = mn == -INFINITY ? 0.f : mn;
-    const float c = expf(m - base), pr = expf(s - base);
-    l = l * c + pr;
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = o[e] * c + pr * v[e];
-    m = mn;
+    int seq = -1;
+    if (hi >= 0) {
+      int k = b - above(lo + 1);               // the k-th sequence with more than lo tiles
+      for (int s0 = 0; s0 < A.n && seq < 0; s0 += 32) {
+        const int s = s0 + lane;
+        const uint32_t has = __ballot_sync(0xffffffffu, s < A.n && depth(s) > lo);
+        const int c = __popc(has);
+        if (k < c) seq = s0 + __fns(has, 0, k + 1);
+        k -= c;
+      }
+    }
+    if (lane == 0) {
+      s_seq = seq;
+      s_tile = lo;
+      s_fail = 0;
+    }
   }
+  __syncthreads();
+  const int seq = s_seq;
+  int4* desc = (int4*)A.ml + b * units + unit;      // splits: what k_kv_prompt_join joins
+  if (seq < 0) {
+    if (splits > 1 && z == 0 && tid == 0) *desc = make_int4(0, 0, 0, 0);
+    return;
+  }
+  const int q0 = A.cu[seq] + s_tile * bt;
+  int ntok = min(bt, A.cu[seq + 1] - q0), len = max(A.len[seq], 0);
+  if (A.cu[seq] < 0 || A.cu[seq + 1] > A.rows || len > A.tab.max_blocks * A.pool.block) {
+    if (tid == 0) atomicOr(A.pool.err, KV_ERR_POS);
+    if (A.cu[seq] < 0 || A.cu[seq + 1] > A.rows) ntok = 0;
+    len = 0;
+  }
+  const int n_new = A.cu[seq + 1] - A.cu[seq];
+  const int pos0 = len - n_new + s_tile * bt;  // cached position of the CTA's first token (may be negative)
+  const int gsz = A.heads / A.pool.kvh, HB = (gsz + gs - 1) / gs, kvh = unit / HB;
+  const int h0 = kvh * gsz + (unit % HB) * gs, nh = min(gs, gsz - (unit % HB) * gs);
+
+  if (splits > 1 && z == 0 && tid == 0) *desc = make_int4(q0, ntok, h0, nh);
+
+  // tiles of positions that query tile w sees: [beg, end)
+  auto range = [&](int w, int& beg, int& end) {
+    const int first = (128 * w) / gs, last = min(ntok, (128 * w + 127) / gs + 1) - 1;   // tokens with a row in it
+    if (first > last) { beg = end = 0; return; }
+    const int plo = pos0 + first, phi = pos0 + last;
+    const int lo = A.window > 0 ? max(0, plo + 1 - A.window) : 0;
+    beg = lo / C::PT;
+    end = len > 0 && phi >= 0 ? phi / C::PT + 1 : beg;
+    if (end < beg) end = beg;
+  };
+  int beg[C::NQ], end[C::NQ], jb = 0x7fffffff, je = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const size_t off = (size_t)i * A.o.st + (size_t)h * A.o.sh + 32 * e + lane;
-    const float r = l == 0.f ? 0.f : o[e] / l;
-    if (A.o.type == KV_F16) ((__half*)A.o.p)[off] = __float2half_rn(r);
-    else ((__nv_bfloat16*)A.o.p)[off] = __float2bfloat16_rn(r);
+  for (int w = 0; w < C::NQ; w++) {
+    range(w, beg[w], end[w]);
+    if (beg[w] < end[w]) { jb = min(jb, beg[w]); je = max(je, end[w]); }
+  }
+  if (jb > je) jb = je;
+  if (splits > 1) {                            // this CTA's share of the tiles
+    const int n = je - jb, a = jb + (int)((long long)n * z / splits), e = jb + (int)((long long)n * (z + 1) / splits);
+    jb = a;
+    je = e;
+#pragma unroll
+    for (int w = 0; w < C::NQ; w++) {
+      beg[w] = max(beg[w], jb);
+      end[w] = max(min(end[w], je), beg[w]);
+    }
+  }
+
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < C::STAGES; i++) {
+      mbar_init(&b_full[i], 1);
+      mbar_init(&b_empty[i], C::DEQ);
+    }
+    mbar_init(&b_k, C::DEQ * 32);
+    mbar_init(&b_v, C::DEQ * 32);
+    mbar_init(&b_kfree, 1);
+    mbar_init(&b_vfree, 1);
+    mbar_init(&b_s[0], 1);
+    mbar_init(&b_s[1], 1);
+    mbar_init(&b_p[0], 128);
+    mbar_init(&b_p[1], 128);
+    mbar_init(&b_o, 1);
+    mbar_init(&b_pv, 1);
+    mbar_init(&b_end, 1);
+    mbar_fence_init();
+  }
+  // Q: each softmax thread its own row, brought to a power of two near 1 (see
+  // ck_kv_attn.cuh), 16 bits
+  float sc = 0.f;
+  const int wq = warp >> 2, rl = 32 * (warp & 3) + lane;    // query tile and row of a softmax thread
+  const int rr = 128 * wq + rl, rtok = rr / gs, rhead = rr % gs;
+  const bool rlive = warp < C::SOFT && rtok < ntok && rhead < nh;
+  if (warp < C::SOFT) {
+    const unsigned short* p = (const unsigned short*)A.q.p + (size_t)(q0 + rtok) * A.q.st + (size_t)(h0 + rhead) * A.q.sh;
+    const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
+    auto load8 = [&](int d, float (&f)[8]) {
+      uint32_t x[4] = {0u, 0u, 0u, 0u};
+      if (rlive) {
+        if (vec) {
+          const uint4 v = *(const uint4*)(p + d);
+          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = p[d + 2 * e] | ((uint32_t)p[d + 2 * e + 1] << 16);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float2 y = A.q.type == KV_F16 ? __half22float2(*(const __half2*)&x[e])
+                                            : make_float2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u));
+        f[2 * e] = y.x;
+        f[2 * e + 1] = y.y;
+      }
+    };
+    float top = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 8) {
+      float f[8];
+      load8(d, f);
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[e]));
+    }
+    int e = (int)(__float_as_uint(top) >> 23) - 127;
+    e = e > 127 ? 8 : max(e, -100);
+    // (the scale's sign goes to q: the largest product is the largest score)
+    const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
+    sc = fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23);
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 8) {
+      float f[8];
+      load8(d, f);
+      const uint4 v = make_uint4(kv_pack2(f[0] * up, f[1] * up), kv_pack2(f[2] * up, f[3] * up),
+                                 kv_pack2(f[4] * up, f[5] * up), kv_pack2(f[6] * up, f[7] * up));
+      *(uint4*)(sm + C::SQ + wq * C::QB + kvp_kmajor<128>(rl, d)) = v;
+    }
+    proxy_fence_smem();
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = s_tmem;
+  const int bpt = A.pool.block / KV_TILE;
+
+  if (warp == C::SOFT + C::DEQ + 1) {
+    // ---- copies: lane i fetches record i of the tile ----
+    for (int j = jb; j < je; j++) {
+      const int it = j - jb, s = it % C::STAGES;
+      if (it >= C::STAGES && !kvp_wait<true>(&b_empty[s], (it / C::STAGES - 1) & 1, &s_fail, A.pool.err)) break;
+      const int tile = j * C::RECS + lane;     // record of the sequence
+      bool ok = lane < C::RECS && tile * KV_TILE < len;
+      int id = 0;
+      if (ok) {
+        id = A.tab.dev[(size_t)seq * A.tab.max_blocks + tile / bpt];
+        ok = (unsigned)id < (unsigned)A.pool.n_blocks;
+        if (!ok) atomicOr(A.pool.err, KV_ERR_BLOCK);
+      }
+      const uint32_t have = __ballot_sync(0xffffffffu, ok);
+      uint8_t* dst = sm + C::SST + s * C::STAGE_BYTES + lane * R::BYTES;
+      // a record that does not exist: zero scales (its values meet p = 0) and
+      // a mark for the softmax
+      if (lane < C::RECS && !ok) {
+        for (int i = R::KS; i < R::BYTES; i += 4) *(uint32_t*)(dst + i) = 0u;
+        proxy_fence_smem();
+      }
+      if (lane == 0) s_miss[j & 7] = ~have & ((1u << C::RECS) - 1);
+      __syncwarp();
+      if (lane == 0) mbar_expect_tx(&b_full[s], __popc(have) * R::BYTES);
+      __syncwarp();
+      if (ok)
+        bulk_g2s(dst, A.pool.base + (((size_t)id * A.pool.kvh + kvh) * bpt + tile % bpt) * R::BYTES, R::BYTES,
+                 &b_full[s]);
+    }
+    if (s_fail)                                // no copy may land after the CTA has gone
+      for (int s = 0; s < min(C::STAGES, je - jb); s++)
+        for (unsigned spins = 0; !mbar_try_wait(&b_full[s], 0) && !mbar_try_wait(&b_full[s], 1) && spins < (1u << 20); spins++) {}
+  } else if (warp == C::SOFT + C::DEQ) {
+    // ---- products ----
+    if (lane == 0) {
+      const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
+      const uint32_t idO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);   // V's dims are contiguous
+      bool ok = true;
+      auto scores = [&](int w, int buf) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; k++)
+          umma_f16(tmem + buf * C::PT, umma_desc(smem_u32(sm + C::SQ + w * C::QB + k * 4096), 128, 256),
+                   umma_desc(smem_u32(sm + C::SK + k * C::PT * 32), 128, 256), idS, k > 0 ? 1u : 0u);
+        umma_commit(&b_s[buf]);
+      };
+      auto output = [&](int w, int buf, bool first) {
+#pragma unroll
+        for (int k = 0; k < C::PT / 16; k++)
+          umma_f16_ts(tmem + C::TO + w * HD, tmem + buf * C::PT + 8 * k,
+                      umma_desc(smem_u32(sm + C::SV + k * 2 * HD * 16), HD * 16, 128), idO, first && k == 0 ? 0u : 1u);
+      };
+      if (C::NQ == 2) {
+        for (int j = jb; ok && j <= je; j++) {
+          bool kw = false, vw = false;
+          for (int w = 0; ok && w < C::NQ; w++) {
+            if (j - 1 >= beg[w] && j - 1 < end[w]) {          // O += P V of the tile before
+              if (!vw) ok = kvp_wait<false>(&b_v, (j - 1 - jb) & 1, &s_fail, A.pool.err);
+              vw = true;
+              ok = ok && kvp_wait<false>(&b_p[w], (j - 1 - beg[w]) & 1, &s_fail, A.pool.err);
+              if (!ok) break;
+              asm volatile("tcgen05.fence::after_thread_sync;");
+              output(w, w, j - 1 == beg[w]);
+            }
+            if (j < je && j >= beg[w] && j < end[w]) {
+              if (!kw) ok = kvp_wait<false>(&b_k, (j - jb) & 1, &s_fail, A.pool.err);
+              kw = true;
+              if (!ok) break;
+              asm volatile("tcgen05.fence::after_thread_sync;");
+              scores(w, w);
+            }
+          }
+          if (!ok) break;
+          if (j > jb) umma_commit(&b_vfree);
+          if (j < je) umma_commit(&b_kfree);
+        }
+      } else {
+        const int n = je - jb;
+        for (int j = 0; ok && j <= n; j++) {
+          if (j < n) {                                        // the next scores before this tile's output
+            ok = kvp_wait<false>(&b_k, j & 1, &s_fail, A.pool.err);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            scores(0, j & 1);
+            umma_commit(&b_kfree);
+          }
+          if (j > 0) {
+            ok = kvp_wait<false>(&b_v, (j - 1) & 1, &s_fail, A.pool.err) &&
+                 kvp_wait<false>(&b_p[(j - 1) & 1], ((j - 1) >> 1) & 1, &s_fail, A.pool.err);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            output(0, (j - 1) & 1, j == 1);
+            umma_commit(&b_vfree);
+            umma_commit(&b_pv);
+          }
+        }
+      }
+      umma_commit(&b_o);
+    }
+  } else if (warp >= C::SOFT) {
+    // ---- K and V from codes ----
+    const int dw = warp - C::SOFT;
+    bool ok = true;
+    for (int j = jb; ok && j < je; j++) {
+      const int it = j - jb, s = it % C::STAGES;
+      const uint8_t* stg = sm + C::SST + s * C::STAGE_BYTES;
+      ok = kvp_wait<true>(&b_full[s], (it / C::STAGES) & 1, &s_fail, A.pool.err) &&
+           (it == 0 || kvp_wait<true>(&b_kfree, (it - 1) & 1, &s_fail, A.pool.err));
+      if (!ok) break;
+      // an item is 8 positions x 64 dims: lane = position & 7 and 16 of the dims
+#pragma unroll 2
+      for (int i = dw; i < C::PT / 8 * (HD / 64); i += C::DEQ) {
+        const int p = (i / (HD / 64)) * 8 + (lane & 7), x = lane >> 3, g = (i % (HD / 64)) * 2 + (x >> 1);
+        const int half = (x & 1) ^ ((lane >> 2) & 1);       // rows 4 apart share their banks: they take the other half
+        const uint8_t* rec = stg + (p >> 4) * R::BYTES;
+        const uint4 c = *(const uint4*)(rec + kv_kchunk<HD>(p & 15, g) + 16 * half);
+        uint32_t du = *(const unsigned short*)(rec + R::KS + ((p & 15) * R::G + g) * 2);
+        if (kvp_bad<VB>(*(const unsigned short*)(rec + R::VS + ((p & 15) * R::G + g) * 2))) du = 0x7fffu;
+        du |= du << 16;
+        uint8_t* dst = sm + C::SK + kvp_kmajor<C::PT>(p, 32 * g + 16 * half);
+        *(uint4*)dst = make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c.x), du), kv_hmul2(kv_half2<0x4342, 128>(c.x), du),
+                                  kv_hmul2(kv_half2<0x4140, 128>(c.y), du), kv_hmul2(kv_half2<0x4342, 128>(c.y), du));
+        *(uint4*)(dst + 128) =
+            make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c.z), du), kv_hmul2(kv_half2<0x4342, 128>(c.z), du),
+                       kv_hmul2(kv_half2<0x4140, 128>(c.w), du), kv_hmul2(kv_half2<0x4342, 128>(c.w), du));
+      }
+      proxy_fence_smem();
+      mbar_arrive(&b_k);
+      if (it > 0 && !kvp_wait<true>(&b_vfree, (it - 1) & 1, &s_fail, A.pool.err)) break;
+      constexpr int CH = R::VROW / 32, CP = CH < 2 ? 1 : CH / 2;   // 32-byte chunks of a position; pairs of them
+      // items: 8 positions x 2 chunks, or 16 positions of a single chunk
+#pragma unroll 2
+      for (int i = dw; i < (CH < 2 ? C::PT / 16 : C::PT / 8 * CP); i += C::DEQ) {
+        const int x = lane >> 3;
+        const int p = CH < 2 ? i * 16 + (x >> 1) * 8 + (lane & 7) : (i / CP) * 8 + (lane & 7);
+        const int c = CH < 2 ? 0 : (i % CP) * 2 + (x >> 1);
+        const int half = x & 1;
+        const uint8_t* rec = stg + (p >> 4) * R::BYTES;
+        const uint4 w = *(const uint4*)(rec + R::V + kv_vchunk<R::VROW>(p & 15, c) + 16 * half);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
+          const int g = VB == 8 ? c : 2 * c + nib;
+          uint32_t d = *(const unsigned short*)(rec + R::VS + ((p & 15) * R::G + g) * 2);
+          if (kvp_bad<VB>(d) || j * C::PT + p >= len) d = 0;
+          d |= d << 16;
+          constexpr int BIAS = VB == 8 ? 128 : 8;
+          uint32_t o[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t u = VB == 8 ? ww[e] : (ww[e] >> (4 * nib)) & 0x0f0f0f0fu;
+            o[2 * e] = kv_hmul2(kv_half2<0x4140, BIAS>(u), d);
+            o[2 * e + 1] = kv_hmul2(kv_half2<0x4342, BIAS>(u), d);
+          }
+          uint8_t* dst = sm + C::SV + kvp_vmajor<HD>(p, 32 * g + 16 * half);
+          *(uint4*)dst = make_uint4(o[0], o[1], o[2], o[3]);
+          *(uint4*)(dst + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
+      proxy_fence_smem();
+      mbar_arrive(&b_v);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b_empty[s]);
+    }
+  } else {
+    // ---- softmax ----
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const int rpos = pos0 + rtok;                                 // position of the row's token
+    const int rlo = A.window > 0 ? max(0, rpos + 1 - A.window) : 0;
+    float m = -INFINITY, l = 0.f;
+    const uint32_t tO = tmem + C::TO + wq * HD + lanes;
+    bool ok = true;
+    for (int j = beg[wq]; ok && j < end[wq]; j++) {
+      const int it = j - beg[wq], buf = C::SB == 2 ? it & 1 : wq, ph = C::SB == 2 ? (it >> 1) & 1 : it & 1;
+      const uint32_t tS = tmem + buf * C::PT + lanes;
+      const int vlo = rlo - j * C::PT, vhi = rlive ? rpos - j * C::PT : -1;   // visible columns: vlo .. vhi
+      ok = kvp_wait<true>(&b_s[buf], ph, &s_fail, A.pool.err);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      const uint32_t miss = s_miss[j & 7];
+      const bool edge = __any_sync(0xffffffffu, vlo > 0 || vhi < C::PT - 1 || miss != 0);
+      // visible ones of the 32 columns from c on
+      auto seen = [&](int c) {
+        const int lo = max(vlo - c, 0), hi = min(vhi - c, 31);
+        uint32_t v = lo > hi ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+        if ((miss >> (c >> 4)) & 1) v &= 0xffff0000u;
+        if ((miss >> ((c >> 4) + 1)) & 1) v &= 0x0000ffffu;
+        return v;
+      };
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < C::PT; c += 32) {
+        uint32_t x[32];
+        tmem_ld32(tS + c, x);
+        if (edge) {
+          const uint32_t v = seen(c);
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if ((v >> e) & 1) mx = fmaxf(mx, __uint_as_float(x[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(x[e]));
+        }
+      }
+      mx = mx == -INFINITY ? mx : mx * sc;
+      if (__any_sync(0xffffffffu, mx > m + KVP_SLACK)) {
+        const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
+        m = mn;
+        l *= a;
+        if (it > 0) {
+          if (C::SB == 2) ok = kvp_wait<true>(&b_pv, (it - 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t x[32];
+            tmem_ld32(tO + c, x);
+#pragma unroll
+            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * a);
+            tmem_st32(tO + c, x);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+      }
+      const float mb = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+      for (int c = 0; c < C::PT; c += 32) {
+        uint32_t x[32], y[16];
+        tmem_ld32(tS + c, x);
+        const uint32_t v = edge ? seen(c) : 0xffffffffu;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          float p0 = kv_ex2(fmaf(__uint_as_float(x[2 * e]), sc, -mb)), p1 = kv_ex2(fmaf(__uint_as_float(x[2 * e + 1]), sc, -mb));
+          if (edge) {
+            if (!((v >> (2 * e)) & 1)) p0 = 0.f;
+            if (!((v >> (2 * e + 1)) & 1)) p1 = 0.f;
+          }
+          l += p0 + p1;
+          y[e] = kv_pack2(p0, p1);
+        }
+        tmem_st16(tS + c / 2, y);                                 // behind what this thread still has to read
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      asm volatile("tcgen05.fence::before_thread_sync;");
+      mbar_arrive(&b_p[buf]);
+    }
+    // O / l, or this CTA's part of it
+    if (ok && beg[wq] < end[wq]) ok = kvp_wait<true>(&b_o, 0, &s_fail, A.pool.err);
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    if (ok) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const size_t off = (size_t)(q0 + rtok) * A.o.st + (size_t)(h0 + rhead) * A.o.sh;
+      const bool vec = kv_vec4(A.o);
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t x[32];
+        if (beg[wq] < end[wq]) {
+          tmem_ld32(tO + c, x);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; e++) x[e] = 0u;
+        }
+        if (splits > 1) {
+          float* part = A.part + (((size_t)(b * units + unit) * splits + z) * (128 * C::NQ) + rr) * HD + c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) *(uint4*)(part + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        } else if (rlive) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            kv_st4(A.o, off + c + e,
+                   l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                            : make_float4(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv,
+                                          __uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv),
+                   vec);
+        }
+      }
+      if (splits > 1)
+        ((float2*)((long long*)A.ml + KV_MAXQ + 1))[((size_t)(b * units + unit) * splits + z) * (128 * C::NQ) + rr] =
+            make_float2(m, l);
+    }
+  }
+  // no CTA leaves, or frees its tensor memory, with a product in flight
+  __syncthreads();
+  if (warp == C::SOFT + C::DEQ && lane == 0) umma_commit(&b_end);
+  if (warp == 0) {
+    unsigned spins = 0;
+    while (!mbar_try_wait(&b_end, 0) && ++spins < (1u << 20)) {}
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// Adds the parts of a split tile: one warp per query row.
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv_prompt_join(KvAttn A, int units, int gs, int splits) {
+  constexpr int ROWS = HD == 256 ? 128 : 256, E = HD / 32;
+  pdl_wait();
+  const int4 d = ((const int4*)A.ml)[blockIdx.x];
+  const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), tok = row / gs, head = row % gs;
+  if (tok >= d.y || head >= d.w) return;
+  const float2* ml = (const float2*)((const long long*)A.ml + KV_MAXQ + 1);
+  float M = -INFINITY, l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) o[e] = 0.f;
+  for (int z = 0; z < splits; z++) M = fmaxf(M, ml[((size_t)blockIdx.x * splits + z) * ROWS + row].x);
+  const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+  for (int z = 0; z < splits; z++) {
+    const size_t at = ((size_t)blockIdx.x * splits + z) * ROWS + row;
+    const float2 e = ml[at];
+    const float w = kv_ex2(e.x - base);
+    l += w * e.y;
+#pragma unroll
+    for (int i = 0; i < E; i++) o[i] += w * A.part[at * HD + 32 * i + lane];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const size_t off = (size_t)(d.x + tok) * A.o.st + (size_t)(d.z + head) * A.o.sh + lane;
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    if (A.o.type == KV_F16) ((__half*)A.o.p)[off + 32 * i] = __float2half_rn(o[i] * inv);
+    else ((__nv_bfloat16*)A.o.p)[off + 32 * i] = __float2bfloat16_rn(o[i] * inv);
   }
 }
