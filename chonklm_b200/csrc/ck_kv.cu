@@ -39,10 +39,19 @@ size_t kv_pool_bytes(const KvPool& p) {
   return (size_t)p.n_blocks * p.kvh * (p.block / KV_TILE) * kv_record_bytes(p.hd, p.vbits);
 }
 
+#ifndef KV_UNIT_PAIRS
+#define KV_UNIT_PAIRS 32
+#endif
+
 #define KV_EACH(X) X(64, 8) X(64, 4) X(128, 8) X(128, 4) X(256, 8) X(256, 4)
 
-static int kv_token_warps(int hd) { return hd == 256 ? KvTok<256, 8>::WARPS : KvTok<128, 8>::WARPS; }
-static_assert(KvTok<64, 8>::WARPS == KvTok<128, 8>::WARPS, "kv_token_warps");
+// warps of an SM in the form by list
+static int kv_token_warps(int hd, int vb) {
+#define KV_CASE(HD, VB) if (hd == HD && vb == VB) return KvTok<HD, VB>::WARPS;
+  KV_EACH(KV_CASE)
+#undef KV_CASE
+  return 0;
+}
 
 // Workspace.  One token: two partial outputs of 8 heads per share (one per
 // warp of the device), the prefix sums of a launch's queries and the partials'
@@ -51,21 +60,40 @@ static_assert(KvTok<64, 8>::WARPS == KvTok<128, 8>::WARPS, "kv_token_warps");
 // which a CTA needs 256), a descriptor of 16 bytes a CTA in the place of the
 // prefix sums.
 int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes) {
-  const size_t slots = (size_t)2 * sms * kv_token_warps(p.hd);
+  const size_t slots = (size_t)sms * (p.hd == 256 ? 16 : 32);
   *part_bytes = slots * 8 * p.hd * sizeof(float);
-  *ml_bytes = (KV_MAXQ + 1) * sizeof(long long) + slots * 8 * sizeof(float2);
+  *ml_bytes = KV_PRE * sizeof(long long) + slots * 8 * sizeof(float2);
   return 0;
 }
 
-cudaError_t kv_setup(const KvPool& p) {
-#define KV_CASE(HD, VB)                                                                                   \
-  if (p.hd == HD && p.vbits == VB) {                                                                      \
-    cudaError_t e = cudaFuncSetAttribute(k_kv_token<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize,  \
-                                         KvTok<HD, VB>::SMEM);                                            \
-    return e != cudaSuccess ? e                                                                           \
-                            : cudaFuncSetAttribute(k_kv_prompt<HD, VB>,                                   \
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB>::SMEM); \
+// the forms of k_kv_token
+template <int HD, int VB>
+struct KvForms {
+  using C = KvTok<HD, VB>;
+  static constexpr auto list = k_kv_token<HD, VB, false, C::WARPS, C::STAGES>;
+  // by unit: 4 warps where the units fill the device, else 8
+  static constexpr int ST4 = HD == 256 ? 1 : 2, ST8 = HD == 256 ? 1 : 2;
+  static constexpr auto unit4 = k_kv_token<HD, VB, true, 4, ST4>;
+  static constexpr auto unit8 = k_kv_token<HD, VB, true, 8, ST8>;
+  static constexpr int SMEM4 = 4 * ST4 * C::PAIR_BYTES, SMEM8 = 8 * ST8 * C::PAIR_BYTES;
+  static cudaError_t setup() {
+    cudaError_t e = cudaFuncSetAttribute(list, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(unit4, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM4);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(unit8, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM8);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB>::SMEM);
+    return e;
   }
+  // form: warps of a unit's CTA, or 0 for the list
+  static cudaError_t launch(int form, const KvAttn& a, int units, int sms, cudaStream_t s, bool pdl) {
+    if (form == 4) return kv_launch(unit4, dim3(a.n * units), dim3(128), SMEM4, s, pdl, a);
+    if (form == 8) return kv_launch(unit8, dim3(a.n * units), dim3(256), SMEM8, s, pdl, a);
+    return kv_launch(list, dim3(sms), dim3(C::WARPS * 32), C::SMEM, s, pdl, a);
+  }
+};
+
+cudaError_t kv_setup(const KvPool& p) {
+#define KV_CASE(HD, VB) if (p.hd == HD && p.vbits == VB) return KvForms<HD, VB>::setup();
   KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
@@ -95,7 +123,7 @@ cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
 }
 
 cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pdl) {
-  const int warps = sms * kv_token_warps(all.pool.hd), units = kv_units(all.heads, all.pool.kvh);
+  const int warps = sms * kv_token_warps(all.pool.hd, all.pool.vbits), units = kv_units(all.heads, all.pool.kvh);
   for (int i0 = 0; i0 < all.n; i0 += KV_MAXQ) {
     KvAttn a = all;
     a.n = all.n - i0 < KV_MAXQ ? all.n - i0 : KV_MAXQ;
@@ -104,20 +132,26 @@ cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pd
     else if (i0) { a.tab.dev += (size_t)i0 * a.tab.max_blocks; a.tab.n_seqs -= i0; }
     a.q.p = (char*)a.q.p + (size_t)i0 * a.q.st * 2;
     a.o.p = (char*)a.o.p + (size_t)i0 * a.o.st * 2;
+    // by unit when none has more than KV_UNIT_PAIRS pairs (the block table's
+    // width and the window bound them)
+    long long pairs = ((long long)a.tab.max_blocks * a.pool.block + KV_PAIR - 1) / KV_PAIR;
+    if (a.window > 0 && pairs > a.window / KV_PAIR + 2) pairs = a.window / KV_PAIR + 2;
+    const int form = pairs > KV_UNIT_PAIRS ? 0 : a.n * units >= 2 * sms ? 4 : 8;
     cudaError_t e = cudaErrorInvalidValue;
-#define KV_CASE(HD, VB)                                                                                             \
-  if (a.pool.hd == HD && a.pool.vbits == VB)                                                                        \
-    e = kv_launch(k_kv_token<HD, VB>, dim3(sms), dim3(KvTok<HD, VB>::WARPS * 32), KvTok<HD, VB>::SMEM, s, pdl, a);
+#define KV_CASE(HD, VB) \
+  if (a.pool.hd == HD && a.pool.vbits == VB) e = KvForms<HD, VB>::launch(form, a, units, sms, s, pdl);
     KV_EACH(KV_CASE)
 #undef KV_CASE
     if (e != cudaSuccess) return e;
+    if (form) continue;
     // thread groups of the join: about half the partials that a unit has when all are alike
-    int rows = 1;
-    while (rows < KV_JOIN_ROWS && 2 * rows * a.n * units < warps) rows *= 2;
-    const dim3 grid(a.n, a.heads);
-    if (a.pool.hd == 64) e = kv_launch(k_kv_join<64>, grid, dim3(rows < 2 ? 32 : rows * 16), 0, s, true, a, warps);
-    else if (a.pool.hd == 128) e = kv_launch(k_kv_join<128>, grid, dim3(rows * 32), 0, s, true, a, warps);
-    else e = kv_launch(k_kv_join<256>, grid, dim3(rows * 64), 0, s, true, a, warps);
+    const int most = 1024 / (a.pool.hd / 4);
+    int rows = a.pool.hd == 64 ? 2 : 1;
+    while (rows < most && 2 * rows * a.n * units < warps) rows *= 2;
+    const dim3 grid(a.n, a.heads), block(rows * a.pool.hd / 4);
+    if (a.pool.hd == 64) e = kv_launch(k_kv_join<64>, grid, block, 0, s, true, a, warps);
+    else if (a.pool.hd == 128) e = kv_launch(k_kv_join<128>, grid, block, 0, s, true, a, warps);
+    else e = kv_launch(k_kv_join<256>, grid, block, 0, s, true, a, warps);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -290,6 +324,7 @@ int ck_kv_create(const ck_kv_cfg* cfg, int device, ck_kv** out) {
   if (e != cudaSuccess) return bail(CK_ECUDA, "device", e);
   size_t pb = 0, mb = 0;
   kv_workspace(p, cfg->heads, h->sms, &pb, &mb);
+
   if ((e = cudaMalloc(&p.base, kv_pool_bytes(p))) != cudaSuccess || (e = cudaMalloc(&p.err, 16)) != cudaSuccess ||
       (e = cudaMalloc(&h->part, pb)) != cudaSuccess || (e = cudaMalloc(&h->ml, mb)) != cudaSuccess)
     return bail(CK_ENOMEM, "cudaMalloc", e);

@@ -64,7 +64,7 @@ struct KvAttn {
   int heads, window;
   float scale;
   KvRows q, o;
-  float *part, *ml;          // token form: partial outputs and their (maximum, sum)
+  float *part, *ml;          // partial outputs; prefix sums and the partials' (maximum, sum)
 };
 
 int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes);

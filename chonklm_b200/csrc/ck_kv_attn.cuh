@@ -3,41 +3,70 @@
 //   s_j = scale * sum_g dk[j][g] * (q_g . ck[j][g])      (codes c, scales d per group g of 32)
 //   o   = sum_j exp(s_j - m) * dv[j][g] * cv[j][g] / sum_j exp(s_j - m)
 //
-// Bound by the cache's bytes.  The visible 16-position records of all
-// (query, kv head) units form one list, cut into equal shares, one per warp of
-// the device: ragged lengths balance by themselves, one long sequence spreads
-// over every SM, and no length is needed on the host.  A warp keeps KV_STAGES
-// records in flight in its own part of shared memory (one cp.async.bulk each,
-// completing on the warp's mbarriers); warps never wait for one another.  A
-// unit that lies in one share is finished by its warp; the others leave
-// unnormalised partial outputs with their (m, l), which k_kv_join adds in the
-// order of the shares (no atomics: the result does not depend on timing).
+// Bound by the cache's bytes (and, close behind, by the instructions that turn
+// codes into operands).  A unit is one query's up to 8 heads of one kv head;
+// they share every record that is read.  A warp takes pairs of 16-position
+// records, keeps several pairs in flight in its own part of shared memory (one
+// cp.async.bulk per record, completing on the warp's mbarriers) and waits for
+// no other warp.  Two ways to hand out the pairs:
+//   by list   all units' visible pairs form one list, cut into equal shares,
+//             one per warp of the device: ragged lengths balance by
+//             themselves, one long sequence spreads over every SM, and no
+//             length is needed on the host.  A unit that lies in one share is
+//             finished by its warp; the others leave unnormalised partial
+//             outputs with their (m, l), which k_kv_join adds in the order of
+//             the shares (no atomics: the result does not depend on timing).
+//   by unit   short caches: one CTA per unit, its warps' parts added through
+//             shared memory; one launch.
 //
-// The up to 8 query heads of a unit share every record that is read: products
-// run on m16n8k16 tensor instructions (a unit has 8 rows, too few for
-// tcgen05's 64-row tiles).  S = Q K^T has the heads as rows and 8 positions as
-// columns; key codes become fp16 exactly (0x6400 | byte is 1024 + byte) and
-// each group's sum is multiplied by its scale in 32 bits.  O^T = V^T P^T has
-// the dims as rows and the heads as columns, and S's accumulator layout is
-// just P^T's operand layout, so P never leaves its registers.  Rounded to 16
-// bits: p = exp(s - m) (11 bits; l sums the unrounded p) and a value
-// code * scale (11 bits, as an fp16 cache would hold it).
+// Products run on m16n8k16 tensor instructions (a unit has 8 rows, too few for
+// tcgen05's 64-row tiles), the heads as the 8 columns: S^T = K Q^T with 16
+// positions as rows, O^T = V^T P^T with 16 dims as rows (P^T from S^T's
+// accumulators by one 8x8 transposition in registers).  A key's byte c + 128
+// is taken as the fp16 number (c + 128) 2^-24 (its bits as they are),
+// -128 2^-24 sum(q) is where the sum begins, and each group's sum is
+// multiplied by its scale in 32 bits.  A value's byte becomes fp16 by
+// 0x6400 | byte = 1024 + byte.  Rounded to 16 bits: p = exp(s - m)
+// (11 bits; l sums the unrounded p) and a value code * scale (11 bits, as an
+// fp16 cache would hold it).
 #pragma once
 #include "ck_kv.cuh"
 
 #define KV_MAXQ 1024         // queries of one launch (their prefix sums sit in shared memory)
+#define KV_PRE (KV_MAXQ + 2) // their place in the workspace (keeps what follows 16-byte aligned)
+#define KV_PAIR 32           // positions of a pair of records
 #define KV_SLACK 6.f         // log2 that a score may exceed the reference maximum before o is rescaled
 #define KV_BOOST 8.f         // p is kept times 2^8 (cancelled by l), so that small p stay normal fp16 numbers
 
+#ifndef KVW64
+#define KVW64 16
+#endif
+#ifndef KVW128
+#define KVW128 12
+#endif
+// by list: one CTA per SM; the warps that the registers allow (accumulators:
+// head_dim / 4 a thread) and the pairs that fit 209 KB
 template <int HD, int VB>
 struct KvTok {
-  // 16 warps of up to 128 registers; 8 at head_dim 256, whose accumulators
-  // take 64.  Stages: what fits 209 KB.
-  static constexpr int WARPS = HD == 256 ? 8 : 16;
-  static constexpr int STAGES = HD == 256 ? 3 : HD == 128 ? 3 : 6;
-  static constexpr int SMEM = WARPS * STAGES * KvRec<HD, VB>::BYTES;
+  static constexpr int WARPS = HD == 256 ? (VB == 8 ? 6 : 8) : HD == 128 ? KVW128 : KVW64;
+  static constexpr int PAIR_BYTES = 2 * KvRec<HD, VB>::BYTES;
+  static constexpr int FIT = 209 * 1024 / WARPS / PAIR_BYTES, STAGES = FIT > 4 ? 4 : FIT;
+  static constexpr int SMEM = WARPS * STAGES * PAIR_BYTES;
 };
 
+// d = a b + c
+__device__ __forceinline__ void kv_mma_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                            uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// transposes an 8x8 matrix of 16-bit elements, two of a row in each thread
+__device__ __forceinline__ uint32_t kv_transpose(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ void kv_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -51,6 +80,22 @@ __device__ __forceinline__ uint32_t kv_half2(uint32_t w) {
   const __half2 h = __hsub2(*(const __half2*)&u, __half2half2(__ushort_as_half((unsigned short)(0x6400 + BIAS))));
   return *(const uint32_t*)&h;
 }
+// codes of an fp16 pair 1024 + byte: byte - 128, or nibble - 8 of 4 bits (the
+// low ones, or the high ones as (1024 + 16 x) / 16 - 72)
+template <int VB>
+__device__ __forceinline__ uint32_t kv_code2(uint32_t h, int nib) {
+  __half2 v;
+  if (VB == 8) {
+    v = __hsub2(*(const __half2*)&h, __half2half2(__ushort_as_half(0x6480)));
+  } else if (nib == 0) {
+    const uint32_t x = h & 0xff0fff0fu;
+    v = __hsub2(*(const __half2*)&x, __half2half2(__ushort_as_half(0x6408)));
+  } else {
+    const uint32_t x = h & 0xfff0fff0u;
+    v = __hfma2(*(const __half2*)&x, __half2half2(__ushort_as_half(0x2c00)), __half2half2(__ushort_as_half(0xd480)));
+  }
+  return *(const uint32_t*)&v;
+}
 __device__ __forceinline__ uint32_t kv_hmul2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
   return *(const uint32_t*)&h;
@@ -59,15 +104,23 @@ __device__ __forceinline__ uint32_t kv_pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *(const uint32_t*)&h;
 }
+// two neighbouring 16-bit elements
+__device__ __forceinline__ float2 kv_pair16(uint32_t x, int type) {
+  return type == KV_F16 ? __half22float2(*(const __half2*)&x)
+                        : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
 __device__ __forceinline__ float kv_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// fp16 scales of two neighbouring positions, all groups: [2][HD/32] halves
+// fp16 scales, all groups: of one position (W = HD / 64 words) or of two
+// neighbouring ones
 template <int W>
 __device__ __forceinline__ void kv_lds(const uint8_t* p, uint32_t (&u)[W]) {
-  if (W == 2) {
+  if (W == 1) {
+    u[0] = *(const uint32_t*)p;
+  } else if (W == 2) {
     const uint2 x = *(const uint2*)p;
     u[0] = x.x; u[1] = x.y;
   } else {
@@ -84,11 +137,11 @@ __device__ __forceinline__ uint32_t kv_scale_pair(const uint32_t (&u)[W], int g)
   return __byte_perm(u[g >> 1], u[G / 2 + (g >> 1)], (g & 1) ? 0x7632 : 0x5410);
 }
 
-// visible records of a query: first record and their number
-__device__ __forceinline__ int kv_tiles(int len, int window, int& t0) {
+// visible pairs of records of a query: the first one and their number
+__device__ __forceinline__ int kv_pairs(int len, int window, int& t0) {
   const int lo = window > 0 && len > window ? len - window : 0;
-  t0 = lo / KV_TILE;
-  return len > 0 ? (len + KV_TILE - 1) / KV_TILE - t0 : 0;
+  t0 = lo / KV_PAIR;
+  return len > 0 ? (len + KV_PAIR - 1) / KV_PAIR - t0 : 0;
 }
 __device__ __forceinline__ int kv_len(const KvAttn& A, int i) {
   const int len = A.len[i] + A.len_add;
@@ -107,31 +160,64 @@ __device__ __forceinline__ int kv_len(const KvAttn& A, int i) {
 __host__ __device__ __forceinline__ int kv_units(int heads, int kvh) { return kvh * ((heads / kvh + 7) / 8); }
 __device__ __forceinline__ long long kv_share(long long total, int warps) { return (total + warps - 1) / warps; }
 
-template <int HD, int VB>
-__global__ void __launch_bounds__(KvTok<HD, VB>::WARPS * 32, 1) k_kv_token(KvAttn A) {
+// The partial outputs of a unit whose records are [a, a + tiles) of the list:
+// a unit is the first one of every share it reaches into but its own first,
+// where it is that only if it begins the share.
+struct KvSlots {
+  int s0, cnt;
+  bool mid;
+  __device__ __forceinline__ KvSlots(long long a, long long tiles, long long per) {
+    s0 = (int)(a / per);
+    cnt = (int)((a + tiles - 1) / per) - s0 + 1;
+    mid = a > s0 * per;
+  }
+  __device__ __forceinline__ int slot(int k) const { return 2 * (s0 + k) + (k == 0 && mid ? 1 : 0); }
+};
+
+// UNIT: by unit, W warps a CTA, ST stages each; else by list.
+template <int HD, int VB, bool UNIT, int W, int ST>
+__global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : 16) / W : 1) k_kv_token(const __grid_constant__ KvAttn A) {
   using R = KvRec<HD, VB>;
-  using C = KvTok<HD, VB>;
-  constexpr int G = R::G, NT = C::WARPS * 32, EPT = KV_MAXQ / NT, ST = C::STAGES;
+  constexpr int G = R::G, NT = W * 32, EPT = (KV_MAXQ + NT - 1) / NT, PB = 2 * R::BYTES;
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ long long pre[KV_MAXQ + 1];
-  __shared__ long long wsum[C::WARPS];
-  __shared__ __align__(8) uint64_t bars[C::WARPS * ST];
+  __shared__ long long pre[UNIT ? 1 : KV_MAXQ + 1];
+  __shared__ long long wsum[W];
+  __shared__ float2 uml[UNIT ? W : 1][8];
+  __shared__ __align__(8) uint64_t bars[W * ST];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gsz = A.heads / A.pool.kvh, HB = (gsz + 7) / 8, U = A.pool.kvh * HB;
   if (lane == 0)
     for (int i = 0; i < ST; i++) mbar_init(&bars[warp * ST + i], 1);
   mbar_fence_init();
+  __syncwarp();
   pdl_wait();
   pdl_launch();
   const int n = A.n_dev ? min(*A.n_dev, A.n) : A.n;
-  {  // prefix sums of the queries' records over all their units
+  const int share = warp * gridDim.x + blockIdx.x;   // neighbouring shares go to different SMs
+  float2* ml = (float2*)((long long*)A.ml + KV_PRE);
+  // where a pair lies: query, unit of the query, pair of the sequence, the
+  // unit's first pair and last + 1
+  struct Place { int q, u, pair, beg, end; };
+  Place f, c;                                // the pair to fetch next, and to compute next
+  long long w0 = 0;
+  int todo;                                  // pairs of this warp
+  if (UNIT) {
+    f.q = blockIdx.x / U;
+    f.u = blockIdx.x % U;
+    if (f.q >= n) return;
+    const int pairs = kv_pairs(kv_len(A, f.q), A.window, f.beg);
+    f.end = f.beg + pairs;
+    f.pair = f.beg + pairs * warp / W;
+    todo = f.beg + pairs * (warp + 1) / W - f.pair;
+  } else {
+    // prefix sums of the queries' pairs over all their units
     long long mine[EPT], run = 0;
 #pragma unroll
     for (int e = 0; e < EPT; e++) {
       const int i = tid * EPT + e;
       int t0;
       mine[e] = run;
-      if (i < n) run += (long long)kv_tiles(kv_len(A, i), A.window, t0) * U;
+      if (i < n) run += (long long)kv_pairs(kv_len(A, i), A.window, t0) * U;
     }
     long long inc = run;
 #pragma unroll
@@ -144,117 +230,118 @@ __global__ void __launch_bounds__(KvTok<HD, VB>::WARPS * 32, 1) k_kv_token(KvAtt
     long long base = 0;
     for (int w = 0; w < warp; w++) base += wsum[w];
 #pragma unroll
-    for (int e = 0; e < EPT; e++) pre[tid * EPT + e] = base + inc - run + mine[e];
+    for (int e = 0; e < EPT; e++)
+      if (tid * EPT + e < KV_MAXQ) pre[tid * EPT + e] = base + inc - run + mine[e];
     if (tid == NT - 1) pre[KV_MAXQ] = base + inc;
     __syncthreads();
+    if (blockIdx.x == 0)                     // for k_kv_join: prefix sums, then the (m, l) pairs
+      for (int i = tid; i <= n; i += NT) ((long long*)A.ml)[i] = pre[i];
+    const long long total = pre[KV_MAXQ], per = kv_share(total, gridDim.x * W);
+    w0 = share * per;
+    todo = (int)min(total - w0, per);
+    if (todo <= 0) return;
   }
-  long long* gpre = (long long*)A.ml;       // for k_kv_join: prefix sums, then the (m, l) pairs
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= n; i += NT) gpre[i] = i < KV_MAXQ ? pre[i] : pre[KV_MAXQ];
-  float2* ml = (float2*)(gpre + KV_MAXQ + 1);
-  const long long total = pre[KV_MAXQ];
-  const long long per = kv_share(total, gridDim.x * C::WARPS);
-  // neighbouring shares go to different SMs, so that few records use all of them
-  const int share = warp * gridDim.x + blockIdx.x;
-  const long long w0 = share * per, w1 = min(total, w0 + per);
-  if (w0 >= w1) return;
-
-  uint8_t* st = ring + (size_t)warp * ST * R::BYTES;
-  uint64_t* bar = &bars[warp * ST];
-  const int r = lane >> 2, t = lane & 3;
-  const int bpt = A.pool.block / KV_TILE;
-  const bool vecq = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
-
-  // where a place of the list lies: query, unit of the query, record of the unit
-  int fq, fu, ft, ftiles, ft0;               // the place to fetch next
-  auto locate = [&](long long at, int& q, int& u, int& tile, int& tiles, int& t0) {
-    int lo = 0, hi = n;                      // last query with pre[q] <= at (queries without records repeat a value)
+  auto locate = [&](int at, Place& p) {      // pair `at` of the share
+    const long long x = w0 + at;
+    int lo = 0, hi = n;                      // last query with pre[q] <= x (queries without pairs repeat a value)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (pre[mid] <= at) lo = mid; else hi = mid;
+      if (pre[mid] <= x) lo = mid; else hi = mid;
     }
-    q = lo;
-    tiles = kv_tiles(kv_len(A, q), A.window, t0);
-    const long long off = at - pre[q];
-    u = (int)(off / tiles);
-    tile = (int)(off % tiles);
+    p.q = lo;
+    const int pairs = kv_pairs(kv_len(A, lo), A.window, p.beg);
+    const long long off = x - pre[lo];
+    p.u = (int)(off / pairs);
+    p.pair = p.beg + (int)(off % pairs);
+    p.end = p.beg + pairs;
   };
-  locate(w0, fq, fu, ft, ftiles, ft0);
-  int cq = fq, cu = fu, ct = ft, ctiles = ftiles, ct0 = ft0;   // the place to compute next
-  long long fetch = w0;
-  int ids = 0, ids_at = -1;                  // block ids of 32 records from ids_at on
-  uint32_t bad = 0;                          // stages whose record does not exist
-  int fstage = 0;
+  if (!UNIT) locate(0, f);
+  c = f;
+
+  uint8_t* st = ring + warp * ST * PB;
+  uint64_t* bar = &bars[warp * ST];
+  const int r = lane >> 2, t = lane & 3;
+  const int lb = 31 - __clz(A.pool.block / KV_TILE), bmask = (1 << lb) - 1;   // records of a block: a power of two
+  const size_t bstride = (size_t)A.pool.kvh * R::BYTES << lb;
+  int fetched = 0, fstage = 0;
+  int ids = 0, ids_at = -64;                 // block ids of the pairs ids_at .. ids_at + 15, two lanes a pair
+  uint32_t bad = 0;                          // records that do not exist: bits 2 stage and 2 stage + 1
   auto issue = [&]() {
-    if (fetch >= w1) return;
-    if (ids_at < 0 || ft >= ids_at + 32) {
-      ids_at = ft;
-      const int seq = A.seq ? A.seq[fq] : fq, tile = ft + lane;
-      ids = tile < ftiles ? A.tab.dev[(size_t)seq * A.tab.max_blocks + (ft0 + tile) / bpt] : 0;
+    if (fetched >= todo) return;
+    if ((unsigned)(f.pair - ids_at) >= 16u) {
+      ids_at = f.pair;
+      const int seq = A.seq ? A.seq[f.q] : f.q, rec = 2 * f.pair + lane;
+      ids = rec < A.tab.max_blocks << lb ? A.tab.dev[(size_t)seq * A.tab.max_blocks + (rec >> lb)] : -1;
+      // the second record of the last pair may lie past the end: not read, masked like any place past the end
+      if (rec * KV_TILE >= kv_len(A, f.q)) ids = -2;
     }
-    const int id = __shfl_sync(0xffffffffu, ids, ft - ids_at);
-    const bool ok = (unsigned)id < (unsigned)A.pool.n_blocks;
-    bad = ok ? bad & ~(1u << fstage) : bad | (1u << fstage);
+    // lane 0 copies the first record, lane 1 the second
+    const int id = __shfl_sync(0xffffffffu, ids, 2 * (f.pair - ids_at) + (lane & 1));
+    const bool ok = lane < 2 && (unsigned)id < (unsigned)A.pool.n_blocks;
+    const uint32_t have = __ballot_sync(0xffffffffu, ok);
     if (lane == 0) {
-      if (ok) {
-        mbar_expect_tx(bar + fstage, R::BYTES);
-        bulk_g2s(st + fstage * R::BYTES,
-                 A.pool.base + (((size_t)id * A.pool.kvh + fu / HB) * bpt + (ft0 + ft) % bpt) * R::BYTES, R::BYTES,
-                 bar + fstage);
-      } else {
-        atomicOr(A.pool.err, KV_ERR_BLOCK);
-        mbar_arrive(bar + fstage);
-      }
+      if (have) mbar_expect_tx(bar + fstage, __popc(have) * R::BYTES);
+      else mbar_arrive(bar + fstage);
     }
+    __syncwarp();
+    if (ok) {
+      const int rec = 2 * f.pair + lane;
+      bulk_g2s(st + fstage * PB + lane * R::BYTES,
+               A.pool.base + ((size_t)(f.u / HB) * R::BYTES << lb) + id * bstride + (rec & bmask) * R::BYTES, R::BYTES,
+               bar + fstage);
+    } else if (lane < 2 && id != -2) {
+      atomicOr(A.pool.err, KV_ERR_BLOCK);
+    }
+    bad = (bad & ~(3u << (2 * fstage))) | ((~have & 3u) << (2 * fstage));
     fstage = fstage + 1 == ST ? 0 : fstage + 1;
-    fetch++;
-    if (++ft == ftiles) {
-      ft = 0;
-      ids_at = -1;
-      if (++fu == U && fetch < w1) locate(fetch, fq, fu, ft, ftiles, ft0);
+    fetched++;
+    if (!UNIT && ++f.pair == f.end) {
+      f.pair = f.beg;
+      ids_at = -64;
+      if (++f.u == U && fetched < todo) locate(fetched, f);
+    } else if (UNIT) {
+      f.pair++;
     }
   };
 #pragma unroll
   for (int i = 0; i < ST; i++) issue();
 
-  int cstage = 0;
+  const bool vecq = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
+  const bool vec = kv_vec4(A.o);
+  int cstage = 0, at = 0;
   uint32_t parity = 0;
-  long long at = w0;
-  while (at < w1) {
+  bool gave_up = false;
+  while (UNIT || at < todo) {
     // one unit, or the part of it in this share
-    const long long ubeg = at - ct, uend = ubeg + ctiles, stop = min(w1, uend);
-    const int len = kv_len(A, cq), vis0 = A.window > 0 && len > A.window ? len - A.window : 0;
-    const int kvh = cu / HB, h0 = kvh * gsz + (cu % HB) * 8, nh = min(8, gsz - (cu % HB) * 8);
-    // Q: rows = heads, the k index in the order of the codes' bytes: thread t
-    // holds dims 8t .. 8t + 7 of each group, two steps of 16
+    const bool from_start = c.pair == c.beg;
+    const int stop = min(todo, at + c.end - c.pair);
+    const int len = kv_len(A, c.q), vis0 = A.window > 0 && len > A.window ? len - A.window : 0;
+    const int kvh = c.u / HB, h0 = kvh * gsz + (c.u % HB) * 8, nh = min(8, gsz - (c.u % HB) * 8);
+    // Q^T: columns = heads, the k index in the order of the codes' bytes:
+    // thread t holds dims 8t .. 8t + 7 of each group of head r, two steps of 16
     uint32_t qa[G][4];
-    float sc;
+    float q0[G][4], sc[2];                   // heads 2t and 2t + 1: where each group's sum begins; scale to log2
     {
-      float f[G][8], top = 0.f;
+      const unsigned short* qp = (const unsigned short*)A.q.p + (size_t)c.q * A.q.st + (size_t)(h0 + r) * A.q.sh + 8 * t;
+      float top = 0.f;
 #pragma unroll
       for (int g = 0; g < G; g++) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) f[g][e] = 0.f;
+        uint32_t* x = qa[g];
+        x[0] = x[1] = x[2] = x[3] = 0u;
         if (r < nh) {
-          const unsigned short* p = (const unsigned short*)A.q.p + (size_t)cq * A.q.st + (size_t)(h0 + r) * A.q.sh + 32 * g + 8 * t;
-          uint32_t x[4];
           if (vecq) {
-            const uint4 v = *(const uint4*)p;
+            const uint4 v = *(const uint4*)(qp + 32 * g);
             x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
-          }
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float2 y = A.q.type == KV_F16 ? __half22float2(*(const __half2*)&x[e])
-                                                : make_float2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u));
-            f[g][2 * e] = y.x;
-            f[g][2 * e + 1] = y.y;
+            for (int e = 0; e < 4; e++) x[e] = qp[32 * g + 2 * e] | ((uint32_t)qp[32 * g + 2 * e + 1] << 16);
           }
         }
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[g][e]));
+        for (int e = 0; e < 4; e++) {
+          const float2 y = kv_pair16(x[e], A.q.type);
+          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
+        }
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -263,138 +350,210 @@ __global__ void __launch_bounds__(KvTok<HD, VB>::WARPS * 32, 1) k_kv_token(KvAtt
       int e = (int)(__float_as_uint(top) >> 23) - 127;
       e = e > 127 ? 8 : max(e, -100);
       const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-      sc = A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23);
+      // 2^24: the codes' fp16 numbers
+      const float scr = A.scale * 1.4426950408889634f * 16777216.f * __uint_as_float((uint32_t)(127 + e - 8) << 23);
+      sc[0] = __shfl_sync(0xffffffffu, scr, 8 * t);
+      sc[1] = __shfl_sync(0xffffffffu, scr, 8 * t + 4);
 #pragma unroll
-      for (int g = 0; g < G; g++)
+      for (int g = 0; g < G; g++) {
+        float sum = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; x++) qa[g][x] = kv_pack2(f[g][2 * x] * up, f[g][2 * x + 1] * up);
+        for (int x = 0; x < 4; x++) {
+          float2 y = kv_pair16(qa[g][x], A.q.type);
+          qa[g][x] = kv_pack2(y.x * up, y.y * up);
+          y = __half22float2(*(const __half2*)&qa[g][x]);
+          sum += y.x + y.y;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        sum *= -128.f / 16777216.f;
+        q0[g][0] = q0[g][2] = __shfl_sync(0xffffffffu, sum, 8 * t);
+        q0[g][1] = q0[g][3] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      }
     }
     float o[2 * G][4];
 #pragma unroll
     for (int i = 0; i < 2 * G; i++)
 #pragma unroll
       for (int e = 0; e < 4; e++) o[i][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
-    for (; at < stop; at++, ct++) {
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};   // heads 2t, 2t + 1; l: this thread's positions
+    for (; at < stop; at++, c.pair++) {
       {
         unsigned spins = 0;
-        while (!mbar_try_wait(bar + cstage, parity)) {
-          if (++spins > (1u << 22)) {
-            atomicOr(A.pool.err, KV_ERR_WAIT);
-            return;
-          }
+        while (!mbar_try_wait(bar + cstage, parity) && ++spins < (1u << 22)) {}
+        if (__any_sync(0xffffffffu, spins >= (1u << 22))) {
+          if (lane == 0) atomicOr(A.pool.err, KV_ERR_WAIT);
+          gave_up = true;
+          break;
         }
       }
-      const uint8_t* rec = st + cstage * R::BYTES;
-      // S
-      float s[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-      uint32_t ks[2][G];
-      kv_lds<G>(rec + R::KS + 2 * t * R::SROW, ks[0]);
-      kv_lds<G>(rec + R::KS + (8 + 2 * t) * R::SROW, ks[1]);
+      const uint8_t* pr = st + cstage * PB;
+      // S^T: positions r and r + 8 of each record, heads 2t and 2t + 1
+      float s[2][4];
 #pragma unroll
-      for (int g = 0; g < G; g++) {
+      for (int k = 0; k < 2; k++) {
+        const uint8_t* rec = pr + k * R::BYTES;
+        uint32_t ks[2][G / 2];
+        kv_lds<G / 2>(rec + R::KS + r * R::SROW, ks[0]);
+        kv_lds<G / 2>(rec + R::KS + (8 + r) * R::SROW, ks[1]);
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const uint2 w = *(const uint2*)(rec + kv_kchunk<HD>(8 * j + r, g) + 8 * t);
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
-          kv_mma(c, qa[g][0], 0u, qa[g][1], 0u, kv_half2<0x4140, 128>(w.x), kv_half2<0x4342, 128>(w.x));
-          kv_mma(c, qa[g][2], 0u, qa[g][3], 0u, kv_half2<0x4140, 128>(w.y), kv_half2<0x4342, 128>(w.y));
-          const uint32_t dp = kv_scale_pair<G>(ks[j], g);
-          const float2 d = __half22float2(*(const __half2*)&dp);
-          s[j][0] = fmaf(c[0], d.x, s[j][0]);
-          s[j][1] = fmaf(c[1], d.y, s[j][1]);
+        for (int x = 0; x < 4; x++) s[k][x] = 0.f;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          const uint8_t* kg = rec + 8 * t + kv_kchunk<HD>(r, g);   // rows r and r + 8 have the same permutation
+          const uint2 w = *(const uint2*)kg, y = *(const uint2*)(kg + 8 * HD);
+          float x[4];
+          kv_mma_from(x, q0[g], __byte_perm(w.x, 0u, 0x4140), __byte_perm(y.x, 0u, 0x4140), __byte_perm(w.x, 0u, 0x4342),
+                      __byte_perm(y.x, 0u, 0x4342), qa[g][0], qa[g][1]);
+          kv_mma(x, __byte_perm(w.y, 0u, 0x4140), __byte_perm(y.y, 0u, 0x4140), __byte_perm(w.y, 0u, 0x4342),
+                 __byte_perm(y.y, 0u, 0x4342), qa[g][2], qa[g][3]);
+          const __half2 d0 = *(const __half2*)&ks[0][g >> 1], d1 = *(const __half2*)&ks[1][g >> 1];
+          const float f0 = (g & 1) ? __high2float(d0) : __low2float(d0), f1 = (g & 1) ? __high2float(d1) : __low2float(d1);
+          s[k][0] = fmaf(x[0], f0, s[k][0]);
+          s[k][1] = fmaf(x[1], f0, s[k][1]);
+          s[k][2] = fmaf(x[2], f1, s[k][2]);
+          s[k][3] = fmaf(x[3], f1, s[k][3]);
         }
+#pragma unroll
+        for (int x = 0; x < 4; x++) s[k][x] *= sc[x & 1];
       }
-      const int p0 = (ct0 + ct) * KV_TILE;
-      const int lo = (bad >> cstage) & 1 ? KV_TILE : vis0 - p0, hi = len - p0;   // visible: lo <= p < hi
-      const bool edge = lo > 0 || hi < KV_TILE;
-#pragma unroll
-      for (int j = 0; j < 2; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int p = 8 * j + 2 * t + e;
-          s[j][e] *= sc;
-          if (edge && (p < lo || p >= hi)) s[j][e] = -INFINITY;
-        }
-      float tm = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
-      if (__any_sync(0xffffffffu, tm > m + KV_SLACK)) {
-        const float mn = fmaxf(m, tm);
-        const float a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
-        m = mn;
-        l *= a;
-        const float a0 = __shfl_sync(0xffffffffu, a, 8 * t), a1 = __shfl_sync(0xffffffffu, a, 8 * t + 4);
-#pragma unroll
-        for (int i = 0; i < 2 * G; i++) {
-          o[i][0] *= a0; o[i][1] *= a1; o[i][2] *= a0; o[i][3] *= a1;
-        }
-      }
-      const float mb = (m == -INFINITY ? 0.f : m) - KV_BOOST;
-      uint32_t pb[2];
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const float x = kv_ex2(s[j][0] - mb), y = kv_ex2(s[j][1] - mb);
-        l += x + y;
-        pb[j] = kv_pack2(x, y);
-      }
-      // O^T += V^T P^T
-      uint32_t vs[2][G];
-      kv_lds<G>(rec + R::VS + 2 * t * R::SROW, vs[0]);
-      kv_lds<G>(rec + R::VS + (8 + 2 * t) * R::SROW, vs[1]);
-      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};   // scales of masked places count as zero (they may be NaN)
+      const int p0 = c.pair * KV_PAIR;
+      const uint32_t gone = (bad >> (2 * cstage)) & 3u;
+      const bool edge = p0 < vis0 || p0 + KV_PAIR > len || gone;
+      auto seen = [&](int p) { return p0 + p >= vis0 && p0 + p < len && !((gone >> (p >> 4)) & 1); };
       if (edge) {
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const int p = 8 * j + 2 * t;
-          keep[j] = (p >= lo && p < hi ? 0xffffu : 0u) | (p + 1 >= lo && p + 1 < hi ? 0xffff0000u : 0u);
+        for (int x = 0; x < 4; x++)
+          if (!seen(8 * x + r)) s[x >> 1][2 * (x & 1)] = s[x >> 1][2 * (x & 1) + 1] = -INFINITY;
+      }
+      float mx[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) mx[h] = fmaxf(fmaxf(s[0][h], s[0][2 + h]), fmaxf(s[1][h], s[1][2 + h]));
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + KV_SLACK || mx[1] > m[1] + KV_SLACK)) {
+        float a[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], x));
+          const float mn = fmaxf(m[h], mx[h]);
+          a[h] = m[h] == -INFINITY ? 0.f : kv_ex2(m[h] - mn);
+          m[h] = mn;
+          l[h] *= a[h];
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * G; i++) {
+          o[i][0] *= a[0]; o[i][1] *= a[1]; o[i][2] *= a[0]; o[i][3] *= a[1];
         }
       }
+      const float mb[2] = {(m[0] == -INFINITY ? 0.f : m[0]) - KV_BOOST, (m[1] == -INFINITY ? 0.f : m[1]) - KV_BOOST};
+      uint32_t pb[2][2];
 #pragma unroll
-      for (int c = 0; c < R::VROW / 32; c++) {
-        uint32_t w[4];
+      for (int k = 0; k < 2; k++)
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-          w[x] = *(const uint32_t*)(rec + R::V + kv_vchunk<R::VROW>(2 * t + (x & 1) + 8 * (x >> 1), c) + 4 * r);
+        for (int j = 0; j < 2; j++) {
+          const float x = kv_ex2(s[k][2 * j] - mb[0]), y = kv_ex2(s[k][2 * j + 1] - mb[1]);
+          l[0] += x;
+          l[1] += y;
+          pb[k][j] = kv_transpose(kv_pack2(x, y));
+        }
+      // O^T += V^T P^T
 #pragma unroll
-        for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
-          const int g = VB == 8 ? c : 2 * c + nib;
-          uint32_t b[2][2], d[2];
+      for (int k = 0; k < 2; k++) {
+        const uint8_t* rec = pr + k * R::BYTES;
+        const uint8_t* vp = rec + R::V + 4 * r;
+        uint32_t vs[2][G];
+        kv_lds<G>(rec + R::VS + 2 * t * R::SROW, vs[0]);
+        kv_lds<G>(rec + R::VS + (8 + 2 * t) * R::SROW, vs[1]);
+        if (edge) {                            // a masked place's scale counts as zero (it may be NaN)
+#pragma unroll
+          for (int x = 0; x < 2 * G; x++) {
+            const int j = x / G, y = x % G, e = y / (G / 2);
+            if (!seen(16 * k + 8 * j + 2 * t + e)) vs[j][y] = 0u;
+          }
+        }
+#pragma unroll
+        for (int ch = 0; ch < R::VROW / 32; ch++) {
+          uint32_t h[2][4];                    // bytes of dims 0 .. 3 as fp16 pairs (position 2t, 2t + 1), from 1024
 #pragma unroll
           for (int j = 0; j < 2; j++) {
-            uint32_t x = w[2 * j], y = w[2 * j + 1];
-            if (VB == 4) {
-              x = (x >> (4 * nib)) & 0x0f0f0f0fu;
-              y = (y >> (4 * nib)) & 0x0f0f0f0fu;
-            }
-            b[j][0] = __byte_perm(x, y, 0x5140);       // dims 0, 1 of both positions
-            b[j][1] = __byte_perm(x, y, 0x7362);       // dims 2, 3
-            d[j] = kv_scale_pair<G>(vs[j], g) & keep[j];
+            const uint32_t x = *(const uint32_t*)(vp + kv_vchunk<R::VROW>(2 * t + 8 * j, ch));
+            const uint32_t y = *(const uint32_t*)(vp + kv_vchunk<R::VROW>(2 * t + 1 + 8 * j, ch));
+            const uint32_t b0 = __byte_perm(x, y, 0x5140), b1 = __byte_perm(x, y, 0x7362);
+            h[j][0] = __byte_perm(b0, 0x64646464u, 0x4140);
+            h[j][1] = __byte_perm(b0, 0x64646464u, 0x4342);
+            h[j][2] = __byte_perm(b1, 0x64646464u, 0x4140);
+            h[j][3] = __byte_perm(b1, 0x64646464u, 0x4342);
           }
-          constexpr int BIAS = VB == 8 ? 128 : 8;
 #pragma unroll
-          for (int e = 0; e < 2; e++)
-            kv_mma(o[2 * g + e], kv_hmul2(kv_half2<0x4140, BIAS>(b[0][e]), d[0]),
-                   kv_hmul2(kv_half2<0x4342, BIAS>(b[0][e]), d[0]), kv_hmul2(kv_half2<0x4140, BIAS>(b[1][e]), d[1]),
-                   kv_hmul2(kv_half2<0x4342, BIAS>(b[1][e]), d[1]), pb[0], pb[1]);
+          for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
+            const int g = VB == 8 ? ch : 2 * ch + nib;
+            uint32_t a[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+              const uint32_t d = kv_scale_pair<G>(vs[j], g);
+#pragma unroll
+              for (int e = 0; e < 4; e++) a[j][e] = kv_hmul2(kv_code2<VB>(h[j][e], nib), d);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+              kv_mma(o[2 * g + e], a[0][2 * e], a[0][2 * e + 1], a[1][2 * e], a[1][2 * e + 1], pb[k][0], pb[k][1]);
+          }
         }
       }
-      __syncwarp();                            // every lane has read the record
+      __syncwarp();                            // every lane has read the pair
       issue();
       if (++cstage == ST) {
         cstage = 0;
         parity ^= 1;
       }
     }
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    if (ubeg >= w0 && uend <= w1) {            // the whole unit
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float i0 = __shfl_sync(0xffffffffu, inv, 8 * t), i1 = __shfl_sync(0xffffffffu, inv, 8 * t + 4);
-      const bool vec = kv_vec4(A.o);
+#pragma unroll
+    for (int x = 4; x < 32; x <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], x);
+    }
+    if (UNIT) {                                // the warps' parts through their ring memory
+      float* part = (float*)st;
 #pragma unroll
       for (int g = 0; g < G; g++) {
-        const size_t off = (size_t)cq * A.o.st + 32 * g + 4 * r;
+        if (2 * t < nh)
+          *(float4*)(part + (2 * t) * HD + 32 * g + 4 * r) =
+              make_float4(o[2 * g][0], o[2 * g][2], o[2 * g + 1][0], o[2 * g + 1][2]);
+        if (2 * t + 1 < nh)
+          *(float4*)(part + (2 * t + 1) * HD + 32 * g + 4 * r) =
+              make_float4(o[2 * g][1], o[2 * g][3], o[2 * g + 1][1], o[2 * g + 1][3]);
+      }
+      if (r == 0) {
+        uml[warp][2 * t] = make_float2(m[0], l[0]);
+        uml[warp][2 * t + 1] = make_float2(m[1], l[1]);
+      }
+      __syncthreads();
+      for (int e = tid; e < nh * (HD / 4); e += NT) {
+        const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; w++) M = fmaxf(M, uml[w][h].x);
+        const float base = M == -INFINITY ? 0.f : M;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+          const float y = kv_ex2(uml[w][h].x - base);
+          const float4 v = *(const float4*)(ring + w * ST * PB + (h * HD + d) * 4);
+          L += y * uml[w][h].y;
+          x.x += y * v.x; x.y += y * v.y; x.z += y * v.z; x.w += y * v.w;
+        }
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        kv_st4(A.o, (size_t)c.q * A.o.st + (size_t)(h0 + h) * A.o.sh + d,
+               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), vec);
+      }
+      return;
+    }
+    if (gave_up) return;
+    if (from_start && c.pair == c.end) {       // the whole unit
+      const float i0 = l[0] == 0.f ? 0.f : 1.f / l[0], i1 = l[1] == 0.f ? 0.f : 1.f / l[1];
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        const size_t off = (size_t)c.q * A.o.st + 32 * g + 4 * r;
         if (2 * t < nh)
           kv_st4(A.o, off + (size_t)(h0 + 2 * t) * A.o.sh,
                  make_float4(o[2 * g][0] * i0, o[2 * g][2] * i0, o[2 * g + 1][0] * i0, o[2 * g + 1][2] * i0), vec);
@@ -402,8 +561,8 @@ __global__ void __launch_bounds__(KvTok<HD, VB>::WARPS * 32, 1) k_kv_token(KvAtt
           kv_st4(A.o, off + (size_t)(h0 + 2 * t + 1) * A.o.sh,
                  make_float4(o[2 * g][1] * i1, o[2 * g][3] * i1, o[2 * g + 1][1] * i1, o[2 * g + 1][3] * i1), vec);
       }
-    } else {                                   // slot 2 * share: the share's first unit, + 1: its last
-      const int slot = 2 * share + (ubeg > w0 ? 1 : 0);
+    } else {                                   // slot 2 * share: the share begins in the unit, + 1: the unit in the share
+      const int slot = 2 * share + (from_start && at > c.pair - c.beg ? 1 : 0);
       float* part = A.part + (size_t)slot * 8 * HD;
 #pragma unroll
       for (int g = 0; g < G; g++) {
@@ -414,11 +573,11 @@ __global__ void __launch_bounds__(KvTok<HD, VB>::WARPS * 32, 1) k_kv_token(KvAtt
           *(float4*)(part + (2 * t + 1) * HD + 32 * g + 4 * r) =
               make_float4(o[2 * g][1], o[2 * g][3], o[2 * g + 1][1], o[2 * g + 1][3]);
       }
-      if (t == 0) ml[(size_t)slot * 8 + r] = make_float2(m, l);
+      if (r == 0) *(float4*)&ml[(size_t)slot * 8 + 2 * t] = make_float4(m[0], l[0], m[1], l[1]);
     }
-    if (at < w1) {
-      ct = 0;
-      if (++cu == U) locate(at, cq, cu, ct, ctiles, ct0);
+    if (at < todo) {
+      c.pair = c.beg;
+      if (++c.u == U) locate(at, c);
     }
   }
 }
@@ -426,18 +585,18 @@ __global__ void __launch_bounds__(KvTok<HD, VB>::WARPS * 32, 1) k_kv_token(KvAtt
 // Join: one CTA per (query, head) adds the partial outputs of its unit's
 // shares; zeros where a query sees nothing.  HD / 4 threads read one partial's
 // row (a float4 each), the CTA's other thread groups the next partials.
-#define KV_JOIN_ROWS 8       // most partials read side by side
 template <int HD>
-__global__ void __launch_bounds__(KV_JOIN_ROWS * HD / 4) k_kv_join(KvAttn A, int warps) {
-  constexpr int L = HD / 4;
-  __shared__ float4 acc[KV_JOIN_ROWS][L];
+__global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
+  constexpr int L = HD / 4, MAXW = 4096;
+  __shared__ float4 acc[1024];
+  __shared__ float wgt[MAXW];                // weights of the partials (shares are at most the device's warps)
   __shared__ float red[64];
   const int tid = threadIdx.x, i = blockIdx.x, h = blockIdx.y, rows = blockDim.x / L;
   pdl_wait();
   pdl_launch();
   if (A.n_dev && i >= *A.n_dev) return;
   const long long* gpre = (const long long*)A.ml;
-  const float2* ml = (const float2*)(gpre + KV_MAXQ + 1);
+  const float2* ml = (const float2*)(gpre + KV_PRE);
   const int n = A.n_dev ? min(*A.n_dev, A.n) : A.n;
   const int gsz = A.heads / A.pool.kvh, HB = (gsz + 7) / 8, U = A.pool.kvh * HB;
   const int kvh = h / gsz, hh = h % gsz, u = kvh * HB + hh / 8, row = hh % 8;
@@ -448,40 +607,42 @@ __global__ void __launch_bounds__(KV_JOIN_ROWS * HD / 4) k_kv_join(KvAttn A, int
     if (y == 0) kv_st4(A.o, off, make_float4(0.f, 0.f, 0.f, 0.f), kv_vec4(A.o));
     return;
   }
-  const long long a = p0 + u * tiles, b = a + tiles;
-  const int s0 = (int)(a / per), s1 = (int)((b - 1) / per), cnt = s1 - s0 + 1;
-  if (cnt == 1) return;                        // finished by its warp
-  // a unit is the first one of every share it reaches into but its own first,
-  // where it is that only if it begins the share
-  auto slot = [&](int k) { return 2 * (s0 + k) + (k == 0 && a > s0 * per ? 1 : 0); };
+  const KvSlots S(p0 + u * tiles, tiles, per);
+  if (S.cnt == 1) return;                    // finished by its warp
   float M = -INFINITY;
-  for (int k = tid; k < cnt; k += blockDim.x) M = fmaxf(M, ml[(size_t)slot(k) * 8 + row].x);
+  for (int k = tid; k < S.cnt; k += blockDim.x) M = fmaxf(M, ml[(size_t)S.slot(k) * 8 + row].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if ((tid & 31) == 0) red[tid >> 5] = M;
   __syncthreads();
-  for (int w = 0; w < ((int)blockDim.x + 31) / 32; w++) M = fmaxf(M, red[w]);
+  for (int w = 0; w < (int)blockDim.x / 32; w++) M = fmaxf(M, red[w]);
   const float base = M == -INFINITY ? 0.f : M;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-#pragma unroll 4
-  for (int k = y; k < cnt; k += rows) {
-    const size_t s = (size_t)slot(k) * 8 + row;
-    const float2 e = ml[s];
-    const float4 v = *(const float4*)(A.part + s * HD + 4 * x);
+  for (int k = tid; k < S.cnt; k += blockDim.x) {
+    const float2 e = ml[(size_t)S.slot(k) * 8 + row];
     const float w = kv_ex2(e.x - base);
+    wgt[k] = w;
     l += w * e.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if ((tid & 31) == 0) red[32 + (tid >> 5)] = l;
+  __syncthreads();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = y; k < S.cnt; k += rows) {
+    const float4 v = *(const float4*)(A.part + ((size_t)S.slot(k) * 8 + row) * HD + 4 * x);
+    const float w = wgt[k];
     o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
   }
-  acc[y][x] = o;
-  __syncthreads();
-  if (x == 0) red[32 + y] = l;
+  acc[tid] = o;
   __syncthreads();
   if (y == 0) {
+    l = 0.f;
+    for (int w = 0; w < (int)blockDim.x / 32; w++) l += red[32 + w];
     for (int k = 1; k < rows; k++) {
-      const float4 v = acc[k][x];
+      const float4 v = acc[k * L + x];
       o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-      l += red[32 + k];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     kv_st4(A.o, off, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), kv_vec4(A.o));

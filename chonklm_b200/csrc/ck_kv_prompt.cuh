@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         }
       }
       if (splits > 1)
-        ((float2*)((long long*)A.ml + KV_MAXQ + 1))[((size_t)(b * units + unit) * splits + z) * (128 * C::NQ) + rr] =
+        ((float2*)((long long*)A.ml + KV_PRE))[((size_t)(b * units + unit) * splits + z) * (128 * C::NQ) + rr] =
             make_float2(m, l);
     }
   }
@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(256) k_kv_prompt_join(KvAttn A, int units, int
   const int4 d = ((const int4*)A.ml)[blockIdx.x];
   const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5), tok = row / gs, head = row % gs;
   if (tok >= d.y || head >= d.w) return;
-  const float2* ml = (const float2*)((const long long*)A.ml + KV_MAXQ + 1);
+  const float2* ml = (const float2*)((const long long*)A.ml + KV_PRE);
   float M = -INFINITY, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; e++) o[e] = 0.f;

@@ -29,6 +29,8 @@ import torch
 
 from . import _lib
 
+_I32 = torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(device).cuda_stream without its object
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 # the C argument structs (include/chonk_b200.h), packed by hand: a call is on
@@ -56,40 +58,41 @@ class QuantKvCache:
         _lib._check(self._L.ck_kv_create(cfg, self.device, ctypes.byref(h)))
         self.h = h
         self._dev = torch.device("cuda", self.device)
+        self._scale = 1.0 / math.sqrt(self.head_dim)
 
-    # -- argument checks ----------------------------------------------------
+    # -- argument checks (each call is on the path of every token: plain comparisons, no helper objects) --
     def _rows(self, name: str, t, n: int, heads: int, f32: bool = True) -> tuple:
-        if t.dtype not in _DT or (t.dtype is torch.float32 and not f32):
+        dt = _DT.get(t.dtype, -1)
+        if dt < 0 or (dt == 0 and not f32):
             raise ValueError(f"{name}: {t.dtype}, expected {'float32, ' if f32 else ''}float16 or bfloat16")
         if t.shape != (n, heads, self.head_dim):
             raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {(n, heads, self.head_dim)}")
-        if t.device != self._dev:
+        if t.get_device() != self.device:
             raise ValueError(f"{name} is on {t.device}, the cache on {self._dev}")
         st, sh, sd = t.stride()
         if sd != 1:
             raise ValueError(f"{name}: the elements of a head are not contiguous")
-        return t.data_ptr(), st, sh, _DT[t.dtype], 0
+        return t.data_ptr(), st, sh, dt, 0
 
-    def _ints(self, name: str, t, n: Optional[int]) -> int:
-        if t.dtype is not torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n) or t.device != self._dev or \
-                not t.is_contiguous():
-            raise ValueError(f"{name}: expected a contiguous int32 vector{'' if n is None else f' of {n}'} on {self._dev}")
+    def _ints(self, name: str, t, n: int) -> int:
+        if t.dtype is not _I32 or t.shape != (n,) or t.get_device() != self.device or not t.is_contiguous():
+            raise ValueError(f"{name}: expected a contiguous int32 vector of {n} on {self._dev}")
         return t.data_ptr()
 
     def _table(self, t) -> tuple:
-        if t.dtype is not torch.int32 or t.dim() != 2 or t.device != self._dev or not t.is_contiguous():
+        if t.dtype is not _I32 or t.dim() != 2 or t.get_device() != self.device or not t.is_contiguous():
             raise ValueError(f"table: expected a contiguous int32 matrix on {self._dev}")
-        return t.data_ptr(), t.shape[0], t.shape[1]
+        return t.data_ptr(), *t.shape
 
     def _vector(self, name: str, t, n: int) -> int:
         if t is None:
             return 0
-        if t.dtype is not torch.float32 or t.shape != (n,) or t.device != self._dev or not t.is_contiguous():
+        if t.dtype is not torch.float32 or t.shape != (n,) or t.get_device() != self.device or not t.is_contiguous():
             raise ValueError(f"{name}: expected a contiguous float32 vector of {n} on {self._dev}")
         return t.data_ptr()
 
     def _stream(self, stream: Optional[int]) -> int:
-        return torch.cuda.current_stream(self._dev).cuda_stream if stream is None else stream
+        return _raw_stream(self.device) if stream is None else stream
 
     def _check(self, rc: int) -> None:
         if rc:
@@ -105,7 +108,7 @@ class QuantKvCache:
         n = k.shape[0]
         if q is not None:
             if out is None:
-                out = torch.empty(q.shape, dtype=torch.float16 if q.dtype is torch.float32 else q.dtype, device=q.device)
+                out = q.new_empty(q.shape, dtype=torch.float16) if q.dtype is torch.float32 else q.new_empty(q.shape)
             qa, oa = self._rows("q", q, n, self.heads), self._rows("out", out, n, self.heads, False)
         else:
             if out is not None:
@@ -122,7 +125,8 @@ class QuantKvCache:
         """(k, v) [n, kv_heads, head_dim] of the tokens (seq[i], pos[i]) as the cache holds them."""
         n = seq.shape[0]
         if out is None:
-            out = tuple(torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self._dev) for _ in range(2))
+            shape = (n, self.kv_heads, self.head_dim)
+            out = torch.empty(shape, dtype=dtype, device=self._dev), torch.empty(shape, dtype=dtype, device=self._dev)
         a = _LOAD.pack(*self._rows("k", out[0], n, self.kv_heads), *self._rows("v", out[1], n, self.kv_heads),
                        *self._table(table), self._ints("seq", seq, n), self._ints("pos", pos, n), n, 0)
         self._check(self._L.ck_kv_load(self.h, a, self._stream(stream)))
@@ -134,10 +138,10 @@ class QuantKvCache:
         cached positions, the new one among them; sequence i of the table, or seq[i].  scale: 1 / sqrt(head_dim)."""
         n = q.shape[0]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
                          *self._table(table), self._ints("length", length, n), 0 if seq is None else self._ints("seq", seq, n),
-                         n, window, 1.0 / math.sqrt(self.head_dim) if scale is None else scale, 0)
+                         n, window, self._scale if scale is None else scale, 0)
         self._check(self._L.ck_kv_attend(self.h, a, self._stream(stream)))
         return out
 
@@ -147,14 +151,14 @@ class QuantKvCache:
         sequence i's length[i] cached positions (row i of the table)."""
         n = q.shape[0]
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        cua = self._ints("cu", cu, None)
-        s = cu.shape[0] - 1
+            out = q.new_empty(q.shape)
+        s = cu.numel() - 1
         if s < 0:
             raise ValueError("cu: expected one entry more than sequences")
+        cua = self._ints("cu", cu, s + 1)
         a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
                          *self._table(table), self._ints("length", length, s), 0, s, window,
-                         1.0 / math.sqrt(self.head_dim) if scale is None else scale, 0)
+                         self._scale if scale is None else scale, 0)
         self._check(self._L.ck_kv_attend_prompt(self.h, a, cua, n, self._stream(stream)))
         return out
 
