@@ -39,6 +39,9 @@ size_t kv_pool_bytes(const KvPool& p) {
   return (size_t)p.n_blocks * p.kvh * (p.block / KV_TILE) * kv_record_bytes(p.hd, p.vbits);
 }
 
+#ifndef KV_STORE_WARPS
+#define KV_STORE_WARPS 4096
+#endif
 #ifndef KV_UNIT_PAIRS
 #define KV_UNIT_PAIRS 32
 #endif
@@ -101,22 +104,32 @@ cudaError_t kv_setup(const KvPool& p) {
 
 cudaError_t kv_store_launch(const KvStore& a, cudaStream_t s, bool pdl) {
   if (a.n == 0) return cudaSuccess;
-  const int vec = (kv_vec4(a.q) ? 1 : 0) | (kv_vec4(a.k) ? 2 : 0) | (kv_vec4(a.v) ? 4 : 0) | (kv_vec4(a.qo) ? 8 : 0);
-  const dim3 grid(a.n, 1);
-  switch (a.pool.hd) {
-    case 64: return kv_launch(k_kv_store<64>, grid, dim3(KV_STORE_THREADS), 0, s, pdl, a, vec);
-    case 128: return kv_launch(k_kv_store<128>, grid, dim3(KV_STORE_THREADS), 0, s, pdl, a, vec);
-    default: return kv_launch(k_kv_store<256>, grid, dim3(KV_STORE_THREADS), 0, s, pdl, a, vec);
-  }
+  const int vec = (kv_vec8(a.q) ? 1 : 0) | (kv_vec8(a.k) ? 2 : 0) | (kv_vec8(a.v) ? 4 : 0) | (kv_vec8(a.qo) ? 8 : 0);
+  // warps of a token: enough for a few warps on every scheduler, at most one a row
+  const int rows = (a.heads + 2 * a.pool.kvh) * a.pool.hd / 512;
+  int lw = 0;
+  while (lw < 3 && (1 << lw) < rows && ((long long)a.n << lw) < KV_STORE_WARPS) lw++;
+  const dim3 grid((unsigned)((((long long)a.n << lw) + 7) / 8)), block(KV_STORE_THREADS);
+#define KV_CASE(HD, VB)                                                                                                 \
+  if (a.pool.hd == HD && a.pool.vbits == VB)                                                                            \
+    return a.k.type == KV_F32   ? kv_launch(k_kv_store<HD, VB, KV_F32>, grid, block, 0, s, pdl, a, vec, lw)            \
+           : a.k.type == KV_F16 ? kv_launch(k_kv_store<HD, VB, KV_F16>, grid, block, 0, s, pdl, a, vec, lw)            \
+                                : kv_launch(k_kv_store<HD, VB, KV_BF16>, grid, block, 0, s, pdl, a, vec, lw);
+  KV_EACH(KV_CASE)
+#undef KV_CASE
+  return cudaErrorInvalidValue;
 }
 
 cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
   if (a.n == 0) return cudaSuccess;
-  const int vec = (kv_vec4(a.k) ? 1 : 0) | (kv_vec4(a.v) ? 2 : 0);
-  const long long lanes = (long long)a.n * a.pool.kvh * (a.pool.hd / 4);
-  const dim3 grid((unsigned)((lanes + KV_LOAD_THREADS - 1) / KV_LOAD_THREADS)), block(KV_LOAD_THREADS);
-#define KV_CASE(HD, VB) \
-  if (a.pool.hd == HD && a.pool.vbits == VB) return kv_launch(k_kv_load<HD, VB>, grid, block, 0, s, false, a, vec);
+  const int vec = (kv_vec8(a.k) ? 1 : 0) | (kv_vec8(a.v) ? 2 : 0);
+  const long long rows = (long long)a.n * a.pool.kvh, per = KV_LOAD_ROWS * KV_LOAD_THREADS / (a.pool.hd / 8);
+  const dim3 grid((unsigned)((rows + per - 1) / per)), block(KV_LOAD_THREADS);
+#define KV_CASE(HD, VB)                                                                                      \
+  if (a.pool.hd == HD && a.pool.vbits == VB)                                                                 \
+    return a.k.type == KV_F32   ? kv_launch(k_kv_load<HD, VB, KV_F32>, grid, block, 0, s, false, a, vec)     \
+           : a.k.type == KV_F16 ? kv_launch(k_kv_load<HD, VB, KV_F16>, grid, block, 0, s, false, a, vec)     \
+                                : kv_launch(k_kv_load<HD, VB, KV_BF16>, grid, block, 0, s, false, a, vec);
   KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
@@ -374,6 +387,8 @@ int ck_kv_store(ck_kv* h, const ck_kv_store_args* a, void* stream) {
   } else if (a->q_out.dev) {
     return h->fail(CK_EINVAL, "ck_kv_store: q_out without q");
   }
+  if (a->k.dtype != a->v.dtype || (a->q.dev && a->q.dtype != a->k.dtype))
+    return h->fail(CK_EINVAL, "ck_kv_store: q, k and v have to be of one type");
   if (!(a->eps >= 0.f) && (a->q_norm || a->k_norm)) return h->fail(CK_EINVAL, "ck_kv_store: eps %g", a->eps);
   p.pool = h->pool;
   p.seq = a->seq;
@@ -402,6 +417,7 @@ int ck_kv_load(ck_kv* h, const ck_kv_load_args* a, void* stream) {
       (rc = check_out(h, "ck_kv_load", "k", a->k, a->n, K)) || (rc = check_out(h, "ck_kv_load", "v", a->v, a->n, K)) ||
       (rc = check_table(h, "ck_kv_load", a->table, &p.tab)))
     return rc;
+  if (a->k.dtype != a->v.dtype) return h->fail(CK_EINVAL, "ck_kv_load: k and v have to be of one type");
   p.pool = h->pool;
   p.seq = a->seq;
   p.pos = a->pos;

@@ -63,7 +63,7 @@ __device__ __forceinline__ uint8_t* kv_record(const KvPool& P, const KvTable& T,
     atomicOr(P.err, KV_ERR_SEQ);
     return nullptr;
   }
-  const int slot = pos / P.block;
+  const int lb = 31 - __clz(P.block), slot = pos >> lb;      // blocks are powers of two
   if (pos < 0 || slot >= T.max_blocks) {
     atomicOr(P.err, KV_ERR_POS);
     return nullptr;
@@ -73,220 +73,347 @@ __device__ __forceinline__ uint8_t* kv_record(const KvPool& P, const KvTable& T,
     atomicOr(P.err, KV_ERR_BLOCK);
     return nullptr;
   }
-  const int tiles = P.block / KV_TILE;
-  return P.base + (((size_t)b * P.kvh + head) * tiles + (pos % P.block) / KV_TILE) * (size_t)rec_bytes;
+  return P.base +
+         ((((size_t)b * P.kvh + head) << (lb - 4)) + ((pos & (P.block - 1)) >> 4)) * (size_t)rec_bytes;
 }
 
-// ---- four neighbouring elements of a row -----------------------------------
-__device__ __forceinline__ float4 kv_ld4(const KvRows& r, size_t off, bool vec) {
-  float4 f;
-  if (r.type == KV_F32) {
-    const float* p = (const float*)r.p + off;
-    f = vec ? *(const float4*)p : make_float4(p[0], p[1], p[2], p[3]);
-  } else {
-    uint2 u;
-    const unsigned short* p = (const unsigned short*)r.p + off;
-    if (vec) u = *(const uint2*)p;
-    else u = make_uint2(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16));
-    if (r.type == KV_F16) {
-      const float2 a = __half22float2(*(const __half2*)&u.x), b = __half22float2(*(const __half2*)&u.y);
-      f = make_float4(a.x, a.y, b.x, b.y);
-    } else {
-      f = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                      __uint_as_float(u.y & 0xffff0000u));
-    }
-  }
-  return f;
+// ---- eight neighbouring elements of a row ----------------------------------
+// they may move as 16-byte vectors: base and strides are multiples of that
+__host__ __device__ inline bool kv_vec8(const KvRows& r) {
+  const int n = r.type == KV_F32 ? 4 : 8;
+  return (uintptr_t)r.p % 16 == 0 && r.st % n == 0 && r.sh % n == 0;
 }
-__device__ __forceinline__ void kv_st4(const KvRows& r, size_t off, float4 f, bool vec) {
-  if (r.type == KV_F32) {
-    float* p = (float*)r.p + off;
-    if (vec) *(float4*)p = f;
-    else { p[0] = f.x; p[1] = f.y; p[2] = f.z; p[3] = f.w; }
-    return;
-  }
-  uint2 u;
-  if (r.type == KV_F16) {
-    const __half2 a = __floats2half2_rn(f.x, f.y), b = __floats2half2_rn(f.z, f.w);
-    u = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
-  } else {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(f.x, f.y), b = __floats2bfloat162_rn(f.z, f.w);
-    u = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
-  }
-  unsigned short* p = (unsigned short*)r.p + off;
-  if (vec) *(uint2*)p = u;
-  else {
-    p[0] = (unsigned short)u.x; p[1] = (unsigned short)(u.x >> 16);
-    p[2] = (unsigned short)u.y; p[3] = (unsigned short)(u.y >> 16);
-  }
-}
-// four elements may move as one vector: base and strides are multiples of it
 __host__ __device__ inline bool kv_vec4(const KvRows& r) {
   const int es = r.type == KV_F32 ? 4 : 2;
   return ((uintptr_t)r.p % (4 * es)) == 0 && r.st % 4 == 0 && r.sh % 4 == 0;
 }
+// two neighbouring 16-bit elements
+__device__ __forceinline__ float2 kv_pair16(uint32_t x, int type) {
+  return type == KV_F16 ? __half22float2(*(const __half2*)&x)
+                        : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t kv_to16(float a, float b, int type) {
+  if (type == KV_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *(const uint32_t*)&h;
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *(const uint32_t*)&h;
+}
+// as they lie in memory, and as numbers
+template <int TYPE>
+struct KvRaw8 {
+  uint4 u[TYPE == KV_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* base, size_t off, bool vec) {
+    constexpr int N = TYPE == KV_F32 ? 2 : 1;
+    const char* p = (const char*)base + off * (TYPE == KV_F32 ? 4 : 2);
+    if (vec) {
+#pragma unroll
+      for (int i = 0; i < N; i++) u[i] = __ldg((const uint4*)p + i);
+    } else {
+      uint32_t x[4 * N];
+#pragma unroll
+      for (int e = 0; e < 4 * N; e++)
+        x[e] = TYPE == KV_F32 ? __ldg((const uint32_t*)p + e)
+                              : __ldg((const unsigned short*)p + 2 * e) | ((uint32_t)__ldg((const unsigned short*)p + 2 * e + 1) << 16);
+#pragma unroll
+      for (int i = 0; i < N; i++) u[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ void zero() {
+    u[0] = make_uint4(0u, 0u, 0u, 0u);
+    u[TYPE == KV_F32 ? 1 : 0] = u[0];
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const uint32_t x[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+    if (TYPE == KV_F32) {
+      const uint4 v = u[TYPE == KV_F32 ? 1 : 0];
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[e] = __uint_as_float(x[e]);
+      f[4] = __uint_as_float(v.x); f[5] = __uint_as_float(v.y); f[6] = __uint_as_float(v.z); f[7] = __uint_as_float(v.w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float2 y = kv_pair16(x[e], TYPE);
+        f[2 * e] = y.x;
+        f[2 * e + 1] = y.y;
+      }
+    }
+  }
+};
+// eight 16-bit elements
+__device__ __forceinline__ void kv_put8(void* base, size_t off, const uint32_t (&u)[4], bool vec) {
+  unsigned short* p = (unsigned short*)base + off;
+  if (vec) {
+    *(uint4*)p = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      p[2 * e] = (unsigned short)u[e];
+      p[2 * e + 1] = (unsigned short)(u[e] >> 16);
+    }
+  }
+}
+__device__ __forceinline__ void kv_st4(const KvRows& r, size_t off, float4 f, bool vec) {
+  const uint2 u = make_uint2(kv_to16(f.x, f.y, r.type), kv_to16(f.z, f.w, r.type));
+  unsigned short* p = (unsigned short*)r.p + off;
+  if (vec) {
+    *(uint2*)p = u;
+  } else {
+    p[0] = (unsigned short)u.x; p[1] = (unsigned short)(u.x >> 16);
+    p[2] = (unsigned short)u.y; p[3] = (unsigned short)(u.y >> 16);
+  }
+}
 
 // ---------------------------------------------------------------------------
-// Write.  One CTA per token (blockIdx.x) and share of its rows (blockIdx.y):
-// a row is one head of q, k or v.  A lane holds 4 neighbouring values (two
-// such quads at head_dim 256; two rows a warp at head_dim 64), so a group is
-// 8 lanes and a norm is one warp reduction.  The cosines and sines of the
-// token's position are made once per CTA.
+// Write.  `wpt` warps share a token's rows (a row is one head of q, k or v;
+// rows of one kind are taken together, so a warp runs one kind's code).  A
+// lane holds 8 neighbouring values of each half of a row: both members of its
+// rotation pairs, with 16-byte loads and stores; a row is HD / 16 lanes, a
+// group of 32 values 4 lanes.  The cosines and sines of the token's position
+// are made once per warp and stay in registers, as do the norm weights.
+// Bound by its bytes for many tokens; the instructions come close (two IEEE
+// divisions a group, which the definition of scale and code needs).
 
-// maximum over the 8 lanes of a group
-__device__ __forceinline__ uint32_t group_umax(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+// the larger magnitude; NaN when either is
+__device__ __forceinline__ float kv_maxabs(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
 }
-__device__ __forceinline__ uint32_t kv_abs4(const float4& f) {
-  return max(max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu),
-             max(__float_as_uint(f.z) & 0x7fffffffu, __float_as_uint(f.w) & 0x7fffffffu));
-}
-__device__ __forceinline__ uint32_t kv_code(float x, float inv, float lo, float hi, int bias) {
-  return (uint32_t)(__float2int_rn(fminf(fmaxf(x * inv, lo), hi)) + bias);
-}
-__device__ __forceinline__ uint32_t kv_pack(const float4& f, float inv, float lo, float hi, int bias) {
-  return kv_code(f.x, inv, lo, hi, bias) | (kv_code(f.y, inv, lo, hi, bias) << 8) |
-         (kv_code(f.z, inv, lo, hi, bias) << 16) | (kv_code(f.w, inv, lo, hi, bias) << 24);
-}
-// scale of the lane's group and its reciprocal (0 where the codes are zero)
-__device__ __forceinline__ __half kv_scale(const float4& f, bool four, float& inv) {
-  const uint32_t top = group_umax(kv_abs4(f));
+// codes of the lane's 8 values (4 lanes hold a group), and the group's scale.
+// FOUR: 4 bits.
+template <bool FOUR>
+__device__ __forceinline__ uint2 kv_quant(const float (&f)[8], __half& scale) {
+  float top = kv_maxabs(kv_maxabs(kv_maxabs(f[0], f[1]), kv_maxabs(f[2], f[3])),
+                        kv_maxabs(kv_maxabs(f[4], f[5]), kv_maxabs(f[6], f[7])));
+  top = kv_maxabs(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = kv_maxabs(top, __shfl_xor_sync(0xffffffffu, top, 2));
   float d;
-  if (four) {
+  if (FOUR) {
     // the sign of the largest magnitude: positive when any value has it positive
-    const float m = __uint_as_float(top);
-    const uint32_t pos = group_umax((f.x == m || f.y == m || f.z == m || f.w == m) ? 1u : 0u);
-    d = (pos ? m : -m) / -8.f;
+    float up = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+    up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 1));
+    up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, 2));
+    d = up == top ? top * -0.125f : top * 0.125f;
   } else {
-    d = __uint_as_float(top) / 127.f;
+    d = top / 127.f;
   }
-  d = fminf(fmaxf(d, -65504.f), 65504.f);
-  const __half h = top >= 0x7f800000u ? __ushort_as_half(0x7fff) : __float2half_rn(d);
-  const float dd = __half2float(h);
-  inv = (top >= 0x7f800000u || dd == 0.f) ? 0.f : 1.f / dd;
-  return h;
+  const bool finite = top < INFINITY;
+  scale = finite ? __float2half_rn(fminf(fmaxf(d, -65504.f), 65504.f)) : __ushort_as_half(0x7fff);
+  const float dd = __half2float(scale);
+  const float inv = finite && dd != 0.f ? 1.f / dd : 0.f;
+  // rounding by adding 1.5 * 2^23 (+ the bias): the code is the sum's low byte.
+  // The lower end (and the upper one of 8 bits) is passed only where the
+  // scale is so small that fp16 holds it roughly, or so large that it was cut
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    x[e] = __fmul_rn(f[e], inv);
+    if (FOUR) x[e] = fminf(x[e], 7.f);
+  }
+  if (__any_sync(0xffffffffu, !(top * fabsf(inv) < (FOUR ? 8.5f : 127.5f)))) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = fminf(fmaxf(x[e], FOUR ? -8.f : -127.f), FOUR ? 7.f : 127.f);
+  }
+  uint32_t c[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) c[e] = __float_as_uint(__fadd_rn(x[e], 12582912.f + (FOUR ? 8.f : 128.f)));
+  return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
 }
 
 #define KV_STORE_THREADS 256
-template <int HD>
-__global__ void __launch_bounds__(KV_STORE_THREADS) k_kv_store(KvStore A, int vec) {
-  constexpr int LPR = HD == 64 ? 16 : 32;    // lanes of a row
-  constexpr int RPW = 32 / LPR;              // rows of a warp
-  constexpr int NQ = HD / (4 * LPR);         // quads of a lane
-  constexpr int NW = KV_STORE_THREADS / 32;
-  __shared__ float2 cs[HD / 2];
-  const int t = blockIdx.x;
+template <int HD, int VB, int TYPE>
+__global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv_store(const __grid_constant__ KvStore A, int vec, int lw) {
+  using R = KvRec<HD, VB>;
+  constexpr int LPR = HD / 16, RPW = 32 / LPR, ES = TYPE == KV_F32 ? 4 : 2;   // lanes of a row, rows of a warp
+  __shared__ float2 cs[KV_STORE_THREADS / 32][HD / 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_launch();
-  if (A.n_dev && t >= *A.n_dev) return;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seq = A.seq[t], pos = A.pos[t] + A.pos_add;
-  if (A.inv_freq) {
-    if (tid < HD / 2) {
-      float sn, cn;
-      sincosf((float)pos * A.inv_freq[tid], &sn, &cn);
-      cs[tid] = make_float2(cn, sn);
+  const int gw = blockIdx.x * (KV_STORE_THREADS / 32) + warp, wpt = 1 << lw, t = gw >> lw, sub = gw & (wpt - 1);
+  if (t >= (A.n_dev ? min(*A.n_dev, A.n) : A.n)) return;
+  const int lr = lane % LPR, y = lane / LPR, kvh = A.pool.kvh;
+
+  // this warp's rounds of RPW rows: q's, then k's, then v's (those dealt out in
+  // the other order, which evens out the warps' shares); each round's rows are
+  // on their way while the one before is worked on
+  const int step = RPW << lw, vsub = (wpt - 1 - sub) * RPW, ls = lw + (HD == 64 ? 3 : HD == 128 ? 2 : 1);
+  auto rounds = [&](int rows, int first) { return first < rows ? (rows - first + step - 1) >> ls : 0; };
+  const int nq = rounds(A.heads, sub * RPW), nk = nq + rounds(kvh, sub * RPW), nv = nk + rounds(kvh, vsub);
+  KvRaw8<TYPE> na, nb;                           // the next round's two halves
+  const char* src = nullptr;
+  long long inc = 0;
+  int fr = 0;                                    // and row
+  auto fetch = [&](int i) {
+    if (i == 0 || i == nq || i == nk) {          // the first round of a kind
+      const bool isq = i < nq, isk = !isq && i < nk;
+      const KvRows& m = isq ? A.q : isk ? A.k : A.v;
+      fr = y + (isq || isk ? sub * RPW : vsub);
+      src = (const char*)m.p + ((long long)t * m.st + (long long)fr * m.sh + 8 * lr) * ES;
+      inc = step * m.sh * ES;
+    } else {
+      fr += step;
+      src += inc;
     }
-    __syncthreads();
-  }
-  const int kvh = A.pool.kvh, H = A.heads, rows = H + 2 * kvh;
-  const int rec_bytes = KV_TILE * (HD + HD * A.pool.vbits / 8 + 4 * (HD / KV_GROUP));
-  const int lr = lane & (LPR - 1);
-  const bool vq = vec & 1, vk = vec & 2, vv = vec & 4, vo = vec & 8;
-  for (int r0 = (blockIdx.y * NW + warp) * RPW; r0 < rows; r0 += gridDim.y * NW * RPW) {
-    const int r = r0 + lane / LPR;
-    const bool live = r < rows;
-    const int kind = r < H ? 0 : r < H + kvh ? 1 : 2;      // q, k, v
-    const int head = kind == 0 ? r : kind == 1 ? r - H : r - H - kvh;
-    float4 f[NQ];
+    if (i < nv && fr < (i < nq ? A.heads : kvh)) {
+      const bool v = vec & (i < nq ? 1 : i < nk ? 2 : 4);
+      na.load(src, 0, v);
+      nb.load(src, HD / 2, v);
+    } else {
+      na.zero();
+      nb.zero();
+    }
+  };
+  fetch(0);
+  const int seq = A.seq[t], pos = A.pos[t] + A.pos_add;
+  const bool rope = A.inv_freq != nullptr, inter = A.interleaved;
+  float cn[8], sn[8];                            // of the lane's 8 pairs
+  if (rope) {
+    for (int i = lane; i < HD / 2; i += 32) {
+      float s, c;
+      sincosf((float)pos * A.inv_freq[i], &s, &c);
+      cs[warp][i] = make_float2(c, s);
+    }
+    __syncwarp();
 #pragma unroll
-    for (int j = 0; j < NQ; j++) {
-      f[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (live) {
-        const KvRows& src = kind == 0 ? A.q : kind == 1 ? A.k : A.v;
-        f[j] = kv_ld4(src, (size_t)t * src.st + (size_t)head * src.sh + 128 * j + 4 * lr,
-                      kind == 0 ? vq : kind == 1 ? vk : vv);
+    for (int e = 0; e < 8; e++) {
+      const float2 x = cs[warp][inter ? (e < 4 ? 0 : HD / 4) + 4 * lr + (e & 3) : 8 * lr + e];
+      cn[e] = x.x;
+      sn[e] = x.y;
+    }
+  }
+  uint8_t* rec0 = seq >= 0 ? kv_record(A.pool, A.tab, seq, pos, R::BYTES, 0) : nullptr;   // of kv head 0
+  const size_t hbytes = (size_t)(A.pool.block / KV_TILE) * R::BYTES;                      // to the next kv head's
+  const int p = pos & (KV_TILE - 1), g = lr >> 2, gb = R::G / 2 + g;                      // groups of the two halves
+
+  float wa[8], wb[8];
+  const float* w = nullptr;
+  auto weights = [&](const float* x) {
+    w = x;
+    if (w && ((uintptr_t)w & 15) == 0) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 x = __ldg((const float4*)(w + 8 * lr + e)), z = __ldg((const float4*)(w + HD / 2 + 8 * lr + e));
+        wa[e] = x.x; wa[e + 1] = x.y; wa[e + 2] = x.z; wa[e + 3] = x.w;
+        wb[e] = z.x; wb[e + 1] = z.y; wb[e + 2] = z.z; wb[e + 3] = z.w;
+      }
+    } else if (w) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        wa[e] = __ldg(w + 8 * lr + e);
+        wb[e] = __ldg(w + HD / 2 + 8 * lr + e);
       }
     }
-    const float* w = kind == 0 ? A.qw : A.kw;
-    if (A.qw || A.kw) {      // the reduction's shuffles need the whole warp
+  };
+  auto turn = [&](float (&a)[8], float (&b)[8]) {   // norm and rotation
+    if (w) {
       float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < NQ; j++) ss += f[j].x * f[j].x + f[j].y * f[j].y + f[j].z * f[j].z + f[j].w * f[j].w;
+      for (int e = 0; e < 8; e++) ss += a[e] * a[e] + b[e] * b[e];
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (kind < 2 && w) {
-        const float inv = 1.0f / sqrtf(ss / (float)HD + A.eps);
+      const float inv = rsqrtf(ss * (1.f / HD) + A.eps);
 #pragma unroll
-        for (int j = 0; j < NQ; j++) {
-          const float* wj = w + 128 * j + 4 * lr;
-          f[j].x = (f[j].x * inv) * wj[0];
-          f[j].y = (f[j].y * inv) * wj[1];
-          f[j].z = (f[j].z * inv) * wj[2];
-          f[j].w = (f[j].w * inv) * wj[3];
-        }
+      for (int e = 0; e < 8; e++) {
+        a[e] = (a[e] * inv) * wa[e];
+        b[e] = (b[e] * inv) * wb[e];
       }
     }
-    if (A.inv_freq) {
-      if (A.interleaved) {
+    if (rope && inter) {
 #pragma unroll
-        for (int j = 0; j < NQ; j++) {
-          const float2 c0 = cs[64 * j + 2 * lr], c1 = cs[64 * j + 2 * lr + 1];
-          const float4 x = f[j];
-          if (kind < 2)
-            f[j] = make_float4(x.x * c0.x - x.y * c0.y, x.x * c0.y + x.y * c0.x, x.z * c1.x - x.w * c1.y,
-                               x.z * c1.y + x.w * c1.x);
-        }
-      } else if (NQ == 2) {   // dims d and d + 128 sit in one lane
-        float* a = (float*)&f[0];
-        float* b = (float*)&f[NQ - 1];
+      for (int e = 0; e < 8; e += 2) {
+        float x = a[e], z = a[e + 1];
+        a[e] = x * cn[e / 2] - z * sn[e / 2];
+        a[e + 1] = x * sn[e / 2] + z * cn[e / 2];
+        x = b[e], z = b[e + 1];
+        b[e] = x * cn[4 + e / 2] - z * sn[4 + e / 2];
+        b[e + 1] = x * sn[4 + e / 2] + z * cn[4 + e / 2];
+      }
+    } else if (rope) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 c = cs[4 * lr + e];
-          const float x = a[e], y = b[e];
-          if (kind < 2) {
-            a[e] = x * c.x - y * c.y;
-            b[e] = x * c.y + y * c.x;
+      for (int e = 0; e < 8; e++) {
+        const float x = a[e], z = b[e];
+        a[e] = x * cn[e] - z * sn[e];
+        b[e] = x * sn[e] + z * cn[e];
+      }
+    }
+  };
+  const bool o16 = A.qo.type == KV_F16;
+  char* qo = (char*)A.qo.p + ((long long)t * A.qo.st + (long long)(y + sub * RPW) * A.qo.sh + 8 * lr) * 2;
+  weights(nq ? A.qw : A.kw);
+#pragma unroll 1
+  for (int i = 0; i < nv; i++) {
+    float a[8], b[8];
+    na.get(a);
+    nb.get(b);
+    const int r = fr;
+    fetch(i + 1);
+    if (i < nq) {
+      turn(a, b);
+      if (r < A.heads) {
+        uint32_t u[4], x[4];
+        if (o16) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            u[e] = kv_to16(a[2 * e], a[2 * e + 1], KV_F16);
+            x[e] = kv_to16(b[2 * e], b[2 * e + 1], KV_F16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            u[e] = kv_to16(a[2 * e], a[2 * e + 1], KV_BF16);
+            x[e] = kv_to16(b[2 * e], b[2 * e + 1], KV_BF16);
           }
         }
-      } else {                // dims d and d + hd/2 sit half a row apart
-        const bool up = lr >= LPR / 2;
-        float* a = (float*)&f[0];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float2 c = cs[(4 * lr + e) & (HD / 2 - 1)];
-          const float o = __shfl_xor_sync(0xffffffffu, a[e], LPR / 2);
-          if (kind < 2) a[e] = up ? o * c.y + a[e] * c.x : a[e] * c.x - o * c.y;
+        kv_put8(qo, 0, u, vec & 8);
+        kv_put8(qo, HD / 2, x, vec & 8);
+      }
+      qo += (long long)step * A.qo.sh * 2;
+    } else if (i < nk) {
+      if (i == nq && nq) weights(A.kw);
+      turn(a, b);
+      __half da, db;
+      const uint2 ca = kv_quant<false>(a, da), cb = kv_quant<false>(b, db);
+      if (r < kvh && rec0) {
+        uint8_t* rec = rec0 + r * hbytes;
+        *(uint2*)(rec + kv_kchunk<HD>(p, g) + 8 * (lr & 3)) = ca;
+        *(uint2*)(rec + kv_kchunk<HD>(p, gb) + 8 * (lr & 3)) = cb;
+        if ((lr & 3) == 0) {
+          *(__half*)(rec + R::KS + (p * R::G + g) * 2) = da;
+          *(__half*)(rec + R::KS + (p * R::G + gb) * 2) = db;
         }
       }
-    }
-    // quantisation is computed by every lane (its shuffles need the whole
-    // warp); q rows only ignore it
-    const bool four = kind == 2 && A.pool.vbits == 4;
-    uint8_t* rec = nullptr;
-    if (live && kind > 0 && seq >= 0) rec = kv_record(A.pool, A.tab, seq, pos, rec_bytes, head);
-    const int p = pos & (KV_TILE - 1);
-    const int vrow = HD * A.pool.vbits / 8;
-#pragma unroll
-    for (int j = 0; j < NQ; j++) {
-      const int g = 4 * j + lr / 8;          // group of this lane's quad
-      float inv;
-      const __half d = kv_scale(f[j], four, inv);
-      const uint32_t c8 = kv_pack(f[j], inv, four ? -8.f : -127.f, four ? 7.f : 127.f, four ? 8 : 128);
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, c8, 8);   // the neighbouring group's codes (4 bits)
-      if (live && kind == 0 && A.qo.p)
-        kv_st4(A.qo, (size_t)t * A.qo.st + (size_t)head * A.qo.sh + 128 * j + 4 * lr, f[j], vo);
-      if (rec) {
-        const int vs = KV_TILE * (HD + vrow) + (kind == 2 ? KV_TILE * 2 * (HD / KV_GROUP) : 0);
-        if ((lr & 7) == 0) *(__half*)(rec + vs + (p * (HD / KV_GROUP) + g) * 2) = d;
-        if (kind == 1) {
-          *(uint32_t*)(rec + kv_kchunk<HD>(p, g) + 4 * (lr & 7)) = c8;
-        } else if (!four) {
-          *(uint32_t*)(rec + KV_TILE * HD + kv_vchunk<HD>(p, g) + 4 * (lr & 7)) = c8;
-        } else if ((g & 1) == 0) {
-          *(uint32_t*)(rec + KV_TILE * HD + kv_vchunk<HD / 2>(p, g >> 1) + 4 * (lr & 7)) = c8 | (other << 4);
+    } else {
+      __half da, db;
+      uint2 ca = kv_quant<VB == 4>(a, da), cb = kv_quant<VB == 4>(b, db);
+      if (VB == 4) {
+        // nibbles of two neighbouring groups share a chunk: at head_dim 64 those
+        // of the lane's halves, else those of lanes 4 apart (the even group's
+        // lanes write them)
+        if (HD == 64) {
+          ca.x |= cb.x << 4;
+          ca.y |= cb.y << 4;
+        } else {
+          ca.x |= __shfl_xor_sync(0xffffffffu, ca.x, 4) << 4;
+          ca.y |= __shfl_xor_sync(0xffffffffu, ca.y, 4) << 4;
+          cb.x |= __shfl_xor_sync(0xffffffffu, cb.x, 4) << 4;
+          cb.y |= __shfl_xor_sync(0xffffffffu, cb.y, 4) << 4;
+        }
+      }
+      if (r < kvh && rec0) {
+        uint8_t* rec = rec0 + r * hbytes;
+        if (VB == 8) {
+          *(uint2*)(rec + R::V + kv_vchunk<R::VROW>(p, g) + 8 * (lr & 3)) = ca;
+          *(uint2*)(rec + R::V + kv_vchunk<R::VROW>(p, gb) + 8 * (lr & 3)) = cb;
+        } else if (HD == 64 || (g & 1) == 0) {
+          *(uint2*)(rec + R::V + kv_vchunk<R::VROW>(p, g >> 1) + 8 * (lr & 3)) = ca;
+          if (HD > 64) *(uint2*)(rec + R::V + kv_vchunk<R::VROW>(p, gb >> 1) + 8 * (lr & 3)) = cb;
+        }
+        if ((lr & 3) == 0) {
+          *(__half*)(rec + R::VS + (p * R::G + g) * 2) = da;
+          *(__half*)(rec + R::VS + (p * R::G + gb) * 2) = db;
         }
       }
     }
@@ -294,34 +421,92 @@ __global__ void __launch_bounds__(KV_STORE_THREADS) k_kv_store(KvStore A, int ve
 }
 
 // ---------------------------------------------------------------------------
-// Read back: a warp takes (token, kv head) rows, a lane 4 neighbouring values
-// of the key and of the value.
+// Read back: a lane takes 8 neighbouring values of a (token, kv head) row's
+// key and value, and KV_LOAD_ROWS rows at once, whose loads are in flight
+// together.
 
 #define KV_LOAD_THREADS 256
-template <int HD, int VB>
-__global__ void __launch_bounds__(KV_LOAD_THREADS) k_kv_load(KvLoad A, int vec) {
-  using R = KvRec<HD, VB>;
-  constexpr int Q = HD / 4;                  // lanes of a row
-  const long long i = (long long)blockIdx.x * KV_LOAD_THREADS + threadIdx.x;
-  const long long row = i / Q;
-  if (row >= (long long)A.n * A.pool.kvh) return;
-  const int lr = (int)(i % Q), t = (int)(row / A.pool.kvh), head = (int)(row % A.pool.kvh);
-  const int seq = A.seq[t], pos = A.pos[t];
-  float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-  const uint8_t* rec = seq >= 0 ? kv_record(A.pool, A.tab, seq, pos, R::BYTES, head) : nullptr;
-  if (rec) {
-    const int p = pos & (KV_TILE - 1), g = lr >> 3;
-    const uint32_t kc = *(const uint32_t*)(rec + kv_kchunk<HD>(p, g) + 4 * (lr & 7));
-    const float kd = __half2float(*(const __half*)(rec + R::KS + (p * R::G + g) * 2));
-    uint32_t vc = *(const uint32_t*)(rec + R::V + kv_vchunk<R::VROW>(p, VB == 8 ? g : g >> 1) + 4 * (lr & 7));
-    const float vd = __half2float(*(const __half*)(rec + R::VS + (p * R::G + g) * 2));
-    if (VB == 4) vc = (vc >> (4 * (g & 1))) & 0x0f0f0f0fu;
-    const float vb = VB == 8 ? 128.f : 8.f;
-    k = make_float4(((float)(kc & 255u) - 128.f) * kd, ((float)((kc >> 8) & 255u) - 128.f) * kd,
-                    ((float)((kc >> 16) & 255u) - 128.f) * kd, ((float)(kc >> 24) - 128.f) * kd);
-    v = make_float4(((float)(vc & 255u) - vb) * vd, ((float)((vc >> 8) & 255u) - vb) * vd,
-                    ((float)((vc >> 16) & 255u) - vb) * vd, ((float)(vc >> 24) - vb) * vd);
+#define KV_LOAD_ROWS 2
+// eight codes (bytes) less their bias, times d, as TYPE.  For fp16 in fp16: a
+// code is exact there and the product is rounded once; else in 32 bits, a byte
+// u becoming a float as the bits of 2^23 + u.
+template <int TYPE>
+__device__ __forceinline__ void kv_out8(uint2 c, __half d, int bias, void* base, size_t off, bool vec) {
+  const uint32_t w[2] = {c.x, c.y};
+  if (TYPE == KV_F16) {
+    uint32_t u[4];
+    const __half2 b = __half2half2(__ushort_as_half((unsigned short)(0x6400 + bias))), dd = __half2half2(d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t x = __byte_perm(w[e >> 1], 0x64646464u, (e & 1) ? 0x4342 : 0x4140);
+      const __half2 y = __hmul2(__hsub2(*(const __half2*)&x, b), dd);
+      u[e] = *(const uint32_t*)&y;
+    }
+    kv_put8(base, off, u, vec);
+    return;
   }
-  kv_st4(A.k, (size_t)t * A.k.st + (size_t)head * A.k.sh + 4 * lr, k, vec & 1);
-  kv_st4(A.v, (size_t)t * A.v.st + (size_t)head * A.v.sh + 4 * lr, v, vec & 2);
+  float f[8];
+  const float fd = __half2float(d), fb = 8388608.f + bias;
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    f[e] = (__uint_as_float(__byte_perm(w[e >> 2], 0x4b000000u, 0x7440 + (e & 3))) - fb) * fd;
+  if (TYPE == KV_F32) {
+    float* p = (float*)base + off;
+    if (vec) {
+      *(float4*)p = make_float4(f[0], f[1], f[2], f[3]);
+      *((float4*)p + 1) = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) p[e] = f[e];
+    }
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) u[e] = kv_to16(f[2 * e], f[2 * e + 1], TYPE);
+    kv_put8(base, off, u, vec);
+  }
+}
+
+template <int HD, int VB, int TYPE>
+__global__ void __launch_bounds__(KV_LOAD_THREADS) k_kv_load(const __grid_constant__ KvLoad A, int vec) {
+  using R = KvRec<HD, VB>;
+  constexpr int LPR = HD / 8, RPB = KV_LOAD_THREADS / LPR;   // lanes of a row, rows of a CTA at a time
+  const int lr = threadIdx.x % LPR, g = lr >> 2, kvh = A.pool.kvh;
+  const long long rows = (long long)A.n * kvh;
+  long long row[KV_LOAD_ROWS];
+  int t[KV_LOAD_ROWS], head[KV_LOAD_ROWS], seq[KV_LOAD_ROWS], pos[KV_LOAD_ROWS];
+#pragma unroll
+  for (int x = 0; x < KV_LOAD_ROWS; x++) {
+    row[x] = ((long long)blockIdx.x * KV_LOAD_ROWS + x) * RPB + threadIdx.x / LPR;
+    t[x] = (int)(min(row[x], rows - 1) / kvh);
+    head[x] = (int)(min(row[x], rows - 1) % kvh);
+    seq[x] = __ldg(A.seq + t[x]);
+    pos[x] = __ldg(A.pos + t[x]);
+  }
+  uint2 kc[KV_LOAD_ROWS], vc[KV_LOAD_ROWS];
+  __half kd[KV_LOAD_ROWS], vd[KV_LOAD_ROWS];
+#pragma unroll
+  for (int x = 0; x < KV_LOAD_ROWS; x++) {
+    const uint8_t* rec = row[x] < rows && seq[x] >= 0 ? kv_record(A.pool, A.tab, seq[x], pos[x], R::BYTES, head[x]) : nullptr;
+    const int p = pos[x] & (KV_TILE - 1);
+    kc[x] = make_uint2(0x80808080u, 0x80808080u);   // zeros, without a sign
+    vc[x] = VB == 8 ? kc[x] : make_uint2(0x88888888u, 0x88888888u);
+    kd[x] = vd[x] = __ushort_as_half(0);
+    if (rec) {
+      kc[x] = *(const uint2*)(rec + kv_kchunk<HD>(p, g) + 8 * (lr & 3));
+      vc[x] = *(const uint2*)(rec + R::V + kv_vchunk<R::VROW>(p, VB == 8 ? g : g >> 1) + 8 * (lr & 3));
+      kd[x] = *(const __half*)(rec + R::KS + (p * R::G + g) * 2);
+      vd[x] = *(const __half*)(rec + R::VS + (p * R::G + g) * 2);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < KV_LOAD_ROWS; x++) {
+    if (row[x] >= rows) break;
+    kv_out8<TYPE>(kc[x], kd[x], 128, A.k.p, (size_t)t[x] * A.k.st + (size_t)head[x] * A.k.sh + 8 * lr, vec & 1);
+    if (VB == 4) {
+      vc[x].x = (vc[x].x >> (4 * (g & 1))) & 0x0f0f0f0fu;
+      vc[x].y = (vc[x].y >> (4 * (g & 1))) & 0x0f0f0f0fu;
+    }
+    kv_out8<TYPE>(vc[x], vd[x], VB == 8 ? 128 : 8, A.v.p, (size_t)t[x] * A.v.st + (size_t)head[x] * A.v.sh + 8 * lr, vec & 2);
+  }
 }

@@ -104,11 +104,6 @@ __device__ __forceinline__ uint32_t kv_pack2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *(const uint32_t*)&h;
 }
-// two neighbouring 16-bit elements
-__device__ __forceinline__ float2 kv_pair16(uint32_t x, int type) {
-  return type == KV_F16 ? __half22float2(*(const __half2*)&x)
-                        : make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
-}
 __device__ __forceinline__ float kv_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

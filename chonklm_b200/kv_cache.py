@@ -108,7 +108,7 @@ class QuantKvCache:
         n = k.shape[0]
         if q is not None:
             if out is None:
-                out = q.new_empty(q.shape, dtype=torch.float16) if q.dtype is torch.float32 else q.new_empty(q.shape)
+                out = torch.empty_like(q, dtype=torch.float16) if q.dtype is torch.float32 else torch.empty_like(q)
             qa, oa = self._rows("q", q, n, self.heads), self._rows("out", out, n, self.heads, False)
         else:
             if out is not None:
@@ -125,8 +125,8 @@ class QuantKvCache:
         """(k, v) [n, kv_heads, head_dim] of the tokens (seq[i], pos[i]) as the cache holds them."""
         n = seq.shape[0]
         if out is None:
-            shape = (n, self.kv_heads, self.head_dim)
-            out = torch.empty(shape, dtype=dtype, device=self._dev), torch.empty(shape, dtype=dtype, device=self._dev)
+            first = torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self._dev)
+            out = first, torch.empty_like(first)
         a = _LOAD.pack(*self._rows("k", out[0], n, self.kv_heads), *self._rows("v", out[1], n, self.kv_heads),
                        *self._table(table), self._ints("seq", seq, n), self._ints("pos", pos, n), n, 0)
         self._check(self._L.ck_kv_load(self.h, a, self._stream(stream)))
@@ -138,7 +138,7 @@ class QuantKvCache:
         cached positions, the new one among them; sequence i of the table, or seq[i].  scale: 1 / sqrt(head_dim)."""
         n = q.shape[0]
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q)
         a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
                          *self._table(table), self._ints("length", length, n), 0 if seq is None else self._ints("seq", seq, n),
                          n, window, self._scale if scale is None else scale, 0)
@@ -151,7 +151,7 @@ class QuantKvCache:
         sequence i's length[i] cached positions (row i of the table)."""
         n = q.shape[0]
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q)
         s = cu.numel() - 1
         if s < 0:
             raise ValueError("cu: expected one entry more than sequences")

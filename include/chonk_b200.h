@@ -278,7 +278,7 @@ typedef struct ck_kv_table {
 } ck_kv_table;
 
 typedef struct ck_kv_store_args {
-  ck_kv_rows q, k, v;              /* f32, f16 or bf16; q.dev NULL: only k and v      */
+  ck_kv_rows q, k, v;              /* f32, f16 or bf16, all of one; q.dev NULL: only k and v */
   ck_kv_rows q_out;                /* f16 or bf16                                     */
   ck_kv_table table;
   const int32_t *seq, *pos;        /* [n] row of the table and position; seq < 0: padding, not stored */
@@ -291,7 +291,7 @@ typedef struct ck_kv_store_args {
 } ck_kv_store_args;
 
 typedef struct ck_kv_load_args {
-  ck_kv_rows k, v;                 /* written: f32, f16 or bf16                       */
+  ck_kv_rows k, v;                 /* written: f32, f16 or bf16, both of one          */
   ck_kv_table table;
   const int32_t *seq, *pos;
   int32_t n;
