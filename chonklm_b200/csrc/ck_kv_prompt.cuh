@@ -16,14 +16,16 @@
 //             V is fed to the second product as it lies, its dims contiguous)
 //   1 thread  issues the products
 //   4 or 8    softmax: a thread owns a query row; it reads S from tensor
-//             memory twice (maximum, then exponentials) and writes P over it
-//             as the second product's operand
+//             memory once, 64 columns at a time, and writes P over what it
+//             has read as the second product's operand.  The exponentials
+//             are taken against a reference maximum that is moved (and O, l
+//             and the tile's earlier P rescaled) only where a score passes
+//             it by 2^8, and for the first scores
 // A CTA holds 256 query rows (two tiles, whose products and softmaxes take
 // turns; the K and V tiles serve both) or, at head_dim 256, 128 rows with two
 // score buffers (the next scores are computed under the present softmax).  A
 // query row is a (token, head of the kv head's group) pair, so the group
-// shares K and V.  O is rescaled only when a row's maximum passes the
-// reference by 2^8.  CTAs are numbered by depth (position of the tile within
+// shares K and V.  CTAs are numbered by depth (position of the tile within
 // its sequence), the deepest first: they take longest.
 //
 // Long caches with few rows would leave SMs idle: the cached positions are
@@ -75,13 +77,30 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem, uint32_t a, uint64_t 
                " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem),
                "r"(a), "l"(db), "r"(idesc), "r"(acc));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]));
+// two 32-bit floats at once
+__device__ __forceinline__ uint64_t kvp_pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-
+__device__ __forceinline__ void kvp_split(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t kvp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t kvp_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float kvp_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 // A value scale that is NaN, or so large that code * scale would pass fp16,
 // must not meet a masked p = 0 in the second product (0 * inf): its values
 // count as zero there, and the position's key becomes NaN, so that exactly the
@@ -121,7 +140,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
   __shared__ int s_seq, s_tile;
-  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_k, b_kfree, b_v, b_vfree, b_s[2], b_p[2],
+  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k, b_kfree, b_v, b_vfree, b_s[2], b_p[2],
       b_o, b_pv, b_end;
   __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 4 ahead)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -134,9 +153,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       const int r = A.cu[s + 1] - A.cu[s];
       return r > 0 ? (r + bt - 1) / bt : 0;
     };
+    const int mine = lane < A.n ? depth(lane) : 0;
     auto above = [&](int d) {
-      int c = 0;
-      for (int s = lane; s < A.n; s += 32) c += max(0, depth(s) - d);
+      int c = max(0, mine - d);
+      for (int s = lane + 32; s < A.n; s += 32) c += max(0, depth(s) - d);
       return __reduce_add_sync(0xffffffffu, c);
     };
     int lo = -1, hi = A.rows / bt + 1;         // f(lo) > b >= f(hi)
@@ -224,6 +244,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       mbar_init(&b_full[i], 1);
       mbar_init(&b_empty[i], C::DEQ);
     }
+    mbar_init(&b_q, C::SOFT * 32);
     mbar_init(&b_k, C::DEQ * 32);
     mbar_init(&b_v, C::DEQ * 32);
     mbar_init(&b_kfree, 1);
@@ -236,57 +257,6 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     mbar_init(&b_pv, 1);
     mbar_init(&b_end, 1);
     mbar_fence_init();
-  }
-  // Q: each softmax thread its own row, brought to a power of two near 1 (see
-  // ck_kv_attn.cuh), 16 bits
-  float sc = 0.f;
-  const int wq = warp >> 2, rl = 32 * (warp & 3) + lane;    // query tile and row of a softmax thread
-  const int rr = 128 * wq + rl, rtok = rr / gs, rhead = rr % gs;
-  const bool rlive = warp < C::SOFT && rtok < ntok && rhead < nh;
-  if (warp < C::SOFT) {
-    const unsigned short* p = (const unsigned short*)A.q.p + (size_t)(q0 + rtok) * A.q.st + (size_t)(h0 + rhead) * A.q.sh;
-    const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
-    auto load8 = [&](int d, float (&f)[8]) {
-      uint32_t x[4] = {0u, 0u, 0u, 0u};
-      if (rlive) {
-        if (vec) {
-          const uint4 v = *(const uint4*)(p + d);
-          x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e++) x[e] = p[d + 2 * e] | ((uint32_t)p[d + 2 * e + 1] << 16);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float2 y = A.q.type == KV_F16 ? __half22float2(*(const __half2*)&x[e])
-                                            : make_float2(__uint_as_float(x[e] << 16), __uint_as_float(x[e] & 0xffff0000u));
-        f[2 * e] = y.x;
-        f[2 * e + 1] = y.y;
-      }
-    };
-    float top = 0.f;
-#pragma unroll 4
-    for (int d = 0; d < HD; d += 8) {
-      float f[8];
-      load8(d, f);
-#pragma unroll
-      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[e]));
-    }
-    int e = (int)(__float_as_uint(top) >> 23) - 127;
-    e = e > 127 ? 8 : max(e, -100);
-    // (the scale's sign goes to q: the largest product is the largest score)
-    const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
-    sc = fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23);
-#pragma unroll 4
-    for (int d = 0; d < HD; d += 8) {
-      float f[8];
-      load8(d, f);
-      const uint4 v = make_uint4(kv_pack2(f[0] * up, f[1] * up), kv_pack2(f[2] * up, f[3] * up),
-                                 kv_pack2(f[4] * up, f[5] * up), kv_pack2(f[6] * up, f[7] * up));
-      *(uint4*)(sm + C::SQ + wq * C::QB + kvp_kmajor<128>(rl, d)) = v;
-    }
-    proxy_fence_smem();
   }
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
@@ -331,7 +301,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     if (lane == 0) {
       const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
       const uint32_t idO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);   // V's dims are contiguous
-      bool ok = true;
+      bool ok = jb >= je || kvp_wait<false>(&b_q, 0, &s_fail, A.pool.err);
       auto scores = [&](int w, int buf) {
 #pragma unroll
         for (int k = 0; k < HD / 16; k++)
@@ -392,7 +362,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       }
       umma_commit(&b_o);
     }
-  } else if (warp >= C::SOFT) {
+  } else if (warp >= C::SOFT && warp < C::SOFT + C::DEQ) {
     // ---- K and V from codes ----
     const int dw = warp - C::SOFT;
     bool ok = true;
@@ -457,9 +427,54 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_empty[s]);
     }
-  } else {
+  } else if (warp < C::SOFT) {
     // ---- softmax ----
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const int wq = warp >> 2, rl = 32 * (warp & 3) + lane;    // query tile and row of this thread
+    const int rr = 128 * wq + rl, rtok = rr / gs, rhead = rr % gs;
+    const bool rlive = rtok < ntok && rhead < nh;
+    float sc = 0.f;
+    {
+      // Q: the warp's 32 rows, HD / 8 lanes a row, brought to a power of two
+      // near 1 (see ck_kv_attn.cuh; the scale's sign goes to q: the largest
+      // product is the largest score) and rounded to 16 bits
+      constexpr int L = HD / 8, RW = 32 / L;
+      const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
+      const int x = lane % L, y = lane / L;
+#pragma unroll 8
+      for (int i = 0; i < 32; i += RW) {
+        const int row = 128 * wq + 32 * (warp & 3) + i + y, tok = row / gs, head = row % gs;
+        KvRaw8<KV_F16> raw;
+        raw.zero();
+        if (tok < ntok && head < nh)
+          raw.load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
+        const uint32_t u[4] = {raw.u[0].x, raw.u[0].y, raw.u[0].z, raw.u[0].w};
+        float2 f[4];
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          f[e] = kv_pair16(u[e], A.q.type);
+          top = fmaxf(top, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
+        }
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = e > 127 ? 8 : max(e, -100);
+        const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
+        // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
+        const float back = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23), 1e-37f);
+#pragma unroll
+        for (int k = 0; k < RW; k++) {         // the row's own thread keeps its factor
+          const float b = __shfl_sync(0xffffffffu, back, k * L);
+          if (lane == i + k) sc = b;
+        }
+        *(uint4*)(sm + C::SQ + wq * C::QB + kvp_kmajor<128>(32 * (warp & 3) + i + y, 8 * x)) =
+            make_uint4(kv_pack2(f[0].x * up, f[0].y * up), kv_pack2(f[1].x * up, f[1].y * up),
+                       kv_pack2(f[2].x * up, f[2].y * up), kv_pack2(f[3].x * up, f[3].y * up));
+      }
+      proxy_fence_smem();
+      mbar_arrive(&b_q);
+    }
     const int rpos = pos0 + rtok;                                 // position of the row's token
     const int rlo = A.window > 0 ? max(0, rpos + 1 - A.window) : 0;
     float m = -INFINITY, l = 0.f;
@@ -468,7 +483,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     for (int j = beg[wq]; ok && j < end[wq]; j++) {
       const int it = j - beg[wq], buf = C::SB == 2 ? it & 1 : wq, ph = C::SB == 2 ? (it >> 1) & 1 : it & 1;
       const uint32_t tS = tmem + buf * C::PT + lanes;
-      const int vlo = rlo - j * C::PT, vhi = rlive ? rpos - j * C::PT : -1;   // visible columns: vlo .. vhi
+      // visible columns: vlo .. vhi (rows of no token see all: their results go nowhere)
+      const int vlo = rlive ? rlo - j * C::PT : 0, vhi = rlive ? rpos - j * C::PT : C::PT;
       ok = kvp_wait<true>(&b_s[buf], ph, &s_fail, A.pool.err);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
@@ -482,58 +498,74 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         if ((miss >> ((c >> 4) + 1)) & 1) v &= 0x0000ffffu;
         return v;
       };
-      float mx = -INFINITY;
+      uint64_t sum2 = kvp_pair(0.f, 0.f);
+      const uint64_t sc2 = kvp_pair(sc, sc);
 #pragma unroll 1
-      for (int c = 0; c < C::PT; c += 32) {
-        uint32_t x[32];
-        tmem_ld32(tS + c, x);
+      for (int c = 0; c < C::PT; c += 64) {
+        uint32_t x[64];
+        tmem_ld32_nowait(tS + c, *(uint32_t (*)[32])&x[0]);
+        tmem_ld32_nowait(tS + c + 32, *(uint32_t (*)[32])&x[32]);
+        const uint64_t v = edge ? seen(c) | ((uint64_t)seen(c + 32) << 32) : ~0ull;
+        tmem_ld_wait(x);
         if (edge) {
-          const uint32_t v = seen(c);
 #pragma unroll
-          for (int e = 0; e < 32; e++)
-            if ((v >> e) & 1) mx = fmaxf(mx, __uint_as_float(x[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(x[e]));
+          for (int e = 0; e < 64; e++)
+            if (!((v >> e) & 1)) x[e] = 0xff800000u;
         }
-      }
-      mx = mx == -INFINITY ? mx : mx * sc;
-      if (__any_sync(0xffffffffu, mx > m + KVP_SLACK)) {
-        const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
-        m = mn;
-        l *= a;
-        if (it > 0) {
-          if (C::SB == 2) ok = kvp_wait<true>(&b_pv, (it - 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
-          if (!ok) break;
-          asm volatile("tcgen05.fence::after_thread_sync;");
-#pragma unroll 1
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t x[32];
-            tmem_ld32(tO + c, x);
+        float mx = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 32; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * a);
-            tmem_st32(tO + c, x);
+        for (int e = 0; e < 64; e += 2) mx = kvp_max3(mx, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+        mx = mx == -INFINITY ? mx : mx * sc;
+        if (__any_sync(0xffffffffu, mx > m + KVP_SLACK)) {
+          // move the reference
+          const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
+          m = mn;
+          l *= a;
+          sum2 = kvp_fma2(sum2, kvp_pair(a, a), kvp_pair(0.f, 0.f));
+          if (c > 0) {                                            // P of the columns before
+            uint32_t y[32];
+            tmem_ld32_nowait(tS, y);
+            tmem_ld_wait(y);
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              const float2 p = __half22float2(*(const __half2*)&y[e]);
+              y[e] = kv_pack2(p.x * a, p.y * a);
+            }
+            tmem_st32(tS, y);
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        }
-      }
-      const float mb = m == -INFINITY ? 0.f : m;
+          if (it > 0) {
+            if (C::SB == 2) ok = kvp_wait<true>(&b_pv, (it - 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
+            asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
-      for (int c = 0; c < C::PT; c += 32) {
-        uint32_t x[32], y[16];
-        tmem_ld32(tS + c, x);
-        const uint32_t v = edge ? seen(c) : 0xffffffffu;
+            for (int d = 0; d < HD; d += 32) {
+              uint32_t y[32];
+              tmem_ld32_nowait(tO + d, y);
+              tmem_ld_wait(y);
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float p0 = kv_ex2(fmaf(__uint_as_float(x[2 * e]), sc, -mb)), p1 = kv_ex2(fmaf(__uint_as_float(x[2 * e + 1]), sc, -mb));
-          if (edge) {
-            if (!((v >> (2 * e)) & 1)) p0 = 0.f;
-            if (!((v >> (2 * e + 1)) & 1)) p1 = 0.f;
+              for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * a);
+              tmem_st32(tO + d, y);
+            }
           }
-          l += p0 + p1;
-          y[e] = kv_pack2(p0, p1);
         }
-        tmem_st16(tS + c / 2, y);                                 // behind what this thread still has to read
+        const float mb = m == -INFINITY ? 0.f : m;
+        const uint64_t mb2 = kvp_pair(-mb, -mb);
+        uint32_t y[32];
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          float p, q;
+          kvp_split(kvp_fma2(kvp_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, mb2), p, q);
+          p = kv_ex2(p);
+          q = kv_ex2(q);
+          sum2 = kvp_add2(sum2, kvp_pair(p, q));
+          y[e / 2] = kv_pack2(p, q);
+        }
+        tmem_st32(tS + c / 2, y);                                 // behind what this thread still has to read
+      }
+      if (!ok) break;
+      {
+        float s0, s1;
+        kvp_split(sum2, s0, s1);
+        l += s0 + s1;
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
@@ -545,12 +577,13 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     if (ok) {
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const size_t off = (size_t)(q0 + rtok) * A.o.st + (size_t)(h0 + rhead) * A.o.sh;
-      const bool vec = kv_vec4(A.o);
+      const bool vec = kv_vec8(A.o);
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t x[32];
         if (beg[wq] < end[wq]) {
-          tmem_ld32(tO + c, x);
+          tmem_ld32_nowait(tO + c, x);
+          tmem_ld_wait(x);
         } else {
 #pragma unroll
           for (int e = 0; e < 32; e++) x[e] = 0u;
@@ -561,12 +594,14 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           for (int e = 0; e < 32; e += 4) *(uint4*)(part + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
         } else if (rlive) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            kv_st4(A.o, off + c + e,
-                   l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                            : make_float4(__uint_as_float(x[e]) * inv, __uint_as_float(x[e + 1]) * inv,
-                                          __uint_as_float(x[e + 2]) * inv, __uint_as_float(x[e + 3]) * inv),
-                   vec);
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t u[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+              u[k] = l == 0.f ? 0u
+                              : kv_to16(__uint_as_float(x[e + 2 * k]) * inv, __uint_as_float(x[e + 2 * k + 1]) * inv, A.o.type);
+            kv_put8(A.o.p, off + c + e, u, vec);
+          }
         }
       }
       if (splits > 1)
