@@ -42,6 +42,9 @@ size_t kv_pool_bytes(const KvPool& p) {
 #ifndef KV_STORE_WARPS
 #define KV_STORE_WARPS 4096
 #endif
+#ifndef KVP_SPLIT_TILES
+#define KVP_SPLIT_TILES 8
+#endif
 #ifndef KV_UNIT_PAIRS
 #define KV_UNIT_PAIRS 32
 #endif
@@ -172,7 +175,7 @@ cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pd
 cudaError_t kv_prompt_launch(const KvAttn& all, int sms, cudaStream_t s) {
   if (all.rows == 0) return cudaSuccess;
   const int gsz = all.heads / all.pool.kvh, hb = (gsz + 127) / 128, gs = (gsz + hb - 1) / hb;   // heads of a unit
-  const int units = all.pool.kvh * hb, bt = (all.pool.hd == 256 ? 128 : 256) / gs, pt = all.pool.hd == 256 ? 64 : 128;
+  const int units = all.pool.kvh * hb, bt = (all.pool.hd == 256 ? 128 : 256) / gs, pt = 64;
   for (int i0 = 0; i0 < all.n; i0 += KVP_MAXS) {
     KvAttn a = all;
     a.n = all.n - i0 < KVP_MAXS ? all.n - i0 : KVP_MAXS;
@@ -182,12 +185,11 @@ cudaError_t kv_prompt_launch(const KvAttn& all, int sms, cudaStream_t s) {
     a.tab.n_seqs -= i0;
     // tiles: at most a partial one per sequence.  The cached length is split
     // when they leave more than half of the SMs idle: what can be split (the
-    // block table's width) into at least 4 position tiles a CTA, as joining
-    // costs about as much as 3 of them
+    // block table's width) into at least KVP_SPLIT_TILES position tiles a CTA
     const long long ctas = ((long long)a.rows / bt + a.n) * units;
     const long long tiles = ((long long)a.tab.max_blocks * a.pool.block + pt - 1) / pt;
     long long splits = ctas ? sms / ctas : 1;
-    if (splits > tiles / 4) splits = tiles / 4;
+    if (splits > tiles / KVP_SPLIT_TILES) splits = tiles / KVP_SPLIT_TILES;
     if (splits < 1) splits = 1;
     if (ctas * splits > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)(ctas * splits));

@@ -12,21 +12,22 @@
 // side by side, on warps of their own:
 //   1 warp    copies records (16 positions of a kv head, one bulk copy each)
 //             through KvPr::STAGES staging buffers
-//   4 or 8    turn codes into fp16 operand tiles (the same arithmetic for both:
-//             V is fed to the second product as it lies, its dims contiguous)
-//   1 thread  issues the products
-//   4 or 8    softmax: a thread owns a query row; it reads S from tensor
-//             memory once, 64 columns at a time, and writes P over what it
-//             has read as the second product's operand.  The exponentials
-//             are taken against a reference maximum that is moved (and O, l
-//             and the tile's earlier P rescaled) only where a score passes
-//             it by 2^8, and for the first scores
+//   4 or 8    turn codes into fp16 operand tiles of 64 positions (the same
+//             arithmetic for both: V is fed to the second product as it lies,
+//             its dims contiguous), K a tile ahead of V
+//   1 thread  issues the products: a tile's scores before the output of the
+//             tile before, so that they are there when the softmax comes to
+//             them (two score buffers a query tile)
+//   4 or 8    softmax: a thread owns a query row; it reads its 64 scores from
+//             tensor memory once and writes P over them as the second
+//             product's operand.  The exponentials are taken against a
+//             reference maximum that is moved (and O and l rescaled) only
+//             where a score passes it by 2^8, and for the first tile
 // A CTA holds 256 query rows (two tiles, whose products and softmaxes take
-// turns; the K and V tiles serve both) or, at head_dim 256, 128 rows with two
-// score buffers (the next scores are computed under the present softmax).  A
-// query row is a (token, head of the kv head's group) pair, so the group
-// shares K and V.  CTAs are numbered by depth (position of the tile within
-// its sequence), the deepest first: they take longest.
+// turns; the K and V tiles serve both) or, at head_dim 256, 128.  A query row
+// is a (token, head of the kv head's group) pair, so the group shares K and V.
+// CTAs are numbered by depth (position of the tile within its sequence), the
+// deepest first: they take longest.
 //
 // Long caches with few rows would leave SMs idle: the cached positions are
 // then split over several CTAs, which leave unnormalised partial rows for
@@ -41,19 +42,19 @@ template <int HD, int VB>
 struct KvPr {
   using R = KvRec<HD, VB>;
   static constexpr int NQ = HD == 256 ? 1 : 2;            // 128-row query tiles
-  static constexpr int PT = HD == 256 ? 64 : 128;         // positions of a K / V tile
-  static constexpr int SB = NQ == 1 ? 2 : 1;              // score buffers of a query tile
+  static constexpr int PT = 64;                           // positions of a K / V tile
+  static constexpr int BUF = HD == 256 ? 1 : 2;           // K and V tiles
   static constexpr int SOFT = 4 * NQ, DEQ = 12 - SOFT;    // warps
   static constexpr int THREADS = (SOFT + DEQ + 2) * 32;
   static constexpr int RECS = PT / KV_TILE;
-  static constexpr int STAGES = HD == 64 ? 4 : 2;
   static constexpr int STAGE_BYTES = RECS * R::BYTES;
+  static constexpr int STAGES = HD == 256 ? 2 : 4;
   static constexpr int QB = 128 * HD * 2, KB = PT * HD * 2;
-  static constexpr int SQ = 0, SK = NQ * QB, SV = SK + KB, SST = SV + KB;
+  static constexpr int SQ = 0, SK = NQ * QB, SV = SK + BUF * KB, SST = SV + BUF * KB;
   // at least 120 KB, so that an SM holds one CTA (each takes all of its tensor memory)
   static constexpr int NEED = SST + STAGES * STAGE_BYTES;
   static constexpr int SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;
-  static constexpr int TO = NQ * SB * PT;                 // tensor memory: score buffers, then O
+  static constexpr int TO = NQ * 2 * PT;                  // tensor memory: two score buffers a query tile, then O
   static_assert(TO + NQ * HD <= 512, "tensor memory");
   static_assert(SMEM <= 227 * 1024 - 1024, "shared memory");
 };
@@ -140,8 +141,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
   __shared__ int s_seq, s_tile;
-  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k, b_kfree, b_v, b_vfree, b_s[2], b_p[2],
-      b_o, b_pv, b_end;
+  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_kfree[C::BUF],
+      b_v[C::BUF], b_vfree[C::BUF], b_s[C::NQ][2], b_p[C::NQ][2], b_pv[C::NQ], b_o, b_end;
   __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 4 ahead)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bt = 128 * C::NQ / gs;             // tokens of a CTA
@@ -245,16 +246,20 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       mbar_init(&b_empty[i], C::DEQ);
     }
     mbar_init(&b_q, C::SOFT * 32);
-    mbar_init(&b_k, C::DEQ * 32);
-    mbar_init(&b_v, C::DEQ * 32);
-    mbar_init(&b_kfree, 1);
-    mbar_init(&b_vfree, 1);
-    mbar_init(&b_s[0], 1);
-    mbar_init(&b_s[1], 1);
-    mbar_init(&b_p[0], 128);
-    mbar_init(&b_p[1], 128);
+    for (int i = 0; i < C::BUF; i++) {
+      mbar_init(&b_k[i], C::DEQ * 32);
+      mbar_init(&b_v[i], C::DEQ * 32);
+      mbar_init(&b_kfree[i], 1);
+      mbar_init(&b_vfree[i], 1);
+    }
+    for (int w = 0; w < C::NQ; w++) {
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&b_s[w][i], 1);
+        mbar_init(&b_p[w][i], 128);
+      }
+      mbar_init(&b_pv[w], 1);
+    }
     mbar_init(&b_o, 1);
-    mbar_init(&b_pv, 1);
     mbar_init(&b_end, 1);
     mbar_fence_init();
   }
@@ -298,135 +303,180 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         for (unsigned spins = 0; !mbar_try_wait(&b_full[s], 0) && !mbar_try_wait(&b_full[s], 1) && spins < (1u << 20); spins++) {}
   } else if (warp == C::SOFT + C::DEQ) {
     // ---- products ----
-    if (lane == 0) {
-      const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
-      const uint32_t idO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);   // V's dims are contiguous
-      bool ok = jb >= je || kvp_wait<false>(&b_q, 0, &s_fail, A.pool.err);
-      auto scores = [&](int w, int buf) {
+    // The whole warp runs the loop and one elected lane issues: operands that
+    // the compiler sees to be the same in every lane go to the tensor core
+    // from uniform registers (from a lone thread's branch each product cost
+    // about 70 cycles to issue, more than it takes).
+    const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
+    const uint32_t idO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);   // V's dims are contiguous
+    const int n = __shfl_sync(0xffffffffu, je - jb, 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    int from[C::NQ], to[C::NQ];                // tiles of each query tile, counted from jb
 #pragma unroll
-        for (int k = 0; k < HD / 16; k++)
-          umma_f16(tmem + buf * C::PT, umma_desc(smem_u32(sm + C::SQ + w * C::QB + k * 4096), 128, 256),
-                   umma_desc(smem_u32(sm + C::SK + k * C::PT * 32), 128, 256), idS, k > 0 ? 1u : 0u);
-        umma_commit(&b_s[buf]);
-      };
-      auto output = [&](int w, int buf, bool first) {
-#pragma unroll
-        for (int k = 0; k < C::PT / 16; k++)
-          umma_f16_ts(tmem + C::TO + w * HD, tmem + buf * C::PT + 8 * k,
-                      umma_desc(smem_u32(sm + C::SV + k * 2 * HD * 16), HD * 16, 128), idO, first && k == 0 ? 0u : 1u);
-      };
-      if (C::NQ == 2) {
-        for (int j = jb; ok && j <= je; j++) {
-          bool kw = false, vw = false;
-          for (int w = 0; ok && w < C::NQ; w++) {
-            if (j - 1 >= beg[w] && j - 1 < end[w]) {          // O += P V of the tile before
-              if (!vw) ok = kvp_wait<false>(&b_v, (j - 1 - jb) & 1, &s_fail, A.pool.err);
-              vw = true;
-              ok = ok && kvp_wait<false>(&b_p[w], (j - 1 - beg[w]) & 1, &s_fail, A.pool.err);
-              if (!ok) break;
-              asm volatile("tcgen05.fence::after_thread_sync;");
-              output(w, w, j - 1 == beg[w]);
-            }
-            if (j < je && j >= beg[w] && j < end[w]) {
-              if (!kw) ok = kvp_wait<false>(&b_k, (j - jb) & 1, &s_fail, A.pool.err);
-              kw = true;
-              if (!ok) break;
-              asm volatile("tcgen05.fence::after_thread_sync;");
-              scores(w, w);
-            }
-          }
-          if (!ok) break;
-          if (j > jb) umma_commit(&b_vfree);
-          if (j < je) umma_commit(&b_kfree);
-        }
-      } else {
-        const int n = je - jb;
-        for (int j = 0; ok && j <= n; j++) {
-          if (j < n) {                                        // the next scores before this tile's output
-            ok = kvp_wait<false>(&b_k, j & 1, &s_fail, A.pool.err);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            scores(0, j & 1);
-            umma_commit(&b_kfree);
-          }
-          if (j > 0) {
-            ok = kvp_wait<false>(&b_v, (j - 1) & 1, &s_fail, A.pool.err) &&
-                 kvp_wait<false>(&b_p[(j - 1) & 1], ((j - 1) >> 1) & 1, &s_fail, A.pool.err);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            output(0, (j - 1) & 1, j == 1);
-            umma_commit(&b_vfree);
-            umma_commit(&b_pv);
-          }
-        }
-      }
-      umma_commit(&b_o);
+    for (int w = 0; w < C::NQ; w++) {
+      from[w] = __shfl_sync(0xffffffffu, beg[w] - jb, 0);
+      to[w] = __shfl_sync(0xffffffffu, end[w] - jb, 0);
     }
+    const bool leader = elect_one();
+    bool ok = n <= 0 || kvp_wait<true>(&b_q, 0, &s_fail, A.pool.err);
+    // descriptors: a step of 16 further along is so many 16-byte units on
+    const uint64_t dq = umma_desc(smem_u32(sm + C::SQ), 128, 256), dk = umma_desc(smem_u32(sm + C::SK), 128, 256);
+    const uint64_t dv = umma_desc(smem_u32(sm + C::SV), HD * 16, 128);
+#pragma unroll 1
+    for (int it = 0; ok && it <= n; it++) {
+      if (it < n) {
+        const int kb = it & (C::BUF - 1);
+        ok = kvp_wait<true>(&b_k[kb], (it / C::BUF) & 1, &s_fail, A.pool.err);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+        for (int w = 0; w < C::NQ; w++)
+          if (it >= from[w] && it < to[w]) {
+            const int buf = (it - from[w]) & 1;
+            const uint32_t d = tm + (2 * w + buf) * C::PT;
+            const uint64_t bd = dk + kb * (C::KB / 16);
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < HD / 16; k++)
+                umma_f16(d, dq + (w * C::QB + k * 4096) / 16, bd + k * C::PT * 32 / 16, idS, k > 0 ? 1u : 0u);
+              umma_commit(&b_s[w][buf]);
+            }
+            __syncwarp();
+          }
+        if (leader) umma_commit(&b_kfree[kb]);
+        __syncwarp();
+      }
+      if (it > 0) {
+        const int vb = (it - 1) & (C::BUF - 1);
+        ok = kvp_wait<true>(&b_v[vb], ((it - 1) / C::BUF) & 1, &s_fail, A.pool.err);
+#pragma unroll
+        for (int w = 0; w < C::NQ; w++)
+          if (ok && it - 1 >= from[w] && it - 1 < to[w]) {
+            const int i = it - 1 - from[w], buf = i & 1;
+            ok = kvp_wait<true>(&b_p[w][buf], (i >> 1) & 1, &s_fail, A.pool.err);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            const uint32_t ad = tm + (2 * w + buf) * C::PT;
+            const uint64_t bd = dv + vb * (C::KB / 16);
+            if (leader) {
+#pragma unroll
+              for (int k = 0; k < C::PT / 16; k++)
+                umma_f16_ts(tm + C::TO + w * HD, ad + 8 * k, bd + k * 2 * HD * 16 / 16, idO, i == 0 && k == 0 ? 0u : 1u);
+              umma_commit(&b_pv[w]);
+            }
+            __syncwarp();
+          }
+        if (leader) umma_commit(&b_vfree[vb]);
+        __syncwarp();
+      }
+    }
+    if (leader) umma_commit(&b_o);
+    __syncwarp();
   } else if (warp >= C::SOFT && warp < C::SOFT + C::DEQ) {
     // ---- K and V from codes ----
-    const int dw = warp - C::SOFT;
-    bool ok = true;
-    for (int j = jb; ok && j < je; j++) {
-      const int it = j - jb, s = it % C::STAGES;
+    // A record's codes are cut into pieces of 8 positions x 64 dims (V in 4
+    // bits: 128 dims; at head_dim 64, 16 positions): a lane takes 16 bytes of
+    // codes.  A warp takes the same piece of every record (of every 2nd or 4th
+    // where a record has fewer pieces than there are warps), up to 4 pieces'
+    // codes in registers at a time, read before the tile they go to is free.
+    // K of the next tile comes before V: the scores are wanted first.
+    const int dw = warp - C::SOFT, x = lane >> 3;
+    constexpr int CH = R::VROW / 32;                         // 32-byte chunks of a position's values
+    constexpr int KP = HD / 32, VP = CH < 2 ? 1 : CH;        // pieces of a record
+    constexpr int KW = C::DEQ / KP, VW = C::DEQ / VP;        // warps that share a piece's records
+    constexpr int KN = C::RECS / KW, VN = C::RECS / VW;      // records of a warp
+    constexpr int KB = KN < 4 ? KN : 4, VB4 = VN < 4 ? VN : 4;
+    static_assert(KW >= 1 && VW >= 1 && KN % KB == 0 && VN % VB4 == 0, "pieces");
+    const int kr = dw / KP, kp = 8 * (dw % KP & 1) + (lane & 7), kg = 2 * (dw % KP >> 1) + (x >> 1);
+    const int khalf = (x & 1) ^ ((lane >> 2) & 1);           // rows 4 apart share their banks: they take the other half
+    const int ksrc = kv_kchunk<HD>(kp, kg) + 16 * khalf, kscl = (kp * R::G + kg) * 2;
+    const int kdst = C::SK + kvp_kmajor<C::PT>(kp, 32 * kg + 16 * khalf);
+    const int vr = dw / VP, vp = CH < 2 ? 8 * (x >> 1) + (lane & 7) : 8 * (dw % VP & 1) + (lane & 7);
+    const int vc = CH < 2 ? 0 : 2 * (dw % VP >> 1) + (x >> 1), vhalf = x & 1;
+    const int vsrc = R::V + kv_vchunk<R::VROW>(vp, vc) + 16 * vhalf;
+    const int vscl = R::VS + (vp * R::G + (VB == 8 ? vc : 2 * vc)) * 2;
+    const int vdst = C::SV + kvp_vmajor<HD>(vp, (VB == 8 ? 32 * vc : 64 * vc) + 16 * vhalf);
+    auto make_k = [&](int it) {
+      const int s = it % C::STAGES, kb = it % C::BUF;
       const uint8_t* stg = sm + C::SST + s * C::STAGE_BYTES;
-      ok = kvp_wait<true>(&b_full[s], (it / C::STAGES) & 1, &s_fail, A.pool.err) &&
-           (it == 0 || kvp_wait<true>(&b_kfree, (it - 1) & 1, &s_fail, A.pool.err));
-      if (!ok) break;
-      // an item is 8 positions x 64 dims: lane = position & 7 and 16 of the dims
-#pragma unroll 2
-      for (int i = dw; i < C::PT / 8 * (HD / 64); i += C::DEQ) {
-        const int p = (i / (HD / 64)) * 8 + (lane & 7), x = lane >> 3, g = (i % (HD / 64)) * 2 + (x >> 1);
-        const int half = (x & 1) ^ ((lane >> 2) & 1);       // rows 4 apart share their banks: they take the other half
-        const uint8_t* rec = stg + (p >> 4) * R::BYTES;
-        const uint4 c = *(const uint4*)(rec + kv_kchunk<HD>(p & 15, g) + 16 * half);
-        uint32_t du = *(const unsigned short*)(rec + R::KS + ((p & 15) * R::G + g) * 2);
-        if (kvp_bad<VB>(*(const unsigned short*)(rec + R::VS + ((p & 15) * R::G + g) * 2))) du = 0x7fffu;
-        du |= du << 16;
-        uint8_t* dst = sm + C::SK + kvp_kmajor<C::PT>(p, 32 * g + 16 * half);
-        *(uint4*)dst = make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c.x), du), kv_hmul2(kv_half2<0x4342, 128>(c.x), du),
-                                  kv_hmul2(kv_half2<0x4140, 128>(c.y), du), kv_hmul2(kv_half2<0x4342, 128>(c.y), du));
-        *(uint4*)(dst + 128) =
-            make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c.z), du), kv_hmul2(kv_half2<0x4342, 128>(c.z), du),
-                       kv_hmul2(kv_half2<0x4140, 128>(c.w), du), kv_hmul2(kv_half2<0x4342, 128>(c.w), du));
-      }
-      proxy_fence_smem();
-      mbar_arrive(&b_k);
-      if (it > 0 && !kvp_wait<true>(&b_vfree, (it - 1) & 1, &s_fail, A.pool.err)) break;
-      constexpr int CH = R::VROW / 32, CP = CH < 2 ? 1 : CH / 2;   // 32-byte chunks of a position; pairs of them
-      // items: 8 positions x 2 chunks, or 16 positions of a single chunk
-#pragma unroll 2
-      for (int i = dw; i < (CH < 2 ? C::PT / 16 : C::PT / 8 * CP); i += C::DEQ) {
-        const int x = lane >> 3;
-        const int p = CH < 2 ? i * 16 + (x >> 1) * 8 + (lane & 7) : (i / CP) * 8 + (lane & 7);
-        const int c = CH < 2 ? 0 : (i % CP) * 2 + (x >> 1);
-        const int half = x & 1;
-        const uint8_t* rec = stg + (p >> 4) * R::BYTES;
-        const uint4 w = *(const uint4*)(rec + R::V + kv_vchunk<R::VROW>(p & 15, c) + 16 * half);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+      bool ok = kvp_wait<true>(&b_full[s], (it / C::STAGES) & 1, &s_fail, A.pool.err);
+      if (!ok) return false;
 #pragma unroll
-        for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
-          const int g = VB == 8 ? c : 2 * c + nib;
-          uint32_t d = *(const unsigned short*)(rec + R::VS + ((p & 15) * R::G + g) * 2);
-          if (kvp_bad<VB>(d) || j * C::PT + p >= len) d = 0;
-          d |= d << 16;
-          constexpr int BIAS = VB == 8 ? 128 : 8;
-          uint32_t o[8];
+      for (int k0 = 0; k0 < KN; k0 += KB) {
+        uint4 c[KB];
+        uint32_t d[KB];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const uint32_t u = VB == 8 ? ww[e] : (ww[e] >> (4 * nib)) & 0x0f0f0f0fu;
-            o[2 * e] = kv_hmul2(kv_half2<0x4140, BIAS>(u), d);
-            o[2 * e + 1] = kv_hmul2(kv_half2<0x4342, BIAS>(u), d);
-          }
-          uint8_t* dst = sm + C::SV + kvp_vmajor<HD>(p, 32 * g + 16 * half);
-          *(uint4*)dst = make_uint4(o[0], o[1], o[2], o[3]);
-          *(uint4*)(dst + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+        for (int k = 0; k < KB; k++) {
+          const uint8_t* rec = stg + (kr + (k0 + k) * KW) * R::BYTES;
+          c[k] = *(const uint4*)(rec + ksrc);
+          d[k] = *(const unsigned short*)(rec + R::KS + kscl);
+          if (kvp_bad<VB>(*(const unsigned short*)(rec + R::VS + kscl))) d[k] = 0x7fffu;
+          d[k] |= d[k] << 16;
+        }
+        if (k0 == 0 && it >= C::BUF) ok = kvp_wait<true>(&b_kfree[kb], (it / C::BUF - 1) & 1, &s_fail, A.pool.err);
+        if (!ok) return false;
+#pragma unroll
+        for (int k = 0; k < KB; k++) {
+          uint8_t* dst = sm + kdst + kb * C::KB + (kr + (k0 + k) * KW) * 512;
+          *(uint4*)dst =
+              make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c[k].x), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].x), d[k]),
+                         kv_hmul2(kv_half2<0x4140, 128>(c[k].y), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].y), d[k]));
+          *(uint4*)(dst + 128) =
+              make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c[k].z), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].z), d[k]),
+                         kv_hmul2(kv_half2<0x4140, 128>(c[k].w), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].w), d[k]));
         }
       }
       proxy_fence_smem();
-      mbar_arrive(&b_v);
+      mbar_arrive(&b_k[kb]);
+      return true;
+    };
+    auto make_v = [&](int it) {
+      const int s = it % C::STAGES, vb = it % C::BUF, j = jb + it;
+      const uint8_t* stg = sm + C::SST + s * C::STAGE_BYTES;
+      bool ok = true;
+#pragma unroll
+      for (int k0 = 0; k0 < VN; k0 += VB4) {
+        uint4 c[VB4];
+        uint32_t d[VB4][2];
+#pragma unroll
+        for (int k = 0; k < VB4; k++) {
+          const int rec = vr + (k0 + k) * VW;
+          c[k] = *(const uint4*)(stg + rec * R::BYTES + vsrc);
+#pragma unroll
+          for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
+            uint32_t e = *(const unsigned short*)(stg + rec * R::BYTES + vscl + 2 * nib);
+            if (kvp_bad<VB>(e) || j * C::PT + rec * KV_TILE + vp >= len) e = 0;
+            d[k][nib] = e | (e << 16);
+          }
+        }
+        if (k0 == 0 && it >= C::BUF) ok = kvp_wait<true>(&b_vfree[vb], (it / C::BUF - 1) & 1, &s_fail, A.pool.err);
+        if (!ok) return false;
+#pragma unroll
+        for (int k = 0; k < VB4; k++) {
+          uint8_t* dst = sm + vdst + vb * C::KB + (vr + (k0 + k) * VW) * (HD * 32);
+          const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
+#pragma unroll
+          for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
+            uint32_t o[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              o[2 * e] = kv_hmul2(kv_code2<VB>(__byte_perm(w[e], 0x64646464u, 0x4140), nib), d[k][nib]);
+              o[2 * e + 1] = kv_hmul2(kv_code2<VB>(__byte_perm(w[e], 0x64646464u, 0x4342), nib), d[k][nib]);
+            }
+            // the other group of a 4-bit chunk: 32 dims on
+            *(uint4*)(dst + nib * 512) = make_uint4(o[0], o[1], o[2], o[3]);
+            *(uint4*)(dst + nib * 512 + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+        }
+      }
+      proxy_fence_smem();
+      mbar_arrive(&b_v[vb]);
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_empty[s]);
-    }
+      return true;
+    };
+    bool ok = jb >= je || make_k(0);
+    for (int it = 0; ok && it < je - jb; it++) ok = (it + 1 >= je - jb || make_k(it + 1)) && make_v(it);
   } else if (warp < C::SOFT) {
     // ---- softmax ----
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -441,36 +491,44 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       constexpr int L = HD / 8, RW = 32 / L;
       const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
       const int x = lane % L, y = lane / L;
-#pragma unroll 8
-      for (int i = 0; i < 32; i += RW) {
-        const int row = 128 * wq + 32 * (warp & 3) + i + y, tok = row / gs, head = row % gs;
-        KvRaw8<KV_F16> raw;
-        raw.zero();
-        if (tok < ntok && head < nh)
-          raw.load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
-        const uint32_t u[4] = {raw.u[0].x, raw.u[0].y, raw.u[0].z, raw.u[0].w};
-        float2 f[4];
-        float top = 0.f;
+      constexpr int B = 8;                      // loads in flight
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += B * RW) {
+        KvRaw8<KV_F16> raw[B];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          f[e] = kv_pair16(u[e], A.q.type);
-          top = fmaxf(top, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
+        for (int n = 0; n < B; n++) {
+          const int row = 128 * wq + 32 * (warp & 3) + i0 + n * RW + y, tok = row / gs, head = row % gs;
+          raw[n].zero();
+          if (tok < ntok && head < nh)
+            raw[n].load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
         }
 #pragma unroll
-        for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        int e = (int)(__float_as_uint(top) >> 23) - 127;
-        e = e > 127 ? 8 : max(e, -100);
-        const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
-        // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
-        const float back = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23), 1e-37f);
+        for (int n = 0; n < B; n++) {
+          const int i = i0 + n * RW;
+          const uint32_t u[4] = {raw[n].u[0].x, raw[n].u[0].y, raw[n].u[0].z, raw[n].u[0].w};
+          float2 f[4];
+          float top = 0.f;
 #pragma unroll
-        for (int k = 0; k < RW; k++) {         // the row's own thread keeps its factor
-          const float b = __shfl_sync(0xffffffffu, back, k * L);
-          if (lane == i + k) sc = b;
+          for (int e = 0; e < 4; e++) {
+            f[e] = kv_pair16(u[e], A.q.type);
+            top = fmaxf(top, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
+          }
+#pragma unroll
+          for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          int e = (int)(__float_as_uint(top) >> 23) - 127;
+          e = e > 127 ? 8 : max(e, -100);
+          const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
+          // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
+          const float back = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23), 1e-37f);
+#pragma unroll
+          for (int k = 0; k < RW; k++) {       // the row's own thread keeps its factor
+            const float b = __shfl_sync(0xffffffffu, back, k * L);
+            if (lane == i + k) sc = b;
+          }
+          *(uint4*)(sm + C::SQ + wq * C::QB + kvp_kmajor<128>(32 * (warp & 3) + i + y, 8 * x)) =
+              make_uint4(kv_pack2(f[0].x * up, f[0].y * up), kv_pack2(f[1].x * up, f[1].y * up),
+                         kv_pack2(f[2].x * up, f[2].y * up), kv_pack2(f[3].x * up, f[3].y * up));
         }
-        *(uint4*)(sm + C::SQ + wq * C::QB + kvp_kmajor<128>(32 * (warp & 3) + i + y, 8 * x)) =
-            make_uint4(kv_pack2(f[0].x * up, f[0].y * up), kv_pack2(f[1].x * up, f[1].y * up),
-                       kv_pack2(f[2].x * up, f[2].y * up), kv_pack2(f[3].x * up, f[3].y * up));
       }
       proxy_fence_smem();
       mbar_arrive(&b_q);
@@ -481,11 +539,11 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     const uint32_t tO = tmem + C::TO + wq * HD + lanes;
     bool ok = true;
     for (int j = beg[wq]; ok && j < end[wq]; j++) {
-      const int it = j - beg[wq], buf = C::SB == 2 ? it & 1 : wq, ph = C::SB == 2 ? (it >> 1) & 1 : it & 1;
-      const uint32_t tS = tmem + buf * C::PT + lanes;
+      const int it = j - beg[wq], buf = it & 1;
+      const uint32_t tS = tmem + (2 * wq + buf) * C::PT + lanes;
       // visible columns: vlo .. vhi (rows of no token see all: their results go nowhere)
       const int vlo = rlive ? rlo - j * C::PT : 0, vhi = rlive ? rpos - j * C::PT : C::PT;
-      ok = kvp_wait<true>(&b_s[buf], ph, &s_fail, A.pool.err);
+      ok = kvp_wait<true>(&b_s[wq][buf], (it >> 1) & 1, &s_fail, A.pool.err);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
       const uint32_t miss = s_miss[j & 7];
@@ -498,57 +556,47 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         if ((miss >> ((c >> 4) + 1)) & 1) v &= 0x0000ffffu;
         return v;
       };
-      uint64_t sum2 = kvp_pair(0.f, 0.f);
-      const uint64_t sc2 = kvp_pair(sc, sc);
+      uint32_t x[64];
+      tmem_ld32_nowait(tS, *(uint32_t (*)[32])&x[0]);
+      tmem_ld32_nowait(tS + 32, *(uint32_t (*)[32])&x[32]);
+      const uint64_t v = edge ? seen(0) | ((uint64_t)seen(32) << 32) : ~0ull;
+      tmem_ld_wait(x);
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 64; e++)
+          if (!((v >> e) & 1)) x[e] = 0xff800000u;
+      }
+      float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        mx = kvp_max3(mx, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+        my = kvp_max3(my, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+      }
+      mx = fmaxf(mx, my);
+      mx = mx == -INFINITY ? mx : mx * sc;
+      if (__any_sync(0xffffffffu, mx > m + KVP_SLACK)) {          // move the reference
+        const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
+        m = mn;
+        l *= a;
+        if (it > 0) {
+          ok = kvp_wait<true>(&b_pv[wq], (it - 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
-      for (int c = 0; c < C::PT; c += 64) {
-        uint32_t x[64];
-        tmem_ld32_nowait(tS + c, *(uint32_t (*)[32])&x[0]);
-        tmem_ld32_nowait(tS + c + 32, *(uint32_t (*)[32])&x[32]);
-        const uint64_t v = edge ? seen(c) | ((uint64_t)seen(c + 32) << 32) : ~0ull;
-        tmem_ld_wait(x);
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < 64; e++)
-            if (!((v >> e) & 1)) x[e] = 0xff800000u;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 64; e += 2) mx = kvp_max3(mx, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-        mx = mx == -INFINITY ? mx : mx * sc;
-        if (__any_sync(0xffffffffu, mx > m + KVP_SLACK)) {
-          // move the reference
-          const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
-          m = mn;
-          l *= a;
-          sum2 = kvp_fma2(sum2, kvp_pair(a, a), kvp_pair(0.f, 0.f));
-          if (c > 0) {                                            // P of the columns before
+          for (int d = 0; d < HD; d += 32) {
             uint32_t y[32];
-            tmem_ld32_nowait(tS, y);
+            tmem_ld32_nowait(tO + d, y);
             tmem_ld_wait(y);
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-              const float2 p = __half22float2(*(const __half2*)&y[e]);
-              y[e] = kv_pack2(p.x * a, p.y * a);
-            }
-            tmem_st32(tS, y);
-          }
-          if (it > 0) {
-            if (C::SB == 2) ok = kvp_wait<true>(&b_pv, (it - 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
-            asm volatile("tcgen05.fence::after_thread_sync;");
-#pragma unroll 1
-            for (int d = 0; d < HD; d += 32) {
-              uint32_t y[32];
-              tmem_ld32_nowait(tO + d, y);
-              tmem_ld_wait(y);
-#pragma unroll
-              for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * a);
-              tmem_st32(tO + d, y);
-            }
+            for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * a);
+            tmem_st32(tO + d, y);
           }
         }
+      }
+      uint64_t sum2 = kvp_pair(0.f, 0.f), sum3 = sum2;
+      {
         const float mb = m == -INFINITY ? 0.f : m;
-        const uint64_t mb2 = kvp_pair(-mb, -mb);
+        const uint64_t sc2 = kvp_pair(sc, sc), mb2 = kvp_pair(-mb, -mb);
         uint32_t y[32];
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
@@ -556,12 +604,13 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           kvp_split(kvp_fma2(kvp_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, mb2), p, q);
           p = kv_ex2(p);
           q = kv_ex2(q);
-          sum2 = kvp_add2(sum2, kvp_pair(p, q));
+          if (e & 2) sum3 = kvp_add2(sum3, kvp_pair(p, q));
+          else sum2 = kvp_add2(sum2, kvp_pair(p, q));
           y[e / 2] = kv_pack2(p, q);
         }
-        tmem_st32(tS + c / 2, y);                                 // behind what this thread still has to read
+        tmem_st32(tS, y);
       }
-      if (!ok) break;
+      sum2 = kvp_add2(sum2, sum3);
       {
         float s0, s1;
         kvp_split(sum2, s0, s1);
@@ -569,7 +618,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
-      mbar_arrive(&b_p[buf]);
+      mbar_arrive(&b_p[wq][buf]);
     }
     // O / l, or this CTA's part of it
     if (ok && beg[wq] < end[wq]) ok = kvp_wait<true>(&b_o, 0, &s_fail, A.pool.err);
@@ -611,7 +660,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   }
   // no CTA leaves, or frees its tensor memory, with a product in flight
   __syncthreads();
-  if (warp == C::SOFT + C::DEQ && lane == 0) umma_commit(&b_end);
+  if (warp == C::SOFT + C::DEQ && elect_one()) umma_commit(&b_end);
   if (warp == 0) {
     unsigned spins = 0;
     while (!mbar_try_wait(&b_end, 0) && ++spins < (1u << 20)) {}
