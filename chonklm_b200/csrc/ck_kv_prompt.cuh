@@ -140,52 +140,70 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
-  __shared__ int s_seq, s_tile;
-  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_kfree[C::BUF],
-      b_v[C::BUF], b_vfree[C::BUF], b_s[C::NQ][2], b_p[C::NQ][2], b_pv[C::NQ], b_o, b_end;
-  __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 4 ahead)
+  __shared__ int s_seq, s_tile, s_cu0, s_cu1, s_len;
+  __shared__ float s_scale[128 * C::NQ];       // factor of each query row's scores
+  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_v[C::BUF], b_s[2], b_p[2],
+      b_pv[2], b_o, b_end;
+  __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 5 ahead)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bt = 128 * C::NQ / gs;             // tokens of a CTA
   const int unit = blockIdx.x % units, zb = blockIdx.x / units, z = zb % splits, b = zb / splits;
 
   if (warp == 0) {
     // tile b, deepest first: D with f(D + 1) <= b < f(D), f(D) = tiles at depth >= D
-    auto depth = [&](int s) {
-      const int r = A.cu[s + 1] - A.cu[s];
-      return r > 0 ? (r + bt - 1) / bt : 0;
-    };
-    const int mine = lane < A.n ? depth(lane) : 0;
+    auto depth = [&](int c0, int c1) { return c1 > c0 ? (c1 - c0 + bt - 1) / bt : 0; };
+    // up to 32 sequences' rows stay in registers
+    const bool in = lane < A.n;
+    const int c0 = in ? A.cu[lane] : 0, c1 = in ? A.cu[lane + 1] : 0, ln = in ? A.len[lane] : 0;
+    const int mine = depth(c0, c1);
     auto above = [&](int d) {
       int c = max(0, mine - d);
-      for (int s = lane + 32; s < A.n; s += 32) c += max(0, depth(s) - d);
+      for (int s = lane + 32; s < A.n; s += 32) c += max(0, depth(A.cu[s], A.cu[s + 1]) - d);
       return __reduce_add_sync(0xffffffffu, c);
     };
-    int lo = -1, hi = A.rows / bt + 1;         // f(lo) > b >= f(hi)
-    if (above(0) <= b) {
-      hi = -1;
-    } else {
-      lo = 0;
+    int lo = 0, seq = -1, most = mine;         // f(lo) > b >= f(hi)
+    for (int s = lane + 32; s < A.n; s += 32) most = max(most, depth(A.cu[s], A.cu[s + 1]));
+    int hi = __reduce_max_sync(0xffffffffu, most);
+    if (above(0) > b) {
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (above(mid) > b) lo = mid; else hi = mid;
       }
-    }
-    int seq = -1;
-    if (hi >= 0) {
       int k = b - above(lo + 1);               // the k-th sequence with more than lo tiles
       for (int s0 = 0; s0 < A.n && seq < 0; s0 += 32) {
         const int s = s0 + lane;
-        const uint32_t has = __ballot_sync(0xffffffffu, s < A.n && depth(s) > lo);
+        const uint32_t has = __ballot_sync(0xffffffffu, (s0 == 0 ? mine : s < A.n ? depth(A.cu[s], A.cu[s + 1]) : 0) > lo);
         const int c = __popc(has);
         if (k < c) seq = s0 + __fns(has, 0, k + 1);
         k -= c;
       }
     }
-    if (lane == 0) {
+    if (seq < 32 ? lane == max(seq, 0) : lane == 0) {
       s_seq = seq;
       s_tile = lo;
+      s_cu0 = seq >= 32 ? A.cu[seq] : c0;
+      s_cu1 = seq >= 32 ? A.cu[seq + 1] : c1;
+      s_len = seq >= 32 ? A.len[seq] : ln;
       s_fail = 0;
     }
+  } else if (warp == 1 && lane == 0) {
+    for (int i = 0; i < C::STAGES; i++) {
+      mbar_init(&b_full[i], 1);
+      mbar_init(&b_empty[i], C::DEQ);
+    }
+    mbar_init(&b_q, (C::SOFT + C::DEQ) * 32);
+    for (int i = 0; i < C::BUF; i++) {
+      mbar_init(&b_k[i], C::DEQ * 32);
+      mbar_init(&b_v[i], C::DEQ * 32);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&b_s[i], 1);
+      mbar_init(&b_p[i], C::SOFT * 32);
+      mbar_init(&b_pv[i], 1);
+    }
+    mbar_init(&b_o, 1);
+    mbar_init(&b_end, 1);
+    mbar_fence_init();
   }
   __syncthreads();
   const int seq = s_seq;
@@ -194,14 +212,13 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     if (splits > 1 && z == 0 && tid == 0) *desc = make_int4(0, 0, 0, 0);
     return;
   }
-  const int q0 = A.cu[seq] + s_tile * bt;
-  int ntok = min(bt, A.cu[seq + 1] - q0), len = max(A.len[seq], 0);
-  if (A.cu[seq] < 0 || A.cu[seq + 1] > A.rows || len > A.tab.max_blocks * A.pool.block) {
+  const int n_new = s_cu1 - s_cu0, q0 = s_cu0 + s_tile * bt;
+  int ntok = min(bt, s_cu1 - q0), len = max(s_len, 0);
+  if (s_cu0 < 0 || s_cu1 > A.rows || len > A.tab.max_blocks * A.pool.block) {
     if (tid == 0) atomicOr(A.pool.err, KV_ERR_POS);
-    if (A.cu[seq] < 0 || A.cu[seq + 1] > A.rows) ntok = 0;
+    if (s_cu0 < 0 || s_cu1 > A.rows) ntok = 0;
     len = 0;
   }
-  const int n_new = A.cu[seq + 1] - A.cu[seq];
   const int pos0 = len - n_new + s_tile * bt;  // cached position of the CTA's first token (may be negative)
   const int gsz = A.heads / A.pool.kvh, HB = (gsz + gs - 1) / gs, kvh = unit / HB;
   const int h0 = kvh * gsz + (unit % HB) * gs, nh = min(gs, gsz - (unit % HB) * gs);
@@ -240,34 +257,59 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  if (tid == 0) {
-    for (int i = 0; i < C::STAGES; i++) {
-      mbar_init(&b_full[i], 1);
-      mbar_init(&b_empty[i], C::DEQ);
-    }
-    mbar_init(&b_q, C::SOFT * 32);
-    for (int i = 0; i < C::BUF; i++) {
-      mbar_init(&b_k[i], C::DEQ * 32);
-      mbar_init(&b_v[i], C::DEQ * 32);
-      mbar_init(&b_kfree[i], 1);
-      mbar_init(&b_vfree[i], 1);
-    }
-    for (int w = 0; w < C::NQ; w++) {
-      for (int i = 0; i < 2; i++) {
-        mbar_init(&b_s[w][i], 1);
-        mbar_init(&b_p[w][i], 128);
-      }
-      mbar_init(&b_pv[w], 1);
-    }
-    mbar_init(&b_o, 1);
-    mbar_init(&b_end, 1);
-    mbar_fence_init();
-  }
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;");
   const uint32_t tmem = s_tmem;
   const int bpt = A.pool.block / KV_TILE;
+
+  if (warp < C::SOFT + C::DEQ) {
+    // Q: HD / 8 lanes a row, brought to a power of two near 1 (see
+    // ck_kv_attn.cuh; the scale's sign goes to q: the largest product is the
+    // largest score) and rounded to 16 bits
+    constexpr int L = HD / 8, RW = 32 / L, ROWS = 128 * C::NQ, NWQ = C::SOFT + C::DEQ;
+    constexpr int STEPS = (ROWS / RW + NWQ - 1) / NWQ, B = 4;   // B loads in flight
+    const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
+    const int x = lane % L, y = lane / L;
+#pragma unroll 1
+    for (int i0 = 0; i0 < STEPS; i0 += B) {
+      KvRaw8<KV_F16> raw[B];
+#pragma unroll
+      for (int k = 0; k < B; k++) {
+        const int row = ((i0 + k) * NWQ + warp) * RW + y, tok = row / gs, head = row - tok * gs;
+        raw[k].zero();
+        if (row < ROWS && tok < ntok && head < nh)
+          raw[k].load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
+      }
+#pragma unroll
+      for (int k = 0; k < B; k++) {
+        const int row = ((i0 + k) * NWQ + warp) * RW + y;
+        const uint32_t u[4] = {raw[k].u[0].x, raw[k].u[0].y, raw[k].u[0].z, raw[k].u[0].w};
+        float2 f[4];
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          f[e] = kv_pair16(u[e], A.q.type);
+          top = kvp_max3(top, fabsf(f[e].x), fabsf(f[e].y));
+        }
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        int e = (int)(__float_as_uint(top) >> 23) - 127;
+        e = e > 127 ? 8 : max(e, -100);
+        const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
+        if (row < ROWS) {
+          // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
+          if (x == 0)
+            s_scale[row] = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23), 1e-37f);
+          *(uint4*)(sm + C::SQ + (row >> 7) * C::QB + kvp_kmajor<128>(row & 127, 8 * x)) =
+              make_uint4(kv_pack2(f[0].x * up, f[0].y * up), kv_pack2(f[1].x * up, f[1].y * up),
+                         kv_pack2(f[2].x * up, f[2].y * up), kv_pack2(f[3].x * up, f[3].y * up));
+        }
+      }
+    }
+    proxy_fence_smem();
+    mbar_arrive(&b_q);
+  }
 
   if (warp == C::SOFT + C::DEQ + 1) {
     // ---- copies: lane i fetches record i of the tile ----
@@ -323,50 +365,44 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     const uint64_t dq = umma_desc(smem_u32(sm + C::SQ), 128, 256), dk = umma_desc(smem_u32(sm + C::SK), 128, 256);
     const uint64_t dv = umma_desc(smem_u32(sm + C::SV), HD * 16, 128);
 #pragma unroll 1
-    for (int it = 0; ok && it <= n; it++) {
-      if (it < n) {
-        const int kb = it & (C::BUF - 1);
+    for (int it = 0; ok && n > 0 && it <= n; it++) {
+      const int kb = it & (C::BUF - 1), vb = (it - 1) & (C::BUF - 1);
+      if (C::BUF == 2 || it < n) {             // K of this tile (two buffers: and V of the one before)
         ok = kvp_wait<true>(&b_k[kb], (it / C::BUF) & 1, &s_fail, A.pool.err);
         if (!ok) break;
+      }
+      if (it < n) {
         asm volatile("tcgen05.fence::after_thread_sync;");
+        if (leader) {
 #pragma unroll
-        for (int w = 0; w < C::NQ; w++)
-          if (it >= from[w] && it < to[w]) {
-            const int buf = (it - from[w]) & 1;
-            const uint32_t d = tm + (2 * w + buf) * C::PT;
-            const uint64_t bd = dk + kb * (C::KB / 16);
-            if (leader) {
+          for (int w = 0; w < C::NQ; w++)
+            if (it >= from[w] && it < to[w]) {
 #pragma unroll
               for (int k = 0; k < HD / 16; k++)
-                umma_f16(d, dq + (w * C::QB + k * 4096) / 16, bd + k * C::PT * 32 / 16, idS, k > 0 ? 1u : 0u);
-              umma_commit(&b_s[w][buf]);
+                umma_f16(tm + (2 * w + (it & 1)) * C::PT, dq + (w * C::QB + k * 4096) / 16,
+                         dk + kb * (C::KB / 16) + k * C::PT * 32 / 16, idS, k > 0 ? 1u : 0u);
             }
-            __syncwarp();
-          }
-        if (leader) umma_commit(&b_kfree[kb]);
+          umma_commit(&b_s[it & 1]);
+        }
         __syncwarp();
       }
       if (it > 0) {
-        const int vb = (it - 1) & (C::BUF - 1);
-        ok = kvp_wait<true>(&b_v[vb], ((it - 1) / C::BUF) & 1, &s_fail, A.pool.err);
+        const int i = it - 1;
+        if (C::BUF == 1) ok = kvp_wait<true>(&b_v[0], i & 1, &s_fail, A.pool.err);
+        ok = ok && kvp_wait<true>(&b_p[i & 1], (i >> 1) & 1, &s_fail, A.pool.err);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        if (leader) {
 #pragma unroll
-        for (int w = 0; w < C::NQ; w++)
-          if (ok && it - 1 >= from[w] && it - 1 < to[w]) {
-            const int i = it - 1 - from[w], buf = i & 1;
-            ok = kvp_wait<true>(&b_p[w][buf], (i >> 1) & 1, &s_fail, A.pool.err);
-            if (!ok) break;
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            const uint32_t ad = tm + (2 * w + buf) * C::PT;
-            const uint64_t bd = dv + vb * (C::KB / 16);
-            if (leader) {
+          for (int w = 0; w < C::NQ; w++)
+            if (i >= from[w] && i < to[w]) {
 #pragma unroll
               for (int k = 0; k < C::PT / 16; k++)
-                umma_f16_ts(tm + C::TO + w * HD, ad + 8 * k, bd + k * 2 * HD * 16 / 16, idO, i == 0 && k == 0 ? 0u : 1u);
-              umma_commit(&b_pv[w]);
+                umma_f16_ts(tm + C::TO + w * HD, tm + (2 * w + (i & 1)) * C::PT + 8 * k,
+                            dv + vb * (C::KB / 16) + k * 2 * HD * 16 / 16, idO, i == from[w] && k == 0 ? 0u : 1u);
             }
-            __syncwarp();
-          }
-        if (leader) umma_commit(&b_vfree[vb]);
+          umma_commit(&b_pv[i & 1]);
+        }
         __syncwarp();
       }
     }
@@ -413,7 +449,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           if (kvp_bad<VB>(*(const unsigned short*)(rec + R::VS + kscl))) d[k] = 0x7fffu;
           d[k] |= d[k] << 16;
         }
-        if (k0 == 0 && it >= C::BUF) ok = kvp_wait<true>(&b_kfree[kb], (it / C::BUF - 1) & 1, &s_fail, A.pool.err);
+        if (k0 == 0 && it >= C::BUF)           // the scores of the tile that was there before are done
+          ok = kvp_wait<true>(&b_s[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < KB; k++) {
@@ -427,7 +464,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         }
       }
       proxy_fence_smem();
-      mbar_arrive(&b_k[kb]);
+      // two buffers: K and the V of the tile before are announced together
+      if (C::BUF == 1 || it == 0) mbar_arrive(&b_k[kb]);
       return true;
     };
     auto make_v = [&](int it) {
@@ -449,7 +487,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
             d[k][nib] = e | (e << 16);
           }
         }
-        if (k0 == 0 && it >= C::BUF) ok = kvp_wait<true>(&b_vfree[vb], (it / C::BUF - 1) & 1, &s_fail, A.pool.err);
+        if (k0 == 0 && it >= C::BUF)           // and so is its output
+          ok = kvp_wait<true>(&b_pv[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < VB4; k++) {
@@ -470,7 +509,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         }
       }
       proxy_fence_smem();
-      mbar_arrive(&b_v[vb]);
+      mbar_arrive(C::BUF == 1 ? &b_v[0] : &b_k[(it + 1) & 1]);
       __syncwarp();
       if (lane == 0) mbar_arrive(&b_empty[s]);
       return true;
@@ -483,67 +522,24 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     const int wq = warp >> 2, rl = 32 * (warp & 3) + lane;    // query tile and row of this thread
     const int rr = 128 * wq + rl, rtok = rr / gs, rhead = rr % gs;
     const bool rlive = rtok < ntok && rhead < nh;
-    float sc = 0.f;
-    {
-      // Q: the warp's 32 rows, HD / 8 lanes a row, brought to a power of two
-      // near 1 (see ck_kv_attn.cuh; the scale's sign goes to q: the largest
-      // product is the largest score) and rounded to 16 bits
-      constexpr int L = HD / 8, RW = 32 / L;
-      const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
-      const int x = lane % L, y = lane / L;
-      constexpr int B = 8;                      // loads in flight
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += B * RW) {
-        KvRaw8<KV_F16> raw[B];
-#pragma unroll
-        for (int n = 0; n < B; n++) {
-          const int row = 128 * wq + 32 * (warp & 3) + i0 + n * RW + y, tok = row / gs, head = row % gs;
-          raw[n].zero();
-          if (tok < ntok && head < nh)
-            raw[n].load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
-        }
-#pragma unroll
-        for (int n = 0; n < B; n++) {
-          const int i = i0 + n * RW;
-          const uint32_t u[4] = {raw[n].u[0].x, raw[n].u[0].y, raw[n].u[0].z, raw[n].u[0].w};
-          float2 f[4];
-          float top = 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            f[e] = kv_pair16(u[e], A.q.type);
-            top = fmaxf(top, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
-          }
-#pragma unroll
-          for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          int e = (int)(__float_as_uint(top) >> 23) - 127;
-          e = e > 127 ? 8 : max(e, -100);
-          const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
-          // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
-          const float back = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23), 1e-37f);
-#pragma unroll
-          for (int k = 0; k < RW; k++) {       // the row's own thread keeps its factor
-            const float b = __shfl_sync(0xffffffffu, back, k * L);
-            if (lane == i + k) sc = b;
-          }
-          *(uint4*)(sm + C::SQ + wq * C::QB + kvp_kmajor<128>(32 * (warp & 3) + i + y, 8 * x)) =
-              make_uint4(kv_pack2(f[0].x * up, f[0].y * up), kv_pack2(f[1].x * up, f[1].y * up),
-                         kv_pack2(f[2].x * up, f[2].y * up), kv_pack2(f[3].x * up, f[3].y * up));
-        }
-      }
-      proxy_fence_smem();
-      mbar_arrive(&b_q);
-    }
+    kvp_wait<true>(&b_q, 0, &s_fail, A.pool.err);
+    const float sc = s_scale[rr];
     const int rpos = pos0 + rtok;                                 // position of the row's token
     const int rlo = A.window > 0 ? max(0, rpos + 1 - A.window) : 0;
     float m = -INFINITY, l = 0.f;
     const uint32_t tO = tmem + C::TO + wq * HD + lanes;
     bool ok = true;
-    for (int j = beg[wq]; ok && j < end[wq]; j++) {
-      const int it = j - beg[wq], buf = it & 1;
+    for (int j = jb; ok && j < je; j++) {
+      const int it = j - jb, buf = it & 1;
       const uint32_t tS = tmem + (2 * wq + buf) * C::PT + lanes;
+      if (j < beg[wq] || j >= end[wq]) {       // a tile of the other query tile alone
+        ok = kvp_wait<true>(&b_s[buf], (it >> 1) & 1, &s_fail, A.pool.err);
+        if (ok) mbar_arrive(&b_p[buf]);
+        continue;
+      }
       // visible columns: vlo .. vhi (rows of no token see all: their results go nowhere)
       const int vlo = rlive ? rlo - j * C::PT : 0, vhi = rlive ? rpos - j * C::PT : C::PT;
-      ok = kvp_wait<true>(&b_s[wq][buf], (it >> 1) & 1, &s_fail, A.pool.err);
+      ok = kvp_wait<true>(&b_s[buf], (it >> 1) & 1, &s_fail, A.pool.err);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
       const uint32_t miss = s_miss[j & 7];
@@ -578,8 +574,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
         m = mn;
         l *= a;
-        if (it > 0) {
-          ok = kvp_wait<true>(&b_pv[wq], (it - 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
+        if (j > beg[wq]) {
+          ok = kvp_wait<true>(&b_pv[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
@@ -618,7 +614,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
-      mbar_arrive(&b_p[wq][buf]);
+      mbar_arrive(&b_p[buf]);
     }
     // O / l, or this CTA's part of it
     if (ok && beg[wq] < end[wq]) ok = kvp_wait<true>(&b_o, 0, &s_fail, A.pool.err);
