@@ -142,8 +142,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   __shared__ volatile int s_fail;
   __shared__ int s_seq, s_tile, s_cu0, s_cu1, s_len;
   __shared__ float s_scale[128 * C::NQ];       // factor of each query row's scores
-  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_v[C::BUF], b_s[2], b_p[2],
-      b_pv[2], b_o, b_end;
+  __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_v[C::BUF], b_kf[2],
+      b_s[C::NQ][2], b_p[C::NQ][2], b_pv[2], b_o, b_end;
   __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 5 ahead)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bt = 128 * C::NQ / gs;             // tokens of a CTA
@@ -197,19 +197,28 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       mbar_init(&b_v[i], C::DEQ * 32);
     }
     for (int i = 0; i < 2; i++) {
-      mbar_init(&b_s[i], 1);
-      mbar_init(&b_p[i], C::SOFT * 32);
+      for (int w = 0; w < C::NQ; w++) {
+        mbar_init(&b_s[w][i], 1);
+        mbar_init(&b_p[w][i], 128);
+      }
+      mbar_init(&b_kf[i], 1);
       mbar_init(&b_pv[i], 1);
     }
     mbar_init(&b_o, 1);
     mbar_init(&b_end, 1);
     mbar_fence_init();
+  } else if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
   const int seq = s_seq;
   int4* desc = (int4*)A.ml + b * units + unit;      // splits: what k_kv_prompt_join joins
   if (seq < 0) {
     if (splits > 1 && z == 0 && tid == 0) *desc = make_int4(0, 0, 0, 0);
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(512));
     return;
   }
   const int n_new = s_cu1 - s_cu0, q0 = s_cu0 + s_tile * bt;
@@ -253,13 +262,6 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     }
   }
 
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;");
   const uint32_t tmem = s_tmem;
   const int bpt = A.pool.block / KV_TILE;
 
@@ -268,22 +270,21 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     // ck_kv_attn.cuh; the scale's sign goes to q: the largest product is the
     // largest score) and rounded to 16 bits
     constexpr int L = HD / 8, RW = 32 / L, ROWS = 128 * C::NQ, NWQ = C::SOFT + C::DEQ;
-    constexpr int STEPS = (ROWS / RW + NWQ - 1) / NWQ, B = 4;   // B loads in flight
+    constexpr int B = (ROWS / RW + NWQ - 1) / NWQ;           // rows of a warp, all on their way at once
     const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
     const int x = lane % L, y = lane / L;
-#pragma unroll 1
-    for (int i0 = 0; i0 < STEPS; i0 += B) {
+    {
       KvRaw8<KV_F16> raw[B];
 #pragma unroll
       for (int k = 0; k < B; k++) {
-        const int row = ((i0 + k) * NWQ + warp) * RW + y, tok = row / gs, head = row - tok * gs;
+        const int row = (k * NWQ + warp) * RW + y, tok = row / gs, head = row - tok * gs;
         raw[k].zero();
         if (row < ROWS && tok < ntok && head < nh)
           raw[k].load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
       }
 #pragma unroll
       for (int k = 0; k < B; k++) {
-        const int row = ((i0 + k) * NWQ + warp) * RW + y;
+        const int row = (k * NWQ + warp) * RW + y;
         const uint32_t u[4] = {raw[k].u[0].x, raw[k].u[0].y, raw[k].u[0].z, raw[k].u[0].w};
         float2 f[4];
         float top = 0.f;
@@ -381,26 +382,30 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
               for (int k = 0; k < HD / 16; k++)
                 umma_f16(tm + (2 * w + (it & 1)) * C::PT, dq + (w * C::QB + k * 4096) / 16,
                          dk + kb * (C::KB / 16) + k * C::PT * 32 / 16, idS, k > 0 ? 1u : 0u);
+              umma_commit(&b_s[w][it & 1]);
             }
-          umma_commit(&b_s[it & 1]);
+          umma_commit(&b_kf[it & 1]);
         }
         __syncwarp();
       }
       if (it > 0) {
         const int i = it - 1;
         if (C::BUF == 1) ok = kvp_wait<true>(&b_v[0], i & 1, &s_fail, A.pool.err);
-        ok = ok && kvp_wait<true>(&b_p[i & 1], (i >> 1) & 1, &s_fail, A.pool.err);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;");
-        if (leader) {
 #pragma unroll
-          for (int w = 0; w < C::NQ; w++)
-            if (i >= from[w] && i < to[w]) {
+        for (int w = 0; w < C::NQ; w++)
+          if (ok && i >= from[w] && i < to[w]) {
+            ok = kvp_wait<true>(&b_p[w][i & 1], ((i >> 1) - ((from[w] + 1 - (i & 1)) >> 1)) & 1, &s_fail, A.pool.err);
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            if (ok && leader) {
 #pragma unroll
               for (int k = 0; k < C::PT / 16; k++)
                 umma_f16_ts(tm + C::TO + w * HD, tm + (2 * w + (i & 1)) * C::PT + 8 * k,
                             dv + vb * (C::KB / 16) + k * 2 * HD * 16 / 16, idO, i == from[w] && k == 0 ? 0u : 1u);
             }
+            __syncwarp();
+          }
+        if (!ok) break;
+        if (leader) {
           umma_commit(&b_pv[i & 1]);
         }
         __syncwarp();
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           d[k] |= d[k] << 16;
         }
         if (k0 == 0 && it >= C::BUF)           // the scores of the tile that was there before are done
-          ok = kvp_wait<true>(&b_s[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
+          ok = kvp_wait<true>(&b_kf[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < KB; k++) {
@@ -529,17 +534,14 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     float m = -INFINITY, l = 0.f;
     const uint32_t tO = tmem + C::TO + wq * HD + lanes;
     bool ok = true;
-    for (int j = jb; ok && j < je; j++) {
+    for (int j = beg[wq]; ok && j < end[wq]; j++) {
       const int it = j - jb, buf = it & 1;
+      // uses of this buffer by this query tile before: its tiles of the same parity
+      const int use = (it >> 1) - ((beg[wq] - jb + 1 - buf) >> 1);
       const uint32_t tS = tmem + (2 * wq + buf) * C::PT + lanes;
-      if (j < beg[wq] || j >= end[wq]) {       // a tile of the other query tile alone
-        ok = kvp_wait<true>(&b_s[buf], (it >> 1) & 1, &s_fail, A.pool.err);
-        if (ok) mbar_arrive(&b_p[buf]);
-        continue;
-      }
       // visible columns: vlo .. vhi (rows of no token see all: their results go nowhere)
       const int vlo = rlive ? rlo - j * C::PT : 0, vhi = rlive ? rpos - j * C::PT : C::PT;
-      ok = kvp_wait<true>(&b_s[buf], (it >> 1) & 1, &s_fail, A.pool.err);
+      ok = kvp_wait<true>(&b_s[wq][buf], use & 1, &s_fail, A.pool.err);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
       const uint32_t miss = s_miss[j & 7];
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
-      mbar_arrive(&b_p[buf]);
+      mbar_arrive(&b_p[wq][buf]);
     }
     // O / l, or this CTA's part of it
     if (ok && beg[wq] < end[wq]) ok = kvp_wait<true>(&b_o, 0, &s_fail, A.pool.err);
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   // no CTA leaves, or frees its tensor memory, with a product in flight
   __syncthreads();
   if (warp == C::SOFT + C::DEQ && elect_one()) umma_commit(&b_end);
-  if (warp == 0) {
+  if (warp == 2) {
     unsigned spins = 0;
     while (!mbar_try_wait(&b_end, 0) && ++spins < (1u << 20)) {}
     __syncwarp();
