@@ -15,9 +15,9 @@
 //   4 or 8    turn codes into fp16 operand tiles of 64 positions (the same
 //             arithmetic for both: V is fed to the second product as it lies,
 //             its dims contiguous), K a tile ahead of V
-//   1 thread  issues the products: a tile's scores before the output of the
-//             tile before, so that they are there when the softmax comes to
-//             them (two score buffers a query tile)
+//   2 warps   issue the products, one the scores, a tile ahead of the softmax
+//             (two score buffers a query tile), one the outputs: a wait costs
+//             either some 200 cycles, in which the other's products run
 //   4 or 8    softmax: a thread owns a query row; it reads its 64 scores from
 //             tensor memory once and writes P over them as the second
 //             product's operand.  The exponentials are taken against a
@@ -45,7 +45,8 @@ struct KvPr {
   static constexpr int PT = 64;                           // positions of a K / V tile
   static constexpr int BUF = HD == 256 ? 1 : 2;           // K and V tiles
   static constexpr int SOFT = 4 * NQ, DEQ = 12 - SOFT;    // warps
-  static constexpr int THREADS = (SOFT + DEQ + 2) * 32;
+  static constexpr int THREADS = (SOFT + DEQ + 3) * 32;
+  static constexpr int W_COPY = SOFT + DEQ, W_S = W_COPY + 1, W_O = W_COPY + 2;   // the single warps
   static constexpr int RECS = PT / KV_TILE;
   static constexpr int STAGE_BYTES = RECS * R::BYTES;
   static constexpr int STAGES = HD == 256 ? 2 : 4;
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       mbar_init(&b_pv[i], 1);
     }
     mbar_init(&b_o, 1);
-    mbar_init(&b_end, 1);
+    mbar_init(&b_end, 2);
     mbar_fence_init();
   } else if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512));
@@ -266,45 +267,50 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   const int bpt = A.pool.block / KV_TILE;
 
   if (warp < C::SOFT + C::DEQ) {
-    // Q: HD / 8 lanes a row, brought to a power of two near 1 (see
-    // ck_kv_attn.cuh; the scale's sign goes to q: the largest product is the
-    // largest score) and rounded to 16 bits
+    // Q in fp16, HD / 8 lanes a row: bf16 rows are brought to a power of two
+    // (as in ck_kv_attn.cuh).  The scale's sign goes to q: the largest product
+    // is the largest score
     constexpr int L = HD / 8, RW = 32 / L, ROWS = 128 * C::NQ, NWQ = C::SOFT + C::DEQ;
     constexpr int B = (ROWS / RW + NWQ - 1) / NWQ;           // rows of a warp, all on their way at once
     const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
     const int x = lane % L, y = lane / L;
     {
       KvRaw8<KV_F16> raw[B];
+      const uint32_t by_gs = (65536 + gs - 1) / gs;            // row / gs for rows up to 255, heads up to 128
 #pragma unroll
       for (int k = 0; k < B; k++) {
-        const int row = (k * NWQ + warp) * RW + y, tok = row / gs, head = row - tok * gs;
+        const int row = (k * NWQ + warp) * RW + y, tok = (row * by_gs) >> 16, head = row - tok * gs;
         raw[k].zero();
         if (row < ROWS && tok < ntok && head < nh)
           raw[k].load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
       }
+      const float fac = fabsf(A.scale) * 1.4426950408889634f;
+      const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
       for (int k = 0; k < B; k++) {
         const int row = (k * NWQ + warp) * RW + y;
-        const uint32_t u[4] = {raw[k].u[0].x, raw[k].u[0].y, raw[k].u[0].z, raw[k].u[0].w};
-        float2 f[4];
-        float top = 0.f;
+        uint32_t u[4] = {raw[k].u[0].x, raw[k].u[0].y, raw[k].u[0].z, raw[k].u[0].w};
+        float back = fac;
+        if (A.q.type != KV_F16) {              // bf16: fp16 as it is
+          uint32_t m = 0;                      // the largest magnitude's bits
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          f[e] = kv_pair16(u[e], A.q.type);
-          top = kvp_max3(top, fabsf(f[e].x), fabsf(f[e].y));
+          for (int e = 0; e < 4; e++) m = __vmaxu2(m, u[e] & 0x7fff7fffu);
+          m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+          for (int o = 1; o < L; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+          int e = (int)(m >> 7) - 127;
+          e = e > 127 ? 8 : max(e, -100);
+          const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
+          back *= __uint_as_float((uint32_t)(127 + e - 8) << 23);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            u[i] = kv_pack2(__uint_as_float(u[i] << 16) * up, __uint_as_float(u[i] & 0xffff0000u) * up);
         }
-#pragma unroll
-        for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        int e = (int)(__float_as_uint(top) >> 23) - 127;
-        e = e > 127 ? 8 : max(e, -100);
-        const float up = copysignf(__uint_as_float((uint32_t)(127 + 8 - e) << 23), A.scale);
         if (row < ROWS) {
           // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
-          if (x == 0)
-            s_scale[row] = fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e - 8) << 23), 1e-37f);
+          if (x == 0) s_scale[row] = fmaxf(back, 1e-37f);
           *(uint4*)(sm + C::SQ + (row >> 7) * C::QB + kvp_kmajor<128>(row & 127, 8 * x)) =
-              make_uint4(kv_pack2(f[0].x * up, f[0].y * up), kv_pack2(f[1].x * up, f[1].y * up),
-                         kv_pack2(f[2].x * up, f[2].y * up), kv_pack2(f[3].x * up, f[3].y * up));
+              make_uint4(u[0] ^ flip, u[1] ^ flip, u[2] ^ flip, u[3] ^ flip);
         }
       }
     }
@@ -312,7 +318,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     mbar_arrive(&b_q);
   }
 
-  if (warp == C::SOFT + C::DEQ + 1) {
+  if (warp == C::W_COPY) {
     // ---- copies: lane i fetches record i of the tile ----
     for (int j = jb; j < je; j++) {
       const int it = j - jb, s = it % C::STAGES;
@@ -344,14 +350,12 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     if (s_fail)                                // no copy may land after the CTA has gone
       for (int s = 0; s < min(C::STAGES, je - jb); s++)
         for (unsigned spins = 0; !mbar_try_wait(&b_full[s], 0) && !mbar_try_wait(&b_full[s], 1) && spins < (1u << 20); spins++) {}
-  } else if (warp == C::SOFT + C::DEQ) {
+  } else if (warp == C::W_S || warp == C::W_O) {
     // ---- products ----
     // The whole warp runs the loop and one elected lane issues: operands that
     // the compiler sees to be the same in every lane go to the tensor core
     // from uniform registers (from a lone thread's branch each product cost
     // about 70 cycles to issue, more than it takes).
-    const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
-    const uint32_t idO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);   // V's dims are contiguous
     const int n = __shfl_sync(0xffffffffu, je - jb, 0);
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     int from[C::NQ], to[C::NQ];                // tiles of each query tile, counted from jb
@@ -361,18 +365,19 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       to[w] = __shfl_sync(0xffffffffu, end[w] - jb, 0);
     }
     const bool leader = elect_one();
-    bool ok = n <= 0 || kvp_wait<true>(&b_q, 0, &s_fail, A.pool.err);
+    bool ok = true;
     // descriptors: a step of 16 further along is so many 16-byte units on
-    const uint64_t dq = umma_desc(smem_u32(sm + C::SQ), 128, 256), dk = umma_desc(smem_u32(sm + C::SK), 128, 256);
-    const uint64_t dv = umma_desc(smem_u32(sm + C::SV), HD * 16, 128);
+    if (warp == C::W_S) {
+      const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
+      const uint64_t dq = umma_desc(smem_u32(sm + C::SQ), 128, 256), dk = umma_desc(smem_u32(sm + C::SK), 128, 256);
+      ok = n <= 0 || kvp_wait<true>(&b_q, 0, &s_fail, A.pool.err);
 #pragma unroll 1
-    for (int it = 0; ok && n > 0 && it <= n; it++) {
-      const int kb = it & (C::BUF - 1), vb = (it - 1) & (C::BUF - 1);
-      if (C::BUF == 2 || it < n) {             // K of this tile (two buffers: and V of the one before)
+      for (int it = 0; ok && it < n; it++) {
+        const int kb = it & (C::BUF - 1);
         ok = kvp_wait<true>(&b_k[kb], (it / C::BUF) & 1, &s_fail, A.pool.err);
+        // the score buffer: its P of two tiles ago has been multiplied
+        if (it >= 2) ok = ok && kvp_wait<true>(&b_pv[it & 1], ((it >> 1) - 1) & 1, &s_fail, A.pool.err);
         if (!ok) break;
-      }
-      if (it < n) {
         asm volatile("tcgen05.fence::after_thread_sync;");
         if (leader) {
 #pragma unroll
@@ -388,31 +393,35 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         }
         __syncwarp();
       }
-      if (it > 0) {
-        const int i = it - 1;
-        if (C::BUF == 1) ok = kvp_wait<true>(&b_v[0], i & 1, &s_fail, A.pool.err);
+    } else {
+      const uint32_t idO = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | (8u << 24);   // V's dims are contiguous
+      const uint64_t dv = umma_desc(smem_u32(sm + C::SV), HD * 16, 128);
+#pragma unroll 1
+      for (int it = 0; ok && it < n; it++) {
+        const int vb = it & (C::BUF - 1);
+        // two buffers: this V is announced with the next K
+        if (C::BUF == 1) ok = kvp_wait<true>(&b_v[0], it & 1, &s_fail, A.pool.err);
+        else ok = kvp_wait<true>(&b_k[(it + 1) & 1], ((it + 1) >> 1) & 1, &s_fail, A.pool.err);
 #pragma unroll
         for (int w = 0; w < C::NQ; w++)
-          if (ok && i >= from[w] && i < to[w]) {
-            ok = kvp_wait<true>(&b_p[w][i & 1], ((i >> 1) - ((from[w] + 1 - (i & 1)) >> 1)) & 1, &s_fail, A.pool.err);
+          if (ok && it >= from[w] && it < to[w]) {
+            ok = kvp_wait<true>(&b_p[w][it & 1], ((it >> 1) - ((from[w] + 1 - (it & 1)) >> 1)) & 1, &s_fail, A.pool.err);
             asm volatile("tcgen05.fence::after_thread_sync;");
             if (ok && leader) {
 #pragma unroll
               for (int k = 0; k < C::PT / 16; k++)
-                umma_f16_ts(tm + C::TO + w * HD, tm + (2 * w + (i & 1)) * C::PT + 8 * k,
-                            dv + vb * (C::KB / 16) + k * 2 * HD * 16 / 16, idO, i == from[w] && k == 0 ? 0u : 1u);
+                umma_f16_ts(tm + C::TO + w * HD, tm + (2 * w + (it & 1)) * C::PT + 8 * k,
+                            dv + vb * (C::KB / 16) + k * 2 * HD * 16 / 16, idO, it == from[w] && k == 0 ? 0u : 1u);
             }
             __syncwarp();
           }
         if (!ok) break;
-        if (leader) {
-          umma_commit(&b_pv[i & 1]);
-        }
+        if (leader) umma_commit(&b_pv[it & 1]);
         __syncwarp();
       }
+      if (leader) umma_commit(&b_o);
+      __syncwarp();
     }
-    if (leader) umma_commit(&b_o);
-    __syncwarp();
   } else if (warp >= C::SOFT && warp < C::SOFT + C::DEQ) {
     // ---- K and V from codes ----
     // A record's codes are cut into pieces of 8 positions x 64 dims (V in 4
@@ -658,7 +667,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   }
   // no CTA leaves, or frees its tensor memory, with a product in flight
   __syncthreads();
-  if (warp == C::SOFT + C::DEQ && elect_one()) umma_commit(&b_end);
+  if ((warp == C::W_S || warp == C::W_O) && elect_one()) umma_commit(&b_end);
   if (warp == 2) {
     unsigned spins = 0;
     while (!mbar_try_wait(&b_end, 0) && ++spins < (1u << 20)) {}
