@@ -112,10 +112,9 @@ __device__ __forceinline__ bool kvp_bad(uint32_t d) {
   return (d & 0x7fffu) > (VB == 8 ? 0x6007u : 0x6fffu);      // 515.5 (x 127) and 8188 (x 8)
 }
 
-// Waits for a phase of bar; gives up (false) after a bounded number of polls
-// or when another role of the CTA has given up.  WARP: called by a whole warp,
-// whose lanes get the same answer.
-template <bool WARP>
+// A whole warp waits for a phase of bar (all lanes get the same answer); gives
+// up (false) after a bounded number of polls or when another role of the CTA
+// has given up.
 __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatile int* fail, int* err) {
   unsigned spins = 0;
   bool ok = true;
@@ -131,7 +130,7 @@ __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatil
       break;
     }
   }
-  return WARP ? __all_sync(0xffffffffu, ok) : ok;
+  return __all_sync(0xffffffffu, ok);
 }
 
 template <int HD, int VB>
@@ -267,52 +266,75 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   const int bpt = A.pool.block / KV_TILE;
 
   if (warp < C::SOFT + C::DEQ) {
-    // Q in fp16, HD / 8 lanes a row: bf16 rows are brought to a power of two
-    // (as in ck_kv_attn.cuh).  The scale's sign goes to q: the largest product
-    // is the largest score
-    constexpr int L = HD / 8, RW = 32 / L, ROWS = 128 * C::NQ, NWQ = C::SOFT + C::DEQ;
-    constexpr int B = (ROWS / RW + NWQ - 1) / NWQ;           // rows of a warp, all on their way at once
+    // Q in fp16, HD / 32 lanes a row, four 16-byte pieces a lane: bf16 rows are
+    // brought to a power of two (as in ck_kv_attn.cuh).  The scale's sign goes
+    // to q: the largest product is the largest score.  Rows go to shared memory
+    // as they are, all of a warp's on their way at once, and are worked on
+    // there.  (One piece a lane is bound by its chain of dependent steps, and
+    // unrolled over its rows by fetching code that runs once: 12000 and 9800
+    // cycles a CTA.)
+    constexpr int L = HD / 32, RW = 32 / L, ROWS = 128 * C::NQ, NWQ = C::SOFT + C::DEQ;
     const bool vec = (uintptr_t)A.q.p % 16 == 0 && A.q.st % 8 == 0 && A.q.sh % 8 == 0;
     const int x = lane % L, y = lane / L;
-    {
-      KvRaw8<KV_F16> raw[B];
-      const uint32_t by_gs = (65536 + gs - 1) / gs;            // row / gs for rows up to 255, heads up to 128
+    const uint32_t by_gs = (65536 + gs - 1) / gs;              // row / gs for rows up to 255, heads up to 128
+    auto place = [&](int row, int p) { return (uint4*)(sm + C::SQ + (row >> 7) * C::QB + kvp_kmajor<128>(row & 127, 8 * (x + L * p))); };
+#pragma unroll 1
+    for (int row = warp * RW + y; row < ROWS; row += NWQ * RW) {
+      const int tok = (row * by_gs) >> 16, head = row - tok * gs;
+      const unsigned short* src = (const unsigned short*)A.q.p + (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x;
+      const bool live = tok < ntok && head < nh;
 #pragma unroll
-      for (int k = 0; k < B; k++) {
-        const int row = (k * NWQ + warp) * RW + y, tok = (row * by_gs) >> 16, head = row - tok * gs;
-        raw[k].zero();
-        if (row < ROWS && tok < ntok && head < nh)
-          raw[k].load(A.q.p, (size_t)(q0 + tok) * A.q.st + (size_t)(h0 + head) * A.q.sh + 8 * x, vec);
+      for (int p = 0; p < 4; p++) {
+        if (!live) {
+          *place(row, p) = make_uint4(0u, 0u, 0u, 0u);
+        } else if (vec) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(place(row, p))), "l"(src + 8 * L * p) : "memory");
+        } else {
+          unsigned short* dst = (unsigned short*)place(row, p);
+#pragma unroll 1
+          for (int e = 0; e < 8; e++) dst[e] = src[8 * L * p + e];
+        }
       }
-      const float fac = fabsf(A.scale) * 1.4426950408889634f;
-      const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");           // each lane goes on with what it copied itself
+    const float fac = fabsf(A.scale) * 1.4426950408889634f;
+    const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 1
+    for (int row = warp * RW + y; row - y < ROWS; row += NWQ * RW) {
+      float back = fac;
+      if (A.q.type != KV_F16 || flip) {
+        uint32_t u[4][4];
 #pragma unroll
-      for (int k = 0; k < B; k++) {
-        const int row = (k * NWQ + warp) * RW + y;
-        uint32_t u[4] = {raw[k].u[0].x, raw[k].u[0].y, raw[k].u[0].z, raw[k].u[0].w};
-        float back = fac;
-        if (A.q.type != KV_F16) {              // bf16: fp16 as it is
-          uint32_t m = 0;                      // the largest magnitude's bits
+        for (int p = 0; p < 4; p++) {
+          const uint4 v = *place(min(row, ROWS - 1), p);
+          u[p][0] = v.x; u[p][1] = v.y; u[p][2] = v.z; u[p][3] = v.w;
+        }
+        if (A.q.type != KV_F16) {
+          uint32_t m[4];                       // the largest magnitude's bits
 #pragma unroll
-          for (int e = 0; e < 4; e++) m = __vmaxu2(m, u[e] & 0x7fff7fffu);
-          m = max(m & 0xffffu, m >> 16);
+          for (int p = 0; p < 4; p++)
+            m[p] = __vmaxu2(__vmaxu2(u[p][0] & 0x7fff7fffu, u[p][1] & 0x7fff7fffu), __vmaxu2(u[p][2] & 0x7fff7fffu, u[p][3] & 0x7fff7fffu));
+          m[0] = __vmaxu2(__vmaxu2(m[0], m[1]), __vmaxu2(m[2], m[3]));
+          m[0] = max(m[0] & 0xffffu, m[0] >> 16);
 #pragma unroll
-          for (int o = 1; o < L; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          int e = (int)(m >> 7) - 127;
+          for (int o = 1; o < L; o <<= 1) m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+          int e = (int)(m[0] >> 7) - 127;
           e = e > 127 ? 8 : max(e, -100);
           const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
           back *= __uint_as_float((uint32_t)(127 + e - 8) << 23);
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            u[i] = kv_pack2(__uint_as_float(u[i] << 16) * up, __uint_as_float(u[i] & 0xffff0000u) * up);
+          for (int p = 0; p < 4; p++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              u[p][i] = kv_pack2(__uint_as_float(u[p][i] << 16) * up, __uint_as_float(u[p][i] & 0xffff0000u) * up);
         }
-        if (row < ROWS) {
-          // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
-          if (x == 0) s_scale[row] = fmaxf(back, 1e-37f);
-          *(uint4*)(sm + C::SQ + (row >> 7) * C::QB + kvp_kmajor<128>(row & 127, 8 * x)) =
-              make_uint4(u[0] ^ flip, u[1] ^ flip, u[2] ^ flip, u[3] ^ flip);
-        }
+        if (row < ROWS)
+#pragma unroll
+          for (int p = 0; p < 4; p++)
+            *place(row, p) = make_uint4(u[p][0] ^ flip, u[p][1] ^ flip, u[p][2] ^ flip, u[p][3] ^ flip);
       }
+      // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
+      if (x == 0 && row < ROWS) s_scale[row] = fmaxf(back, 1e-37f);
     }
     proxy_fence_smem();
     mbar_arrive(&b_q);
@@ -322,7 +344,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     // ---- copies: lane i fetches record i of the tile ----
     for (int j = jb; j < je; j++) {
       const int it = j - jb, s = it % C::STAGES;
-      if (it >= C::STAGES && !kvp_wait<true>(&b_empty[s], (it / C::STAGES - 1) & 1, &s_fail, A.pool.err)) break;
+      if (it >= C::STAGES && !kvp_wait(&b_empty[s], (it / C::STAGES - 1) & 1, &s_fail, A.pool.err)) break;
       const int tile = j * C::RECS + lane;     // record of the sequence
       bool ok = lane < C::RECS && tile * KV_TILE < len;
       int id = 0;
@@ -370,13 +392,13 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     if (warp == C::W_S) {
       const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
       const uint64_t dq = umma_desc(smem_u32(sm + C::SQ), 128, 256), dk = umma_desc(smem_u32(sm + C::SK), 128, 256);
-      ok = n <= 0 || kvp_wait<true>(&b_q, 0, &s_fail, A.pool.err);
+      ok = n <= 0 || kvp_wait(&b_q, 0, &s_fail, A.pool.err);
 #pragma unroll 1
       for (int it = 0; ok && it < n; it++) {
         const int kb = it & (C::BUF - 1);
-        ok = kvp_wait<true>(&b_k[kb], (it / C::BUF) & 1, &s_fail, A.pool.err);
+        ok = kvp_wait(&b_k[kb], (it / C::BUF) & 1, &s_fail, A.pool.err);
         // the score buffer: its P of two tiles ago has been multiplied
-        if (it >= 2) ok = ok && kvp_wait<true>(&b_pv[it & 1], ((it >> 1) - 1) & 1, &s_fail, A.pool.err);
+        if (it >= 2) ok = ok && kvp_wait(&b_pv[it & 1], ((it >> 1) - 1) & 1, &s_fail, A.pool.err);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;");
         if (leader) {
@@ -400,12 +422,12 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       for (int it = 0; ok && it < n; it++) {
         const int vb = it & (C::BUF - 1);
         // two buffers: this V is announced with the next K
-        if (C::BUF == 1) ok = kvp_wait<true>(&b_v[0], it & 1, &s_fail, A.pool.err);
-        else ok = kvp_wait<true>(&b_k[(it + 1) & 1], ((it + 1) >> 1) & 1, &s_fail, A.pool.err);
+        if (C::BUF == 1) ok = kvp_wait(&b_v[0], it & 1, &s_fail, A.pool.err);
+        else ok = kvp_wait(&b_k[(it + 1) & 1], ((it + 1) >> 1) & 1, &s_fail, A.pool.err);
 #pragma unroll
         for (int w = 0; w < C::NQ; w++)
           if (ok && it >= from[w] && it < to[w]) {
-            ok = kvp_wait<true>(&b_p[w][it & 1], ((it >> 1) - ((from[w] + 1 - (it & 1)) >> 1)) & 1, &s_fail, A.pool.err);
+            ok = kvp_wait(&b_p[w][it & 1], ((it >> 1) - ((from[w] + 1 - (it & 1)) >> 1)) & 1, &s_fail, A.pool.err);
             asm volatile("tcgen05.fence::after_thread_sync;");
             if (ok && leader) {
 #pragma unroll
@@ -449,7 +471,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     auto make_k = [&](int it) {
       const int s = it % C::STAGES, kb = it % C::BUF;
       const uint8_t* stg = sm + C::SST + s * C::STAGE_BYTES;
-      bool ok = kvp_wait<true>(&b_full[s], (it / C::STAGES) & 1, &s_fail, A.pool.err);
+      bool ok = kvp_wait(&b_full[s], (it / C::STAGES) & 1, &s_fail, A.pool.err);
       if (!ok) return false;
 #pragma unroll
       for (int k0 = 0; k0 < KN; k0 += KB) {
@@ -464,7 +486,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           d[k] |= d[k] << 16;
         }
         if (k0 == 0 && it >= C::BUF)           // the scores of the tile that was there before are done
-          ok = kvp_wait<true>(&b_kf[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
+          ok = kvp_wait(&b_kf[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < KB; k++) {
@@ -502,7 +524,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           }
         }
         if (k0 == 0 && it >= C::BUF)           // and so is its output
-          ok = kvp_wait<true>(&b_pv[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
+          ok = kvp_wait(&b_pv[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < VB4; k++) {
@@ -529,14 +551,21 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       return true;
     };
     bool ok = jb >= je || make_k(0);
-    for (int it = 0; ok && it < je - jb; it++) ok = (it + 1 >= je - jb || make_k(it + 1)) && make_v(it);
+    for (int it = 0; ok && it < je - jb; it++) {
+      if (it + 1 < je - jb) ok = make_k(it + 1);
+      // (nothing to announce with the last V: as a next K would, wait for the
+      // scores two tiles before it, so that no warp announces twice into one
+      // phase while another has not announced once)
+      else if (C::BUF == 2 && it > 0) ok = kvp_wait(&b_kf[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_fail, A.pool.err);
+      ok = ok && make_v(it);
+    }
   } else if (warp < C::SOFT) {
     // ---- softmax ----
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const int wq = warp >> 2, rl = 32 * (warp & 3) + lane;    // query tile and row of this thread
     const int rr = 128 * wq + rl, rtok = rr / gs, rhead = rr % gs;
     const bool rlive = rtok < ntok && rhead < nh;
-    kvp_wait<true>(&b_q, 0, &s_fail, A.pool.err);
+    kvp_wait(&b_q, 0, &s_fail, A.pool.err);
     const float sc = s_scale[rr];
     const int rpos = pos0 + rtok;                                 // position of the row's token
     const int rlo = A.window > 0 ? max(0, rpos + 1 - A.window) : 0;
@@ -550,7 +579,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       const uint32_t tS = tmem + (2 * wq + buf) * C::PT + lanes;
       // visible columns: vlo .. vhi (rows of no token see all: their results go nowhere)
       const int vlo = rlive ? rlo - j * C::PT : 0, vhi = rlive ? rpos - j * C::PT : C::PT;
-      ok = kvp_wait<true>(&b_s[wq][buf], use & 1, &s_fail, A.pool.err);
+      ok = kvp_wait(&b_s[wq][buf], use & 1, &s_fail, A.pool.err);
       if (!ok) break;
       asm volatile("tcgen05.fence::after_thread_sync;");
       const uint32_t miss = s_miss[j & 7];
@@ -586,7 +615,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         m = mn;
         l *= a;
         if (j > beg[wq]) {
-          ok = kvp_wait<true>(&b_pv[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
+          ok = kvp_wait(&b_pv[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll 1
@@ -628,7 +657,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       mbar_arrive(&b_p[wq][buf]);
     }
     // O / l, or this CTA's part of it
-    if (ok && beg[wq] < end[wq]) ok = kvp_wait<true>(&b_o, 0, &s_fail, A.pool.err);
+    if (ok && beg[wq] < end[wq]) ok = kvp_wait(&b_o, 0, &s_fail, A.pool.err);
     asm volatile("tcgen05.fence::after_thread_sync;");
     if (ok) {
       const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -314,6 +314,26 @@ def test_prompt_attention(layout, case, window):
     assert torch.equal(got, c.attend_prompt(q, cu, _i32(lens), table, window=window))
 
 
+@pytest.mark.parametrize("n", [1, 64, 65, 128, 129, 192])
+@pytest.mark.parametrize("layout", [(6, 3, 64), (16, 8, 128), (4, 1, 256)])
+def test_prompt_attention_of_many_short_sequences(layout, n):
+    """A few position tiles a CTA, on every SM at once and many times over: the roles of a CTA hand over from the first
+    tile to the last without a long run in between, and every pass gives the same bits."""
+    H, K, hd = layout
+    lens = [n] * 120
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=n)
+    q = torch.randn(sum(lens), H, hd, generator=g).mul_(2).half().cuda()
+    cu, ln = _i32(np.arange(121) * n), _i32(lens)
+    first = c.attend_prompt(q, cu, ln, table)
+    c.check()
+    want, mag, top = _ref_attention(q[: 2 * n], k[:2], v[:2], lens[:2], lens[:2], 1 / math.sqrt(hd), 0)
+    _close(first[: 2 * n], want, mag, top, 2.0 ** -11)
+    for _ in range(200):
+        again = c.attend_prompt(q, cu, ln, table)
+    c.check()
+    assert torch.equal(first, again)
+
+
 @pytest.mark.parametrize("v_bits", [8, 4])
 @pytest.mark.parametrize("block", [16, 128])
 @pytest.mark.parametrize("layout", LAYOUTS)
