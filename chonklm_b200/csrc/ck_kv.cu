@@ -126,8 +126,7 @@ cudaError_t kv_store_launch(const KvStore& a, cudaStream_t s, bool pdl) {
 cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
   if (a.n == 0) return cudaSuccess;
   const int vec = (kv_vec8(a.k) ? 1 : 0) | (kv_vec8(a.v) ? 2 : 0);
-  const long long rows = (long long)a.n * a.pool.kvh, per = KV_LOAD_ROWS * KV_LOAD_THREADS / (a.pool.hd / 8);
-  const dim3 grid((unsigned)((rows + per - 1) / per)), block(KV_LOAD_THREADS);
+  const dim3 grid((a.n + KV_LOAD_THREADS / 32 - 1) / (KV_LOAD_THREADS / 32)), block(KV_LOAD_THREADS);
 #define KV_CASE(HD, VB)                                                                                      \
   if (a.pool.hd == HD && a.pool.vbits == VB)                                                                 \
     return a.k.type == KV_F32   ? kv_launch(k_kv_load<HD, VB, KV_F32>, grid, block, 0, s, false, a, vec)     \
