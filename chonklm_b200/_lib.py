@@ -113,6 +113,8 @@ def lib():
             L.ck_trace_read.argtypes = [P, P, S]
             L.ck_matmul.argtypes = [I, P, S, I, I, P, I, P, I]
             L.ck_batch_create.argtypes = [P, I, I, pp(P)]
+            L.ck_batch_create_kv.argtypes = [P, I, I, I, pp(P)]
+            L.ck_batch_read_kv.argtypes = [P, I, I, P, P, I, pp(I)]
             L.ck_batch_add_seq.argtypes = [P, pp(U), I, I, pp(U), I, pp(I)]
             L.ck_batch_step.argtypes = [P, pp(I)]
             L.ck_batch_collect.argtypes = [P, I, pp(U), I, pp(I), pp(I)]
@@ -301,13 +303,19 @@ def _check_batch(rc: int, b) -> None:
 
 class Batch:
     """Batched decode over an Engine's weights (ck_batch_*): sequences are
-    added, stepped together one position per step, and collected."""
+    added, stepped together one position per step, and collected.  kv: the
+    cache, "f16", "q8" (keys and values in 8 bits) or "q8v4" (values in 4)."""
 
-    def __init__(self, engine: "Engine", max_seqs: int, kv_blocks: int = 0):
+    KV = {"f16": 0, "q8": 1, "q8v4": 2}
+
+    def __init__(self, engine: "Engine", max_seqs: int, kv_blocks: int = 0, kv: str = "f16"):
         self._L = lib()
         self.engine = engine   # keeps the weights alive
+        if kv not in self.KV:
+            raise ValueError(f"unknown cache {kv!r}: expected one of {', '.join(self.KV)}")
         b = ctypes.c_void_p()
-        _check(self._L.ck_batch_create(engine.h, int(max_seqs), int(kv_blocks), ctypes.byref(b)), engine.h)
+        _check(self._L.ck_batch_create_kv(engine.h, int(max_seqs), int(kv_blocks), self.KV[kv], ctypes.byref(b)),
+               engine.h)
         self.b = b
 
     def add(self, prompt: Sequence[int], max_new: int, eos_ids: Sequence[int] = ()) -> int:
@@ -331,6 +339,16 @@ class Batch:
         _check_batch(self._L.ck_batch_collect(self.b, int(seq_id), _u32p(out), out.size, ctypes.byref(n),
                                               ctypes.byref(done)), self.b)
         return out[:min(n.value, out.size)].tolist(), bool(done.value)
+
+    def read_kv(self, seq_id: int, layer: int) -> Tuple[np.ndarray, np.ndarray]:
+        """Keys and values [positions, kv_heads, head_dim] of a running sequence as a quantised cache holds them."""
+        cfg = self.engine.cfg
+        n = ctypes.c_int(0)
+        _check_batch(self._L.ck_batch_read_kv(self.b, int(seq_id), int(layer), None, None, 0, ctypes.byref(n)), self.b)
+        k, v = (np.zeros((n.value, cfg.kv_heads, cfg.head_dim), dtype=np.float32) for _ in range(2))
+        _check_batch(self._L.ck_batch_read_kv(self.b, int(seq_id), int(layer), k.ctypes.data, v.ctypes.data, n.value,
+                                              ctypes.byref(n)), self.b)
+        return k, v
 
     def stats(self) -> Tuple[int, int, int]:
         a, b, c = ctypes.c_uint64(0), ctypes.c_uint64(0), ctypes.c_uint64(0)

@@ -22,8 +22,12 @@
 //   data (pdl_wait).
 // * The step's kernels read the active count T from device memory, so one
 //   CUDA graph, captured at the first step, serves every T.
-// Supported: llama / qwen3 architectures with an fp16 KV cache, greedy
-// decoding.
+// * With a quantised cache (ck_batch_create_kv: keys in 8 bits, values in 8 or
+//   4) the attention of a layer is the cache's own operators (ck_kv.cu): norms,
+//   rotation and the quantised K/V store of every entry (k_kv_store), then the
+//   entries' attention, a long sequence's positions split over the device
+//   (k_kv_token, k_kv_join), and k_bhalf_tiles.
+// Supported: llama / qwen3 architectures, greedy decoding.
 
 #define CK_BLK 16        // positions per KV block
 
@@ -883,6 +887,22 @@ __global__ void __launch_bounds__(NT, 2 * CK_THREADS / NT) k_battn_g(BAttn P, BS
   if (tid == 0 && kvh == 0) P.xo.xs[t] = 1.0f;
 }
 
+// fp16 rows [T][k] as the next matmul's operand tiles: hi = the value, lo = 0,
+// scale 1 (the quantised cache's attention output).
+__global__ void __launch_bounds__(128) k_bhalf_tiles(const __half* a, int k, BStep st, BXh x) {
+  const int t = blockIdx.x, nch = tc_nch(k);
+  pdl_wait();
+  pdl_launch();
+  if (t >= *st.nact) return;
+  for (int i = 8 * threadIdx.x; i < nch * TC_KC; i += 8 * 128) {
+    // columns past k in the last chunk meet zero weights: keep them finite
+    const uint4 v = i < k ? *(const uint4*)(a + (size_t)t * k + i) : make_uint4(0u, 0u, 0u, 0u);
+    *(uint4*)(x.xt + tc_index(t, i, nch, 0)) = v;
+    *(uint4*)(x.xt + tc_index(t, i, nch, 1)) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (threadIdx.x == 0) x.xs[t] = 1.0f;
+}
+
 // Greedy id of every active entry: ARGMAX_STAGE1/2 rules (NaN never wins,
 // ties go to the lower index) over its logits row.
 __global__ void __launch_bounds__(CK_THREADS) k_bargmax(const float* logits, int V, BStep st, uint32_t* ids) {
@@ -922,6 +942,12 @@ struct ck_batch {
   std::vector<void*> allocs;
   std::string err;
   __half* kv = nullptr;       // [layers][K|V][n_blocks][kv_heads][CK_BLK][head_dim]
+  // quantised cache (kv_kind not CK_BATCH_KV_F16): the layers' pages, the
+  // rotated q and the attention output in fp16, the attention's workspace
+  int kv_kind = CK_BATCH_KV_F16, sms = 0;
+  KvPool pool{};              // of layer 0; layer i begins i * kv_pool_bytes further along
+  __half *q16 = nullptr, *o16 = nullptr;
+  float *kv_part = nullptr, *kv_ml = nullptr;
   uint32_t* d_tok = nullptr;
   int *d_slot = nullptr, *d_pos = nullptr, *d_nact = nullptr, *d_btab = nullptr, *d_err = nullptr;
   uint32_t* d_ids = nullptr;
@@ -1132,6 +1158,74 @@ void bprep(ck_batch* b, cudaStream_t s, int kind, const float* a, const float* b
   launch_pdl(k_bprep, dim3(b->max_seqs), dim3(CK_THREADS), s, p, bstep(b), x);
 }
 
+KvPool kvq_pool(const ck_batch* b, int layer) {
+  KvPool p = b->pool;
+  p.base += (size_t)layer * kv_pool_bytes(p);
+  return p;
+}
+KvTable kvq_table(const ck_batch* b) {
+  KvTable t;
+  t.dev = b->d_btab;
+  t.n_seqs = b->max_seqs;
+  t.max_blocks = b->max_blocks;
+  return t;
+}
+KvRows kvq_rows(const void* p, int heads, int hd, int type) {
+  KvRows r;
+  r.p = (void*)p;
+  r.st = (long long)heads * hd;
+  r.sh = hd;
+  r.type = type;
+  return r;
+}
+
+// A layer's attention over its quantised pages: the active entries' K and V
+// stored, then their attention into the o projection's operand tiles.
+int kvq_enqueue(ck_batch* b, cudaStream_t s, int layer) {
+  ck_engine* h = b->h;
+  const ck_model_cfg& c = h->cfg;
+  const int hd = c.head_dim;
+  KvStore w;
+  memset(&w, 0, sizeof w);
+  w.pool = kvq_pool(b, layer);
+  w.tab = kvq_table(b);
+  w.seq = b->d_slot;
+  w.pos = b->d_pos;
+  w.n_dev = b->d_nact;
+  w.n = b->max_seqs;
+  w.heads = c.heads;
+  w.q = kvq_rows(b->q, c.heads, hd, KV_F32);
+  w.k = kvq_rows(b->k, c.kv_heads, hd, KV_F32);
+  w.v = kvq_rows(b->v, c.kv_heads, hd, KV_F32);
+  w.qo = kvq_rows(b->q16, c.heads, hd, KV_F16);
+  w.qw = c.qk_norm ? h->L[layer].q_norm : nullptr;
+  w.kw = c.qk_norm ? h->L[layer].k_norm : nullptr;
+  w.inv_freq = h->inv_freq + (size_t)layer * (hd / 2);
+  w.eps = c.qk_norm_eps;
+  w.interleaved = c.rope_interleaved;
+  CKB(b, kv_store_launch(w, s, true));
+  KvAttn a;
+  memset(&a, 0, sizeof a);
+  a.pool = w.pool;
+  a.tab = w.tab;
+  a.seq = b->d_slot;
+  a.len = b->d_pos;
+  a.len_add = 1;              // the position just stored
+  a.n_dev = b->d_nact;
+  a.n = b->max_seqs;
+  a.heads = c.heads;
+  a.window = (int)c.layer_window[layer];
+  a.scale = (float)(1.0 / sqrt((double)hd));   // ATTN_SCALE (:1711)
+  a.q = kvq_rows(b->q16, c.heads, hd, KV_F16);
+  a.o = kvq_rows(b->o16, c.heads, hd, KV_F16);
+  a.part = b->kv_part;
+  a.ml = b->kv_ml;
+  CKB(b, kv_attend_launch(a, b->sms, s, true));
+  CKB(b, launch_pdl(k_bhalf_tiles, dim3(b->max_seqs), dim3(128), s, (const __half*)b->o16, c.heads * hd, bstep(b),
+                    b->xh));
+  return CK_OK;
+}
+
 // The whole step on stream s (captured once into a graph).
 int batch_enqueue(ck_batch* b, cudaStream_t s) {
   ck_engine* h = b->h;
@@ -1150,6 +1244,9 @@ int batch_enqueue(ck_batch* b, cudaStream_t s) {
     int rc = bgemm_launch(b, s, H, {bseg(W.q, wt[0], b->q, nullptr, qd), bseg(W.k, wt[1], b->k, nullptr, kvd),
                                     bseg(W.v, wt[2], b->v, nullptr, kvd)}, b->xn, nullptr, i > 0);
     if (rc) return rc;
+    if (b->kv_kind != CK_BATCH_KV_F16) {
+      if ((rc = kvq_enqueue(b, s, i))) return rc;
+    } else {
     BAttn a;
     a.q = b->q; a.k = b->k; a.v = b->v;
     a.qw = c.qk_norm ? W.q_norm : nullptr;
@@ -1172,6 +1269,7 @@ int batch_enqueue(ck_batch* b, cudaStream_t s) {
     else if (hd == 64) CKB(b, launch_pdl(k_battn<2>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
     else if (hd == 128) CKB(b, launch_pdl(k_battn<4>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
     else CKB(b, launch_pdl(k_battn<8>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
+    }
     if ((rc = bgemm_launch(b, s, qd, {bseg(W.o, wt[3], b->x, b->x, H)}, b->xh, W.post_norm))) return rc;
     if (b->glu) {   // silu(gate) * up straight into the down projection's tiles (xh.xs stays 1)
       BSeg gu = bseg(W.gate, wt[4], nullptr, nullptr, 0);
@@ -1201,8 +1299,14 @@ int batch_enqueue(ck_batch* b, cudaStream_t s) {
 extern "C" {
 
 int ck_batch_create(ck_engine* h, int max_seqs, int kv_blocks, ck_batch** out) {
+  return ck_batch_create_kv(h, max_seqs, kv_blocks, CK_BATCH_KV_F16, out);
+}
+
+int ck_batch_create_kv(ck_engine* h, int max_seqs, int kv_blocks, int kv_kind, ck_batch** out) {
   if (!h || !out) return set_global(CK_EINVAL, "ck_batch_create: bad argument");
   *out = nullptr;
+  if (kv_kind != CK_BATCH_KV_F16 && kv_kind != CK_BATCH_KV_Q8 && kv_kind != CK_BATCH_KV_Q8V4)
+    return h->fail(CK_EINVAL, "unknown cache kind %d", kv_kind);
   if (!h->finalized) return h->fail(CK_ESTATE, "engine not finalized");
   const ck_model_cfg& c = h->cfg;
   if (c.arch != CK_ARCH_LLAMA) return h->fail(CK_EINVAL, "batched decode supports the llama / qwen3 architectures");
@@ -1231,8 +1335,28 @@ int ck_batch_create(ck_engine* h, int max_seqs, int kv_blocks, ck_batch** out) {
     return bail(b->fail(CK_ECUDA, "stream"));
   const int H = c.hidden, qd = c.heads * c.head_dim, kvd = c.kv_heads * c.head_dim, I = c.intermediate;
   const size_t S = (size_t)max_seqs;
-  const size_t kv_bytes = (size_t)c.layers * 2 * b->n_blocks * c.kv_heads * CK_BLK * c.head_dim * 2;
-  if ((rc = balloc(b, &b->kv, kv_bytes)) || (rc = balloc(b, &b->d_tok, S * 4)) ||
+  b->kv_kind = kv_kind;
+  if (kv_kind == CK_BATCH_KV_F16) {
+    const size_t kv_bytes = (size_t)c.layers * 2 * b->n_blocks * c.kv_heads * CK_BLK * c.head_dim * 2;
+    if ((rc = balloc(b, &b->kv, kv_bytes))) return bail(rc);
+  } else {
+    KvPool& p = b->pool;
+    p.n_blocks = b->n_blocks;
+    p.kvh = c.kv_heads;
+    p.block = CK_BLK;
+    p.hd = c.head_dim;
+    p.vbits = kv_kind == CK_BATCH_KV_Q8 ? 8 : 4;
+    size_t pb = 0, mb = 0;
+    if (cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, h->device) != cudaSuccess ||
+        kv_setup(p) != cudaSuccess)
+      return bail(b->fail(CK_ECUDA, "quantised cache set-up"));
+    kv_workspace(p, c.heads, b->sms, &pb, &mb);
+    if ((rc = balloc(b, &p.base, (size_t)c.layers * kv_pool_bytes(p))) || (rc = balloc(b, &b->kv_part, pb)) ||
+        (rc = balloc(b, &b->kv_ml, mb)) || (rc = balloc(b, &b->q16, S * qd * 2)) ||
+        (rc = balloc(b, &b->o16, S * qd * 2)))
+      return bail(rc);
+  }
+  if ( (rc = balloc(b, &b->d_tok, S * 4)) ||
       (rc = balloc(b, &b->d_slot, S * 4)) || (rc = balloc(b, &b->d_pos, S * 4)) ||
       (rc = balloc(b, &b->d_nact, 16)) || (rc = balloc(b, &b->d_btab, S * max_blocks * 4)) ||
       (rc = balloc(b, &b->d_err, 16)) || (rc = balloc(b, &b->d_ids, S * 4)) ||
@@ -1279,6 +1403,7 @@ int ck_batch_create(ck_engine* h, int max_seqs, int kv_blocks, ck_batch** out) {
     if (cudaGetLastError() != cudaSuccess || cudaStreamSynchronize(b->stream) != cudaSuccess)
       return bail(b->fail(CK_ECUDA, "weight tiles"));
   }
+  b->pool.err = b->d_err + 1;
   if (cudaMemset(b->d_err, 0, 16) != cudaSuccess || cudaMemset(b->d_nact, 0, 16) != cudaSuccess ||
       cudaMemset(b->d_btab, 0, S * max_blocks * 4) != cudaSuccess)
     return bail(b->fail(CK_ECUDA, "memset"));
@@ -1371,11 +1496,12 @@ int ck_batch_step(ck_batch* b, int* n_active) {
   CKB(b, cudaGraphLaunch(b->graph, s));
   CKB(b, cudaMemcpyAsync(pids, b->d_ids, (size_t)T * 4, cudaMemcpyDeviceToHost, s));
   int* perr = pn + 1;
-  CKB(b, cudaMemcpyAsync(perr, b->d_err, 4, cudaMemcpyDeviceToHost, s));
+  CKB(b, cudaMemcpyAsync(perr, b->d_err, 8, cudaMemcpyDeviceToHost, s));   // the step's bits, the quantised cache's
   CKB(b, cudaStreamSynchronize(s));
-  if (*perr) {
-    const int bits = *perr;
-    cudaMemset(b->d_err, 0, 4);
+  if (perr[0] | perr[1]) {
+    const int bits = perr[0];
+    cudaMemset(b->d_err, 0, 8);
+    if (perr[1]) return b->fail(CK_EDEVICE, "batched step: quantised cache, device error bits 0x%x", perr[1]);
     if (bits & CK_DERR_TOKEN) return b->fail(CK_EDEVICE, "token id outside embedding table");
     return b->fail(CK_EDEVICE, "batched step: a device wait timed out (bits 0x%x)", bits);
   }
@@ -1431,6 +1557,53 @@ int ck_batch_stats(ck_batch* b, uint64_t* steps, uint64_t* tokens_fed, uint64_t*
   if (steps) *steps = b->steps;
   if (tokens_fed) *tokens_fed = b->fed;
   if (tokens_generated) *tokens_generated = b->generated;
+  return CK_OK;
+}
+
+// Cached keys and values of a running sequence in one layer, as the quantised
+// pages hold them.
+int ck_batch_read_kv(ck_batch* b, int seq_id, int layer, float* k, float* v, int cap, int* n_out) {
+  if (!b || !n_out || cap < 0 || (cap > 0 && (!k || !v))) return set_global(CK_EINVAL, "ck_batch_read_kv: bad argument");
+  const ck_model_cfg& c = b->h->cfg;
+  if (b->kv_kind == CK_BATCH_KV_F16) return b->fail(CK_EINVAL, "ck_batch_read_kv: the batch's cache is not quantised");
+  if (layer < 0 || layer >= c.layers) return b->fail(CK_EINVAL, "ck_batch_read_kv: layer %d of %d", layer, c.layers);
+  int slot = -1;
+  for (int i = 0; i < b->max_seqs; i++)
+    if (b->seqs[i].used && b->seqs[i].id == seq_id) slot = i;
+  if (slot < 0) return b->fail(CK_EINVAL, "unknown or finished sequence %d", seq_id);
+  *n_out = b->seqs[slot].pos;
+  const int n = *n_out < cap ? *n_out : cap;
+  if (n == 0) return CK_OK;
+  if (b->btab_dirty) return b->fail(CK_ESTATE, "ck_batch_read_kv: no step since the last change of the block tables");
+  CKB(b, cudaSetDevice(b->h->device));
+  const size_t rows = (size_t)n * c.kv_heads * c.head_dim * 4;
+  std::vector<int> at(2 * (size_t)n, slot);
+  for (int i = 0; i < n; i++) at[n + i] = i;
+  int* d_at = nullptr;
+  float *dk = nullptr, *dv = nullptr;
+  cudaError_t e = cudaMalloc(&d_at, at.size() * 4);
+  if (e == cudaSuccess) e = cudaMalloc(&dk, rows);
+  if (e == cudaSuccess) e = cudaMalloc(&dv, rows);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(d_at, at.data(), at.size() * 4, cudaMemcpyHostToDevice, b->stream);
+  if (e == cudaSuccess) {
+    KvLoad a;
+    memset(&a, 0, sizeof a);
+    a.pool = kvq_pool(b, layer);
+    a.tab = kvq_table(b);
+    a.seq = d_at;
+    a.pos = d_at + n;
+    a.n = n;
+    a.k = kvq_rows(dk, c.kv_heads, c.head_dim, KV_F32);
+    a.v = kvq_rows(dv, c.kv_heads, c.head_dim, KV_F32);
+    e = kv_load_launch(a, b->stream);
+  }
+  if (e == cudaSuccess) e = cudaMemcpyAsync(k, dk, rows, cudaMemcpyDeviceToHost, b->stream);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(v, dv, rows, cudaMemcpyDeviceToHost, b->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(b->stream);
+  cudaFree(d_at);
+  cudaFree(dk);
+  cudaFree(dv);
+  if (e != cudaSuccess) return b->fail(CK_ECUDA, "ck_batch_read_kv: %s", cudaGetErrorString(e));
   return CK_OK;
 }
 

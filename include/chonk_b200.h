@@ -221,6 +221,20 @@ typedef struct ck_batch ck_batch;
 /* max_seqs concurrent sequences; kv_blocks 16-position blocks of KV pool
  * (0 = enough for every slot at the full context length). */
 int ck_batch_create(ck_engine* h, int max_seqs, int kv_blocks, ck_batch** out);
+/* The same with a cache of another kind: keys in 8 bits, values in 8 or 4 (an
+ * fp16 scale per 32 values; the quantised paged cache's operators below run
+ * each layer's attention, which splits long sequences over the device).
+ * 2.1 or 1.6 bytes per pair of values instead of 4: longer contexts or more
+ * sequences in the same pool.  Ids then follow the quantised cache and may
+ * differ from those over fp16. */
+#define CK_BATCH_KV_F16 0
+#define CK_BATCH_KV_Q8 1      /* values in 8 bits */
+#define CK_BATCH_KV_Q8V4 2    /* values in 4 bits */
+int ck_batch_create_kv(ck_engine* h, int max_seqs, int kv_blocks, int kv_kind, ck_batch** out);
+/* Keys and values [n][kv_heads][head_dim] of a running sequence's first
+ * min(n, cap) positions in one layer, as a quantised batch's pages hold them
+ * (host fp32); *n = its cached positions. */
+int ck_batch_read_kv(ck_batch* b, int seq_id, int layer, float* k, float* v, int cap, int* n);
 /* Queue a sequence: prompt of n >= 1 ids, up to max_new >= 1 generated ids
  * (capped at the context left, as generateLlamaWgsl does), stopping after
  * an id in eos_ids (which is kept).  CK_EBUSY when every slot is taken,
