@@ -18,19 +18,33 @@
 namespace {
 
 template <typename... KArgs, typename... Args>
-cudaError_t kv_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl, Args... args) {
+cudaError_t kv_launch_cluster(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, int cs, cudaStream_t s, bool pdl,
+                              Args... args) {
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute at[2];
+  int na = 0;
+  if (pdl) {
+    at[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[na++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cs > 1) {
+    at[na].id = cudaLaunchAttributeClusterDimension;
+    at[na].val.clusterDim.x = cs;
+    at[na].val.clusterDim.y = at[na].val.clusterDim.z = 1;
+    na++;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = na;
   return cudaLaunchKernelEx(&cfg, k, args...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t kv_launch(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl, Args... args) {
+  return kv_launch_cluster(k, grid, block, smem, 1, s, pdl, args...);
 }
 
 }  // namespace
@@ -39,15 +53,10 @@ size_t kv_pool_bytes(const KvPool& p) {
   return (size_t)p.n_blocks * p.kvh * (p.block / KV_TILE) * kv_record_bytes(p.hd, p.vbits);
 }
 
-#ifndef KV_STORE_WARPS
-#define KV_STORE_WARPS 4096
-#endif
-#ifndef KVP_SPLIT_TILES
-#define KVP_SPLIT_TILES 8
-#endif
-#ifndef KV_UNIT_PAIRS
-#define KV_UNIT_PAIRS 32
-#endif
+
+#define KV_STORE_WARPS 4096  // warps that a write spreads its tokens over, a token's rows among up to 8
+#define KVP_SPLIT_TILES 8    // position tiles of a CTA, at least, where a prompt's cached positions are split
+#define KV_UNIT_PAIRS 32     // pairs of records of a unit, at most, for one-token attention by unit
 
 #define KV_EACH(X) X(64, 8) X(64, 4) X(128, 8) X(128, 4) X(256, 8) X(256, 4)
 
@@ -77,11 +86,12 @@ template <int HD, int VB>
 struct KvForms {
   using C = KvTok<HD, VB>;
   static constexpr auto list = k_kv_token<HD, VB, false, C::WARPS, C::STAGES>;
-  // by unit: 4 warps where the units fill the device, else 8
+  // by unit: 4 warps where the units fill the device, else 8 in up to 8 CTAs
   static constexpr int ST4 = HD == 256 ? 1 : 2, ST8 = HD == 256 ? 1 : 2;
   static constexpr auto unit4 = k_kv_token<HD, VB, true, 4, ST4>;
   static constexpr auto unit8 = k_kv_token<HD, VB, true, 8, ST8>;
-  static constexpr int SMEM4 = 4 * ST4 * C::PAIR_BYTES, SMEM8 = 8 * ST8 * C::PAIR_BYTES;
+  static constexpr int SUM = 8 * HD * 4;   // a CTA's sum
+  static constexpr int SMEM4 = 4 * ST4 * C::PAIR_BYTES + SUM, SMEM8 = 8 * ST8 * C::PAIR_BYTES + SUM;
   static cudaError_t setup() {
     cudaError_t e = cudaFuncSetAttribute(list, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit4, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM4);
@@ -90,11 +100,19 @@ struct KvForms {
       e = cudaFuncSetAttribute(k_kv_prompt<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB>::SMEM);
     return e;
   }
-  // form: warps of a unit's CTA, or 0 for the list
-  static cudaError_t launch(int form, const KvAttn& a, int units, int sms, cudaStream_t s, bool pdl) {
-    if (form == 4) return kv_launch(unit4, dim3(a.n * units), dim3(128), SMEM4, s, pdl, a);
-    if (form == 8) return kv_launch(unit8, dim3(a.n * units), dim3(256), SMEM8, s, pdl, a);
-    return kv_launch(list, dim3(sms), dim3(C::WARPS * 32), C::SMEM, s, pdl, a);
+  // pairs: most pairs of records that a unit can have.  *listed: whether the
+  // list was taken (its parts want joining).  By unit costs one launch instead
+  // of two, by list balances: 256 queries over up to 384 positions 14 us by
+  // unit, 23 by list; 24 over a window of 512 (head_dim 256) 12.5 and 20.5;
+  // from some 1000 positions on the longest unit of a ragged batch decides
+  static cudaError_t launch(const KvAttn& a, int units, long long pairs, int sms, cudaStream_t s, bool pdl, bool* listed) {
+    const long long n = (long long)a.n * units;
+    *listed = pairs > KV_UNIT_PAIRS;
+    if (*listed) return kv_launch(list, dim3(sms), dim3(C::WARPS * 32), C::SMEM, s, pdl, a, 1);
+    if (n >= 2 * sms) return kv_launch(unit4, dim3((unsigned)n), dim3(128), SMEM4, s, pdl, a, 1);
+    int cs = 1;   // idle SMs, while a warp has more than one pair
+    while (cs < 8 && 2 * cs * n <= sms && cs * 8 < pairs) cs *= 2;
+    return kv_launch_cluster(unit8, dim3((unsigned)(n * cs)), dim3(256), SMEM8, cs, s, pdl, a, cs);
   }
 };
 
@@ -147,18 +165,17 @@ cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pd
     else if (i0) { a.tab.dev += (size_t)i0 * a.tab.max_blocks; a.tab.n_seqs -= i0; }
     a.q.p = (char*)a.q.p + (size_t)i0 * a.q.st * 2;
     a.o.p = (char*)a.o.p + (size_t)i0 * a.o.st * 2;
-    // by unit when none has more than KV_UNIT_PAIRS pairs (the block table's
-    // width and the window bound them)
+    // most pairs of records of a unit: the block table's width and the window bound them
     long long pairs = ((long long)a.tab.max_blocks * a.pool.block + KV_PAIR - 1) / KV_PAIR;
     if (a.window > 0 && pairs > a.window / KV_PAIR + 2) pairs = a.window / KV_PAIR + 2;
-    const int form = pairs > KV_UNIT_PAIRS ? 0 : a.n * units >= 2 * sms ? 4 : 8;
+    bool listed = false;
     cudaError_t e = cudaErrorInvalidValue;
 #define KV_CASE(HD, VB) \
-  if (a.pool.hd == HD && a.pool.vbits == VB) e = KvForms<HD, VB>::launch(form, a, units, sms, s, pdl);
+  if (a.pool.hd == HD && a.pool.vbits == VB) e = KvForms<HD, VB>::launch(a, units, pairs, sms, s, pdl, &listed);
     KV_EACH(KV_CASE)
 #undef KV_CASE
     if (e != cudaSuccess) return e;
-    if (form) continue;
+    if (!listed) continue;
     // thread groups of the join: about half the partials that a unit has when all are alike
     const int most = 1024 / (a.pool.hd / 4);
     int rows = a.pool.hd == 64 ? 2 : 1;

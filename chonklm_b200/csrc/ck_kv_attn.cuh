@@ -16,8 +16,8 @@
 //             finished by its warp; the others leave unnormalised partial
 //             outputs with their (m, l), which k_kv_join adds in the order of
 //             the shares (no atomics: the result does not depend on timing).
-//   by unit   short caches: one CTA per unit, its warps' parts added through
-//             shared memory; one launch.
+//   by unit   short caches: one CTA or one cluster of CTAs per unit, the warps' parts added through shared memory, the CTAs'
+//             through distributed shared memory; one launch.
 //
 // Products run on m16n8k16 tensor instructions (a unit has 8 rows, too few for
 // tcgen05's 64-row tiles), the heads as the 8 columns: S^T = K Q^T with 16
@@ -38,17 +38,11 @@
 #define KV_SLACK 6.f         // log2 that a score may exceed the reference maximum before o is rescaled
 #define KV_BOOST 8.f         // p is kept times 2^8 (cancelled by l), so that small p stay normal fp16 numbers
 
-#ifndef KVW64
-#define KVW64 16
-#endif
-#ifndef KVW128
-#define KVW128 12
-#endif
 // by list: one CTA per SM; the warps that the registers allow (accumulators:
 // head_dim / 4 a thread) and the pairs that fit 209 KB
 template <int HD, int VB>
 struct KvTok {
-  static constexpr int WARPS = HD == 256 ? (VB == 8 ? 6 : 8) : HD == 128 ? KVW128 : KVW64;
+  static constexpr int WARPS = HD == 256 ? (VB == 8 ? 6 : 8) : HD == 128 ? 12 : 16;
   static constexpr int PAIR_BYTES = 2 * KvRec<HD, VB>::BYTES;
   static constexpr int FIT = 209 * 1024 / WARPS / PAIR_BYTES, STAGES = FIT > 4 ? 4 : FIT;
   static constexpr int SMEM = WARPS * STAGES * PAIR_BYTES;
@@ -162,22 +156,53 @@ struct KvSlots {
   int s0, cnt;
   bool mid;
   __device__ __forceinline__ KvSlots(long long a, long long tiles, long long per) {
-    s0 = (int)(a / per);
-    cnt = (int)((a + tiles - 1) / per) - s0 + 1;
+    const long long last = a + tiles - 1;
+    if (last >> 32) {
+      s0 = (int)(a / per);
+      cnt = (int)(last / per) - s0 + 1;
+    } else {                                   // (a 64-bit division is some 100 instructions)
+      s0 = (int)((uint32_t)a / (uint32_t)per);
+      cnt = (int)((uint32_t)last / (uint32_t)per) - s0 + 1;
+    }
     mid = a > s0 * per;
   }
   __device__ __forceinline__ int slot(int k) const { return 2 * (s0 + k) + (k == 0 && mid ? 1 : 0); }
 };
 
-// UNIT: by unit, W warps a CTA, ST stages each; else by list.
+__device__ __forceinline__ uint32_t kv_cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void kv_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// the same shared-memory address in CTA `rank` of the cluster
+__device__ __forceinline__ uint32_t kv_mapa(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 kv_ld_cluster4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 kv_ld_cluster2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+// UNIT: by unit, W warps a CTA, ST stages each, `cs` CTAs a unit; else by list.
 template <int HD, int VB, bool UNIT, int W, int ST>
-__global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : 16) / W : 1) k_kv_token(const __grid_constant__ KvAttn A) {
+__global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : HD == 64 ? 24 : 16) / W : 1) k_kv_token(const __grid_constant__ KvAttn A, int cs) {
   using R = KvRec<HD, VB>;
   constexpr int G = R::G, NT = W * 32, EPT = (KV_MAXQ + NT - 1) / NT, PB = 2 * R::BYTES;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ long long pre[UNIT ? 1 : KV_MAXQ + 1];
   __shared__ long long wsum[W];
-  __shared__ float2 uml[UNIT ? W : 1][8];
+  __shared__ float2 uml[UNIT ? W : 1][8], cml[8];
   __shared__ __align__(8) uint64_t bars[W * ST];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gsz = A.heads / A.pool.kvh, HB = (gsz + 7) / 8, U = A.pool.kvh * HB;
@@ -197,13 +222,14 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : 16) / W : 1) k
   long long w0 = 0;
   int todo;                                  // pairs of this warp
   if (UNIT) {
-    f.q = blockIdx.x / U;
-    f.u = blockIdx.x % U;
+    const int rank = blockIdx.x % cs, w = rank * W + warp, ws = cs * W;
+    f.q = blockIdx.x / cs / U;
+    f.u = blockIdx.x / cs % U;
     if (f.q >= n) return;
-    const int pairs = kv_pairs(kv_len(A, f.q), A.window, f.beg);
-    f.end = f.beg + pairs;
-    f.pair = f.beg + pairs * warp / W;
-    todo = f.beg + pairs * (warp + 1) / W - f.pair;
+    const long long pairs = kv_pairs(kv_len(A, f.q), A.window, f.beg);
+    f.end = f.beg + (int)pairs;
+    f.pair = f.beg + (int)(pairs * w / ws);
+    todo = f.beg + (int)(pairs * (w + 1) / ws) - f.pair;
   } else {
     // prefix sums of the queries' pairs over all their units
     long long mine[EPT], run = 0;
@@ -523,6 +549,7 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : 16) / W : 1) k
         uml[warp][2 * t + 1] = make_float2(m[1], l[1]);
       }
       __syncthreads();
+      float4* mine = (float4*)(ring + W * ST * PB);   // this CTA's sum, for the cluster
       for (int e = tid; e < nh * (HD / 4); e += NT) {
         const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
         float M = -INFINITY, L = 0.f;
@@ -537,9 +564,36 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : 16) / W : 1) k
           L += y * uml[w][h].y;
           x.x += y * v.x; x.y += y * v.y; x.z += y * v.z; x.w += y * v.w;
         }
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-        kv_st4(A.o, (size_t)c.q * A.o.st + (size_t)(h0 + h) * A.o.sh + d,
-               make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), vec);
+        if (cs == 1) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          kv_st4(A.o, (size_t)c.q * A.o.st + (size_t)(h0 + h) * A.o.sh + d,
+                 make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), vec);
+        } else {
+          mine[e] = x;
+          if (d == 0) cml[h] = make_float2(M, L);
+        }
+      }
+      if (cs > 1) {
+        kv_cluster_sync();
+        for (int e = (int)kv_cluster_rank() * NT + tid; e < nh * (HD / 4); e += cs * NT) {
+          const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
+          float M = -INFINITY, L = 0.f;
+          for (int k = 0; k < cs; k++) M = fmaxf(M, kv_ld_cluster2(kv_mapa(&cml[h], k)).x);
+          const float base = M == -INFINITY ? 0.f : M;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int k = 0; k < cs; k++) {
+            const float2 ml2 = kv_ld_cluster2(kv_mapa(&cml[h], k));
+            const float4 v = kv_ld_cluster4(kv_mapa(&mine[e], k));
+            const float y = kv_ex2(ml2.x - base);
+            L += y * ml2.y;
+            x.x += y * v.x; x.y += y * v.y; x.z += y * v.z; x.w += y * v.w;
+          }
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          kv_st4(A.o, (size_t)c.q * A.o.st + (size_t)(h0 + h) * A.o.sh + d,
+                 make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), vec);
+        }
+        kv_cluster_sync();                       // no CTA leaves while another reads its sum
       }
       return;
     }
@@ -595,7 +649,9 @@ __global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
   const int n = A.n_dev ? min(*A.n_dev, A.n) : A.n;
   const int gsz = A.heads / A.pool.kvh, HB = (gsz + 7) / 8, U = A.pool.kvh * HB;
   const int kvh = h / gsz, hh = h % gsz, u = kvh * HB + hh / 8, row = hh % 8;
-  const long long p0 = gpre[i], tiles = (gpre[i + 1] - p0) / U, per = kv_share(gpre[n], warps);
+  const long long p0 = gpre[i], all = gpre[i + 1] - p0, total = gpre[n];
+  const long long tiles = all >> 32 ? all / U : (uint32_t)all / (uint32_t)U;
+  const long long per = total >> 32 ? kv_share(total, warps) : ((uint32_t)total + warps - 1) / (uint32_t)warps;
   const int x = tid % L, y = tid / L;
   const size_t off = (size_t)i * A.o.st + (size_t)h * A.o.sh + 4 * x;
   if (tiles == 0) {
@@ -605,7 +661,12 @@ __global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
   const KvSlots S(p0 + u * tiles, tiles, per);
   if (S.cnt == 1) return;                    // finished by its warp
   float M = -INFINITY;
-  for (int k = tid; k < S.cnt; k += blockDim.x) M = fmaxf(M, ml[(size_t)S.slot(k) * 8 + row].x);
+  float2 first = make_float2(-INFINITY, 0.f);
+  for (int k = tid; k < S.cnt; k += blockDim.x) {
+    const float2 e = ml[(size_t)S.slot(k) * 8 + row];
+    if (k == tid) first = e;
+    M = fmaxf(M, e.x);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if ((tid & 31) == 0) red[tid >> 5] = M;
@@ -614,7 +675,7 @@ __global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
   const float base = M == -INFINITY ? 0.f : M;
   float l = 0.f;
   for (int k = tid; k < S.cnt; k += blockDim.x) {
-    const float2 e = ml[(size_t)S.slot(k) * 8 + row];
+    const float2 e = k == tid ? first : ml[(size_t)S.slot(k) * 8 + row];
     const float w = kv_ex2(e.x - base);
     wgt[k] = w;
     l += w * e.y;
