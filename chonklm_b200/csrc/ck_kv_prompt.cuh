@@ -49,7 +49,7 @@ struct KvPr {
   static constexpr int W_COPY = SOFT + DEQ, W_S = W_COPY + 1, W_O = W_COPY + 2;   // the single warps
   static constexpr int RECS = PT / KV_TILE;
   static constexpr int STAGE_BYTES = RECS * R::BYTES;
-  static constexpr int STAGES = HD == 256 ? 2 : 4;
+  static constexpr int STAGES = HD == 256 ? (VB == 8 ? 2 : 3) : 4;   // what fits
   static constexpr int QB = 128 * HD * 2, KB = PT * HD * 2;
   static constexpr int SQ = 0, SK = NQ * QB, SV = SK + BUF * KB, SST = SV + BUF * KB;
   // at least 120 KB, so that an SM holds one CTA (each takes all of its tensor memory)
