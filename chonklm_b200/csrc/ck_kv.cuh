@@ -172,8 +172,12 @@ __device__ __forceinline__ void kv_st4(const KvRows& r, size_t off, float4 f, bo
 // rotation pairs, with 16-byte loads and stores; a row is HD / 16 lanes, a
 // group of 32 values 4 lanes.  The cosines and sines of the token's position
 // are made once per warp and stay in registers, as do the norm weights.
-// Bound by its bytes for many tokens; the instructions come close (two IEEE
-// divisions a group, which the definition of scale and code needs).
+// By bytes it would be bound by memory, but the instructions come first: 16
+// heads and 8 kv heads of 128 take some 2500 warp instructions a token, two
+// IEEE divisions a group among them, which the definition of scale and code
+// needs.  Ragged prompts written and read back (302 MB in all) take 90 us, 71
+// of them the write; a first form, in which a lane held neighbouring values
+// of one half and loaded a row when it came to it, took 222.
 
 // the larger magnitude; NaN when either is
 __device__ __forceinline__ float kv_maxabs(float a, float b) {
@@ -423,9 +427,9 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
 // ---------------------------------------------------------------------------
 // Read back: a warp takes a token, a lane 8 neighbouring values of one of its
 // heads' key and value, and KV_LOAD_ROWS heads at once, whose loads are in
-// flight together.  Bound by its bytes; a row a thread with places looked up
-// for each took twice the instructions and 68 us where this takes 57 (293 MB, 79 % of the
-// copy bandwidth).
+// flight together.  Bound by its bytes: 293 MB in 57 us, 79 % of the copy
+// bandwidth.  A row at a time, its place looked up for each, took twice the
+// instructions and 68 us.
 
 #define KV_LOAD_THREADS 256
 #define KV_LOAD_ROWS 4

@@ -294,6 +294,28 @@ def test_token_attention_rows_of_the_table():
     _close(got, want, mag, top, 0)
 
 
+@pytest.mark.parametrize("window", [0, 40, 1600])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256), (24, 1, 128)])
+def test_token_attention_by_list(layout, window):
+    """Block tables too wide for a CTA per unit: ragged lengths, empty queries among them, cut into shares and joined; as
+    many queries as two launches take, by table row and by `seq`."""
+    H, K, hd = layout
+    lens = [1500, 0, 3, 700, 0, 0, 64, 1100, 1, 2100]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=21)
+    q = torch.randn(len(lens), H, hd, generator=g).mul_(2).half().cuda()
+    got = c.attend(q, _i32(lens), table, window=window)
+    want, mag, top = _ref_attention(q, k, v, lens, [1] * len(lens), 1 / math.sqrt(hd), window)
+    _close(got, want, mag, top, 0)
+    assert torch.equal(got, c.attend(q, _i32(lens), table, window=window))
+    n = 1100
+    order = torch.arange(n) % len(lens)
+    many = c.attend(q[order.cuda()].contiguous(), _i32(torch.tensor(lens)[order]), table, window=window, seq=_i32(order))
+    wide = c.attend(q[order.cuda()].contiguous(), _i32(torch.tensor(lens)[order]), table[order.cuda()].contiguous(), window=window)
+    c.check()
+    assert torch.equal(many, wide)
+    _close(many[-20:], *(t[order[-20:].cuda()] for t in (want, mag, top)), 0)   # the second launch's, shared out otherwise
+
+
 PROMPTS = [([1], [1]), ([5], [5]), ([127], [127]), ([129], [129]), ([300], [43]), ([513], [513]),
            ([64, 1, 257, 40, 700], [64, 1, 130, 3, 65]), ([33, 20], [0, 20]), ([16] * 40, [7] * 40)]
 
@@ -312,6 +334,38 @@ def test_prompt_attention(layout, case, window):
     want, mag, top = _ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), window)
     _close(got, want, mag, top, 2.0 ** -11)
     assert torch.equal(got, c.attend_prompt(q, cu, _i32(lens), table, window=window))
+
+
+@pytest.mark.parametrize("window", [0, 900])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+def test_prompt_attention_over_a_long_cache(layout, window):
+    """Few rows on long caches: the positions are split over CTAs and joined; rows and sequences that see nothing, and
+    parts of a split that nothing of a tile falls into."""
+    H, K, hd = layout
+    lens, news = [3000, 17, 0, 1500, 5], [33, 17, 2, 1, 9]
+    c, table, k, v, g = _filled(H, K, hd, lens, 32, 8, seed=6)
+    q = torch.randn(sum(news), H, hd, generator=g).mul_(2).half().cuda()
+    cu = _i32(np.concatenate([[0], np.cumsum(news)]))
+    got = c.attend_prompt(q, cu, _i32(lens), table, window=window)
+    c.check()
+    want, mag, top = _ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), window)
+    _close(got, want, mag, top, 2.0 ** -11)
+    assert torch.equal(got, c.attend_prompt(q, cu, _i32(lens), table, window=window))
+
+
+def test_prompt_attention_of_more_sequences_than_a_launch_takes():
+    H, K, hd, S = 4, 2, 64, 1090
+    lens = [1 + i % 37 for i in range(S)]
+    news = [min(n, 1 + i % 5) for i, n in enumerate(lens)]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=12)
+    q = torch.randn(sum(news), H, hd, generator=g).mul_(2).half().cuda()
+    cu = np.concatenate([[0], np.cumsum(news)])
+    got = c.attend_prompt(q, _i32(cu), _i32(lens), table)
+    c.check()
+    for part in (slice(0, 40), slice(1010, S)):
+        rows = slice(int(cu[part.start]), int(cu[part.stop]))
+        want, mag, top = _ref_attention(q[rows], k[part], v[part], lens[part], news[part], 1 / math.sqrt(hd), 0)
+        _close(got[rows], want, mag, top, 2.0 ** -11)
 
 
 @pytest.mark.parametrize("n", [1, 64, 65, 128, 129, 192])
