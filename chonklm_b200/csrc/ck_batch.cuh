@@ -944,7 +944,8 @@ struct ck_batch {
   __half* kv = nullptr;       // [layers][K|V][n_blocks][kv_heads][CK_BLK][head_dim]
   // quantised cache (kv_kind not CK_BATCH_KV_F16): the layers' pages, the
   // rotated q and the attention output in fp16, the attention's workspace
-  int kv_kind = CK_BATCH_KV_F16, sms = 0;
+  int kv_kind = CK_BATCH_KV_F16;
+  KvDev kvdev{};
   KvPool pool{};              // of layer 0; layer i begins i * kv_pool_bytes further along
   __half *q16 = nullptr, *o16 = nullptr;
   float *kv_part = nullptr, *kv_ml = nullptr;
@@ -1220,7 +1221,7 @@ int kvq_enqueue(ck_batch* b, cudaStream_t s, int layer) {
   a.o = kvq_rows(b->o16, c.heads, hd, KV_F16);
   a.part = b->kv_part;
   a.ml = b->kv_ml;
-  CKB(b, kv_attend_launch(a, b->sms, s, true));
+  CKB(b, kv_attend_launch(a, b->kvdev, s, true));
   CKB(b, launch_pdl(k_bhalf_tiles, dim3(b->max_seqs), dim3(128), s, (const __half*)b->o16, c.heads * hd, bstep(b),
                     b->xh));
   return CK_OK;
@@ -1347,10 +1348,9 @@ int ck_batch_create_kv(ck_engine* h, int max_seqs, int kv_blocks, int kv_kind, c
     p.hd = c.head_dim;
     p.vbits = kv_kind == CK_BATCH_KV_Q8 ? 8 : 4;
     size_t pb = 0, mb = 0;
-    if (cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, h->device) != cudaSuccess ||
-        kv_setup(p) != cudaSuccess)
+    if (kv_setup(p, h->device, &b->kvdev) != cudaSuccess)
       return bail(b->fail(CK_ECUDA, "quantised cache set-up"));
-    kv_workspace(p, c.heads, b->sms, &pb, &mb);
+    kv_workspace(p, c.heads, b->kvdev.sms, &pb, &mb);
     if ((rc = balloc(b, &p.base, (size_t)c.layers * kv_pool_bytes(p))) || (rc = balloc(b, &b->kv_part, pb)) ||
         (rc = balloc(b, &b->kv_ml, mb)) || (rc = balloc(b, &b->q16, S * qd * 2)) ||
         (rc = balloc(b, &b->o16, S * qd * 2)))

@@ -56,7 +56,7 @@ size_t kv_pool_bytes(const KvPool& p) {
 
 #define KV_STORE_WARPS 4096  // warps that a write spreads its tokens over, a token's rows among up to 8
 #define KVP_SPLIT_TILES 8    // position tiles of a CTA, at least, where a prompt's cached positions are split
-#define KV_UNIT_PAIRS 32     // pairs of records of a unit, at most, for one-token attention by unit
+#define KV_UNIT_PAIRS 64     // pairs of records of a CTA, at most, for one-token attention by unit
 
 #define KV_EACH(X) X(64, 8) X(64, 4) X(128, 8) X(128, 4) X(256, 8) X(256, 4)
 
@@ -92,32 +92,59 @@ struct KvForms {
   static constexpr auto unit8 = k_kv_token<HD, VB, true, 8, ST8>;
   static constexpr int SUM = 8 * HD * 4;   // a CTA's sum
   static constexpr int SMEM4 = 4 * ST4 * C::PAIR_BYTES + SUM, SMEM8 = 8 * ST8 * C::PAIR_BYTES + SUM;
-  static cudaError_t setup() {
+  static cudaError_t setup(KvDev* d) {
     cudaError_t e = cudaFuncSetAttribute(list, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit4, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM4);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit8, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM8);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(k_kv_prompt<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB>::SMEM);
-    return e;
+    return e == cudaSuccess ? fit(d) : e;
+  }
+  // clusters of unit8 that run at once: they lie within a GPC, so fewer than SMs / size
+  static cudaError_t fit(KvDev* d) {
+    for (int i = 0; i < 4; i++) {
+      cudaLaunchConfig_t cfg;
+      memset(&cfg, 0, sizeof cfg);
+      cfg.gridDim = dim3(1 << i);
+      cfg.blockDim = dim3(256);
+      cfg.dynamicSmemBytes = SMEM8;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = 1 << i;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      const cudaError_t e = cudaOccupancyMaxActiveClusters(&d->clusters[i], unit8, &cfg);
+      if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
   }
   // pairs: most pairs of records that a unit can have.  *listed: whether the
   // list was taken (its parts want joining).  By unit costs one launch instead
-  // of two, by list balances: 256 queries over up to 384 positions 14 us by
-  // unit, 23 by list; 24 over a window of 512 (head_dim 256) 12.5 and 20.5;
-  // from some 1000 positions on the longest unit of a ragged batch decides
-  static cudaError_t launch(const KvAttn& a, int units, long long pairs, int sms, cudaStream_t s, bool pdl, bool* listed) {
+  // of two, by list balances; a CTA of a unit may have up to KV_UNIT_PAIRS
+  // pairs.  Measured at head_dim 128 (us by unit, by list), lengths from a
+  // third of the longest up: 16 queries of 2 units over up to 2000 positions 9
+  // and 15, over 8000 18 and 22, over 16000 30 and 28; 64 of 8 units over 1040
+  // 28 and 29, over 2000 49 and 47, over 8000 157 and 135.  Clusters that do
+  // not all run at once make a second wave: 16 of 8 CTAs, where 15 fit, 12.4,
+  // in clusters of 4 8.0
+  static cudaError_t launch(const KvAttn& a, int units, long long pairs, const KvDev& d, cudaStream_t s, bool pdl,
+                            bool* listed) {
     const long long n = (long long)a.n * units;
-    *listed = pairs > KV_UNIT_PAIRS;
-    if (*listed) return kv_launch(list, dim3(sms), dim3(C::WARPS * 32), C::SMEM, s, pdl, a, 1);
-    if (n >= 2 * sms) return kv_launch(unit4, dim3((unsigned)n), dim3(128), SMEM4, s, pdl, a, 1);
-    int cs = 1;   // idle SMs, while a warp has more than one pair
-    while (cs < 8 && 2 * cs * n <= sms && cs * 8 < pairs) cs *= 2;
+    int lc = 0;   // log2 of a unit's CTAs: more while SMs are idle and a warp has more than one pair
+    while (lc < 3 && (n << (lc + 1)) <= d.sms && n <= d.clusters[lc + 1] && (8 << lc) < pairs) lc++;
+    const int cs = 1 << lc;
+    *listed = pairs > (long long)KV_UNIT_PAIRS * cs;
+    if (*listed) return kv_launch(list, dim3(d.sms), dim3(C::WARPS * 32), C::SMEM, s, pdl, a, 1);
+    if (n >= 2 * d.sms) return kv_launch(unit4, dim3((unsigned)n), dim3(128), SMEM4, s, pdl, a, 1);
     return kv_launch_cluster(unit8, dim3((unsigned)(n * cs)), dim3(256), SMEM8, cs, s, pdl, a, cs);
   }
 };
 
-cudaError_t kv_setup(const KvPool& p) {
-#define KV_CASE(HD, VB) if (p.hd == HD && p.vbits == VB) return KvForms<HD, VB>::setup();
+cudaError_t kv_setup(const KvPool& p, int device, KvDev* d) {
+  const cudaError_t e = cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, device);
+  if (e != cudaSuccess) return e;
+#define KV_CASE(HD, VB) if (p.hd == HD && p.vbits == VB) return KvForms<HD, VB>::setup(d);
   KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
@@ -155,8 +182,8 @@ cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
   return cudaErrorInvalidValue;
 }
 
-cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pdl) {
-  const int warps = sms * kv_token_warps(all.pool.hd, all.pool.vbits), units = kv_units(all.heads, all.pool.kvh);
+cudaError_t kv_attend_launch(const KvAttn& all, const KvDev& d, cudaStream_t s, bool pdl) {
+  const int warps = d.sms * kv_token_warps(all.pool.hd, all.pool.vbits), units = kv_units(all.heads, all.pool.kvh);
   for (int i0 = 0; i0 < all.n; i0 += KV_MAXQ) {
     KvAttn a = all;
     a.n = all.n - i0 < KV_MAXQ ? all.n - i0 : KV_MAXQ;
@@ -171,7 +198,7 @@ cudaError_t kv_attend_launch(const KvAttn& all, int sms, cudaStream_t s, bool pd
     bool listed = false;
     cudaError_t e = cudaErrorInvalidValue;
 #define KV_CASE(HD, VB) \
-  if (a.pool.hd == HD && a.pool.vbits == VB) e = KvForms<HD, VB>::launch(a, units, pairs, sms, s, pdl, &listed);
+  if (a.pool.hd == HD && a.pool.vbits == VB) e = KvForms<HD, VB>::launch(a, units, pairs, d, s, pdl, &listed);
     KV_EACH(KV_CASE)
 #undef KV_CASE
     if (e != cudaSuccess) return e;
@@ -233,7 +260,8 @@ cudaError_t kv_prompt_launch(const KvAttn& all, int sms, cudaStream_t s) {
 
 struct ck_kv {
   ck_kv_cfg cfg;
-  int device, sms;
+  int device;
+  KvDev dev;
   KvPool pool;
   float *part, *ml;
   char err[256];
@@ -351,16 +379,15 @@ int ck_kv_create(const ck_kv_cfg* cfg, int device, ck_kv** out) {
     return kv_global(code, "ck_kv_create: %s: %s", what, cudaGetErrorString(e));
   };
   if (on.rc != cudaSuccess) return bail(CK_ECUDA, "device", on.rc);
-  cudaError_t e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device);
-  if (e != cudaSuccess) return bail(CK_ECUDA, "device", e);
+  cudaError_t e = kv_setup(p, device, &h->dev);
+  if (e != cudaSuccess) return bail(CK_ECUDA, "set-up", e);
   size_t pb = 0, mb = 0;
-  kv_workspace(p, cfg->heads, h->sms, &pb, &mb);
+  kv_workspace(p, cfg->heads, h->dev.sms, &pb, &mb);
 
   if ((e = cudaMalloc(&p.base, kv_pool_bytes(p))) != cudaSuccess || (e = cudaMalloc(&p.err, 16)) != cudaSuccess ||
       (e = cudaMalloc(&h->part, pb)) != cudaSuccess || (e = cudaMalloc(&h->ml, mb)) != cudaSuccess)
     return bail(CK_ENOMEM, "cudaMalloc", e);
-  if ((e = cudaMemset(p.err, 0, 16)) != cudaSuccess || (e = kv_setup(p)) != cudaSuccess ||
-      (e = cudaDeviceSynchronize()) != cudaSuccess)
+  if ((e = cudaMemset(p.err, 0, 16)) != cudaSuccess || (e = cudaDeviceSynchronize()) != cudaSuccess)
     return bail(CK_ECUDA, "set-up", e);
   *out = h;
   return CK_OK;
@@ -478,7 +505,7 @@ int ck_kv_attend(ck_kv* h, const ck_kv_attend_args* a, void* stream) {
     return h->fail(CK_EINVAL, "ck_kv_attend: %d queries for %d rows of the block table", a->n, a->table.n_seqs);
   OnDevice on(h->device);
   KVC(on.rc);
-  KVC(kv_attend_launch(p, h->sms, (cudaStream_t)stream, false));
+  KVC(kv_attend_launch(p, h->dev, (cudaStream_t)stream, false));
   return CK_OK;
 }
 
@@ -494,7 +521,7 @@ int ck_kv_attend_prompt(ck_kv* h, const ck_kv_attend_args* a, const int32_t* cu,
   p.cu = cu;
   OnDevice on(h->device);
   KVC(on.rc);
-  KVC(kv_prompt_launch(p, h->sms, (cudaStream_t)stream));
+  KVC(kv_prompt_launch(p, h->dev.sms, (cudaStream_t)stream));
   return CK_OK;
 }
 

@@ -67,11 +67,17 @@ struct KvAttn {
   float *part, *ml;          // partial outputs; prefix sums and the partials' (maximum, sum)
 };
 
+// what a launch has to know of the device
+struct KvDev {
+  int sms;
+  int clusters[4];           // clusters of 1, 2, 4 and 8 CTAs of k_kv_token by unit that run at once
+};
+
 int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes);
-cudaError_t kv_setup(const KvPool& p);   // kernel attributes; not inside a stream capture
+cudaError_t kv_setup(const KvPool& p, int device, KvDev* d);   // kernel attributes too; not inside a stream capture
 cudaError_t kv_store_launch(const KvStore& a, cudaStream_t s, bool pdl);
 cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s);
-cudaError_t kv_attend_launch(const KvAttn& a, int sms, cudaStream_t s, bool pdl);
+cudaError_t kv_attend_launch(const KvAttn& a, const KvDev& d, cudaStream_t s, bool pdl);
 cudaError_t kv_prompt_launch(const KvAttn& a, int sms, cudaStream_t s);
 size_t kv_pool_bytes(const KvPool& p);
 

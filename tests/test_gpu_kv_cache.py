@@ -316,6 +316,26 @@ def test_token_attention_by_list(layout, window):
     _close(many[-20:], *(t[order[-20:].cuda()] for t in (want, mag, top)), 0)   # the second launch's, shared out otherwise
 
 
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("window", [0, 700])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_token_attention_of_wide_tables(layout, window, v_bits):
+    """The same lengths under tables of several widths: few and many CTAs a unit, and shares of a list (the widest, where
+    no window bounds what can be visible).  Entries past a sequence's end are never read."""
+    H, K, hd = layout
+    lens = [1500, 0, 3, 700, 64, 1, 2100]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, v_bits, seed=22)
+    q = torch.randn(len(lens), H, hd, generator=g).mul_(2).half().cuda()
+    want, mag, top = _ref_attention(q, k, v, lens, [1] * len(lens), 1 / math.sqrt(hd), window)
+    for blocks in (table.shape[1], 300, 600, 1100):
+        wide = torch.full((len(lens), blocks), -7, dtype=torch.int32, device="cuda")
+        wide[:, : table.shape[1]] = table
+        got = c.attend(q, _i32(lens), wide, window=window)
+        c.check()
+        _close(got, want, mag, top, 0)
+        assert torch.equal(got, c.attend(q, _i32(lens), wide, window=window))
+
+
 PROMPTS = [([1], [1]), ([5], [5]), ([127], [127]), ([129], [129]), ([300], [43]), ([513], [513]),
            ([64, 1, 257, 40, 700], [64, 1, 130, 3, 65]), ([33, 20], [0, 20]), ([16] * 40, [7] * 40)]
 
