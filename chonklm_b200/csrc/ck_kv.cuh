@@ -179,6 +179,31 @@ __device__ __forceinline__ void kv_st4(const KvRows& r, size_t off, float4 f, bo
 // of them the write; a first form, in which a lane held neighbouring values
 // of one half and loaded a row when it came to it, took 222.
 
+// two 32-bit floats at once
+__device__ __forceinline__ uint64_t kv_two(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void kv_split(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t kv_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t kv_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t kv_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // the larger magnitude; NaN when either is
 __device__ __forceinline__ float kv_maxabs(float a, float b) {
   float r;
@@ -211,10 +236,11 @@ __device__ __forceinline__ uint2 kv_quant(const float (&f)[8], __half& scale) {
   // The lower end (and the upper one of 8 bits) is passed only where the
   // scale is so small that fp16 holds it roughly, or so large that it was cut
   float x[8];
+  const uint64_t inv2 = kv_two(inv, inv), magic = kv_two(12582912.f + (FOUR ? 8.f : 128.f), 12582912.f + (FOUR ? 8.f : 128.f));
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    x[e] = __fmul_rn(f[e], inv);
-    if (FOUR) x[e] = fminf(x[e], 7.f);
+  for (int e = 0; e < 8; e += 2) {
+    kv_split(kv_mul2(kv_two(f[e], f[e + 1]), inv2), x[e], x[e + 1]);
+    if (FOUR) x[e] = fminf(x[e], 7.f), x[e + 1] = fminf(x[e + 1], 7.f);
   }
   if (__any_sync(0xffffffffu, !(top * fabsf(inv) < (FOUR ? 8.5f : 127.5f)))) {
 #pragma unroll
@@ -222,7 +248,11 @@ __device__ __forceinline__ uint2 kv_quant(const float (&f)[8], __half& scale) {
   }
   uint32_t c[8];
 #pragma unroll
-  for (int e = 0; e < 8; e++) c[e] = __float_as_uint(__fadd_rn(x[e], 12582912.f + (FOUR ? 8.f : 128.f)));
+  for (int e = 0; e < 8; e += 2) {
+    const uint64_t y = kv_add2(kv_two(x[e], x[e + 1]), magic);
+    c[e] = (uint32_t)y;
+    c[e + 1] = (uint32_t)(y >> 32);
+  }
   return make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
                     __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
 }
@@ -313,16 +343,23 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
   };
   auto turn = [&](float (&a)[8], float (&b)[8]) {   // norm and rotation
     if (w) {
-      float ss = 0.f;
+      uint64_t s2 = kv_two(0.f, 0.f);
 #pragma unroll
-      for (int e = 0; e < 8; e++) ss += a[e] * a[e] + b[e] * b[e];
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t x = kv_two(a[e], a[e + 1]), z = kv_two(b[e], b[e + 1]);
+        s2 = kv_fma2(z, z, kv_fma2(x, x, s2));
+      }
+      float ss, s1;
+      kv_split(s2, ss, s1);
+      ss += s1;
 #pragma unroll
       for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float inv = rsqrtf(ss * (1.f / HD) + A.eps);
+      const uint64_t inv2 = kv_two(inv, inv);
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        a[e] = (a[e] * inv) * wa[e];
-        b[e] = (b[e] * inv) * wb[e];
+      for (int e = 0; e < 8; e += 2) {
+        kv_split(kv_mul2(kv_mul2(kv_two(a[e], a[e + 1]), inv2), kv_two(wa[e], wa[e + 1])), a[e], a[e + 1]);
+        kv_split(kv_mul2(kv_mul2(kv_two(b[e], b[e + 1]), inv2), kv_two(wb[e], wb[e + 1])), b[e], b[e + 1]);
       }
     }
     if (rope && inter) {
@@ -337,10 +374,11 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
       }
     } else if (rope) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float x = a[e], z = b[e];
-        a[e] = x * cn[e] - z * sn[e];
-        b[e] = x * sn[e] + z * cn[e];
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t x = kv_two(a[e], a[e + 1]), z = kv_two(b[e], b[e + 1]);
+        const uint64_t c = kv_two(cn[e], cn[e + 1]), s = kv_two(sn[e], sn[e + 1]);
+        kv_split(kv_fma2(kv_mul2(z, s), kv_two(-1.f, -1.f), kv_mul2(x, c)), a[e], a[e + 1]);
+        kv_split(kv_fma2(x, s, kv_mul2(z, c)), b[e], b[e + 1]);
       }
     }
   };

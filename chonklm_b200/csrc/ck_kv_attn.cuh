@@ -19,7 +19,7 @@
 //   by unit   short caches: one CTA or one cluster of CTAs per unit, the
 //             warps' parts added through shared memory, the CTAs' through
 //             distributed shared memory; one launch.
-// Measured at head_dim 128, 8-bit values: 64 sequences of 493 MB in all take
+// Measured at head_dim 128, 4-bit values: 64 sequences of 493 MB in all take
 // 92 us by list (5.4 TB/s, 82 % of the copy bandwidth; 375 warp instructions
 // a record, issue slots 61 % busy) and the join 9 more.  A warp a record, a
 // row of heads as the product's rows, took 139 us: pairs halve the fixed work

@@ -88,25 +88,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem, uint32_t a, uint64_t 
                " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem),
                "r"(a), "l"(db), "r"(idesc), "r"(acc));
 }
-// two 32-bit floats at once
-__device__ __forceinline__ uint64_t kvp_pair(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void kvp_split(uint64_t r, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
-}
-__device__ __forceinline__ uint64_t kvp_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t kvp_add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float kvp_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -638,27 +619,27 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           }
         }
       }
-      uint64_t sum2 = kvp_pair(0.f, 0.f), sum3 = sum2;
+      uint64_t sum2 = kv_two(0.f, 0.f), sum3 = sum2;
       {
         const float mb = m == -INFINITY ? 0.f : m;
-        const uint64_t sc2 = kvp_pair(sc, sc), mb2 = kvp_pair(-mb, -mb);
+        const uint64_t sc2 = kv_two(sc, sc), mb2 = kv_two(-mb, -mb);
         uint32_t y[32];
 #pragma unroll
         for (int e = 0; e < 64; e += 2) {
           float p, q;
-          kvp_split(kvp_fma2(kvp_pair(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, mb2), p, q);
+          kv_split(kv_fma2(kv_two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, mb2), p, q);
           p = kv_ex2(p);
           q = kv_ex2(q);
-          if (e & 2) sum3 = kvp_add2(sum3, kvp_pair(p, q));
-          else sum2 = kvp_add2(sum2, kvp_pair(p, q));
+          if (e & 2) sum3 = kv_add2(sum3, kv_two(p, q));
+          else sum2 = kv_add2(sum2, kv_two(p, q));
           y[e / 2] = kv_pack2(p, q);
         }
         tmem_st32(tS, y);
       }
-      sum2 = kvp_add2(sum2, sum3);
+      sum2 = kv_add2(sum2, sum3);
       {
         float s0, s1;
-        kvp_split(sum2, s0, s1);
+        kv_split(sum2, s0, s1);
         l += s0 + s1;
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
