@@ -171,13 +171,15 @@ __device__ __forceinline__ void kv_st4(const KvRows& r, size_t off, float4 f, bo
 // lane holds 8 neighbouring values of each half of a row: both members of its
 // rotation pairs, with 16-byte loads and stores; a row is HD / 16 lanes, a
 // group of 32 values 4 lanes.  The cosines and sines of the token's position
-// are made once per warp and stay in registers, as do the norm weights.
-// By bytes it would be bound by memory, but the instructions come first: 16
+// are made once per warp and lie in shared memory with the norm weights, so
+// that four CTAs fit an SM (three for 32-bit rows).
+// Its bytes would bound it, but what does is latency, then instructions: 16
 // heads and 8 kv heads of 128 take some 2500 warp instructions a token, two
 // IEEE divisions a group among them, which the definition of scale and code
-// needs.  Ragged prompts written and read back (302 MB in all) take 90 us, 71
-// of them the write; a first form, in which a lane held neighbouring values
-// of one half and loaded a row when it came to it, took 222.
+// needs.  Ragged prompts of 214 MB take 52 us (63 % of the copy bandwidth); with
+// cosines, sines and weights in registers, three CTAs an SM, 69; with the same
+// operands one by one instead of in pairs 71; five CTAs (48 registers) 72.  For
+// 32-bit rows three CTAs take 69 us, two 79, four 73.
 
 // two 32-bit floats at once
 __device__ __forceinline__ uint64_t kv_two(float a, float b) {
@@ -259,13 +261,23 @@ __device__ __forceinline__ uint2 kv_quant(const float (&f)[8], __half& scale) {
 
 #define KV_STORE_THREADS 256
 template <int HD, int VB, int TYPE>
-__global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv_store(const __grid_constant__ KvStore A, int vec, int lw) {
+__global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 3 : 4) k_kv_store(const __grid_constant__ KvStore A, int vec, int lw) {
   using R = KvRec<HD, VB>;
   constexpr int LPR = HD / 16, RPW = 32 / LPR, ES = TYPE == KV_F32 ? 4 : 2;   // lanes of a row, rows of a warp
-  __shared__ float2 cs[KV_STORE_THREADS / 32][HD / 2];
+  // a lane's 8 cosines, sines or weights of a half row are two 16-byte pieces:
+  // first pieces of all lanes, then second ones
+  __shared__ __align__(16) float cs[KV_STORE_THREADS / 32][2][HD / 2], sw[2][2][HD / 2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_wait();
   pdl_launch();
+  if (A.qw || A.kw) {
+    for (int i = threadIdx.x; i < 2 * HD; i += KV_STORE_THREADS) {
+      const float* w = i < HD ? A.qw : A.kw;
+      const int x = i & (HD / 2 - 1);
+      if (w) sw[i / HD][(i / (HD / 2)) & 1][((x >> 2) & 1) * (HD / 4) + (x >> 3) * 4 + (x & 3)] = w[i & (HD - 1)];
+    }
+    __syncthreads();
+  }
   const int gw = blockIdx.x * (KV_STORE_THREADS / 32) + warp, wpt = 1 << lw, t = gw >> lw, sub = gw & (wpt - 1);
   if (t >= (A.n_dev ? min(*A.n_dev, A.n) : A.n)) return;
   const int lr = lane % LPR, y = lane / LPR, kvh = A.pool.kvh;
@@ -303,46 +315,27 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
   fetch(0);
   const int seq = A.seq[t], pos = A.pos[t] + A.pos_add;
   const bool rope = A.inv_freq != nullptr, inter = A.interleaved;
-  float cn[8], sn[8];                            // of the lane's 8 pairs
   if (rope) {
     for (int i = lane; i < HD / 2; i += 32) {
       float s, c;
       sincosf((float)pos * A.inv_freq[i], &s, &c);
-      cs[warp][i] = make_float2(c, s);
+      const int x = inter ? i & (HD / 4 - 1) : i, at = inter ? (i / (HD / 4)) * (HD / 4) + x
+                                                             : ((x >> 2) & 1) * (HD / 4) + (x >> 3) * 4 + (x & 3);
+      cs[warp][0][at] = c;
+      cs[warp][1][at] = s;
     }
     __syncwarp();
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const float2 x = cs[warp][inter ? (e < 4 ? 0 : HD / 4) + 4 * lr + (e & 3) : 8 * lr + e];
-      cn[e] = x.x;
-      sn[e] = x.y;
-    }
   }
+  auto eight = [&](const float* x, uint64_t (&u)[4]) {       // the lane's of x [HD / 2], in pairs
+    const ulonglong2 v = *(const ulonglong2*)(x + 4 * lr), z = *(const ulonglong2*)(x + HD / 4 + 4 * lr);
+    u[0] = v.x; u[1] = v.y; u[2] = z.x; u[3] = z.y;
+  };
   uint8_t* rec0 = seq >= 0 ? kv_record(A.pool, A.tab, seq, pos, R::BYTES, 0) : nullptr;   // of kv head 0
   const size_t hbytes = (size_t)(A.pool.block / KV_TILE) * R::BYTES;                      // to the next kv head's
   const int p = pos & (KV_TILE - 1), g = lr >> 2, gb = R::G / 2 + g;                      // groups of the two halves
 
-  float wa[8], wb[8];
-  const float* w = nullptr;
-  auto weights = [&](const float* x) {
-    w = x;
-    if (w && ((uintptr_t)w & 15) == 0) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 x = __ldg((const float4*)(w + 8 * lr + e)), z = __ldg((const float4*)(w + HD / 2 + 8 * lr + e));
-        wa[e] = x.x; wa[e + 1] = x.y; wa[e + 2] = x.z; wa[e + 3] = x.w;
-        wb[e] = z.x; wb[e + 1] = z.y; wb[e + 2] = z.z; wb[e + 3] = z.w;
-      }
-    } else if (w) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        wa[e] = __ldg(w + 8 * lr + e);
-        wb[e] = __ldg(w + HD / 2 + 8 * lr + e);
-      }
-    }
-  };
-  auto turn = [&](float (&a)[8], float (&b)[8]) {   // norm and rotation
-    if (w) {
+  auto turn = [&](float (&a)[8], float (&b)[8], int key, bool norm) {   // norm and rotation
+    if (norm) {
       uint64_t s2 = kv_two(0.f, 0.f);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
@@ -356,13 +349,26 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
       for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float inv = rsqrtf(ss * (1.f / HD) + A.eps);
       const uint64_t inv2 = kv_two(inv, inv);
+      uint64_t wa[4], wb[4];
+      eight(sw[key][0], wa);
+      eight(sw[key][1], wb);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        kv_split(kv_mul2(kv_mul2(kv_two(a[e], a[e + 1]), inv2), kv_two(wa[e], wa[e + 1])), a[e], a[e + 1]);
-        kv_split(kv_mul2(kv_mul2(kv_two(b[e], b[e + 1]), inv2), kv_two(wb[e], wb[e + 1])), b[e], b[e + 1]);
+        kv_split(kv_mul2(kv_mul2(kv_two(a[e], a[e + 1]), inv2), wa[e / 2]), a[e], a[e + 1]);
+        kv_split(kv_mul2(kv_mul2(kv_two(b[e], b[e + 1]), inv2), wb[e / 2]), b[e], b[e + 1]);
       }
     }
-    if (rope && inter) {
+    if (!rope) return;
+    uint64_t c[4], n[4];
+    eight(cs[warp][0], c);
+    eight(cs[warp][1], n);
+    if (inter) {
+      float cn[8], sn[8];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        kv_split(c[e], cn[2 * e], cn[2 * e + 1]);
+        kv_split(n[e], sn[2 * e], sn[2 * e + 1]);
+      }
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         float x = a[e], z = a[e + 1];
@@ -372,19 +378,17 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
         b[e] = x * cn[4 + e / 2] - z * sn[4 + e / 2];
         b[e + 1] = x * sn[4 + e / 2] + z * cn[4 + e / 2];
       }
-    } else if (rope) {
+    } else {
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const uint64_t x = kv_two(a[e], a[e + 1]), z = kv_two(b[e], b[e + 1]);
-        const uint64_t c = kv_two(cn[e], cn[e + 1]), s = kv_two(sn[e], sn[e + 1]);
-        kv_split(kv_fma2(kv_mul2(z, s), kv_two(-1.f, -1.f), kv_mul2(x, c)), a[e], a[e + 1]);
-        kv_split(kv_fma2(x, s, kv_mul2(z, c)), b[e], b[e + 1]);
+        kv_split(kv_fma2(kv_mul2(z, n[e / 2]), kv_two(-1.f, -1.f), kv_mul2(x, c[e / 2])), a[e], a[e + 1]);
+        kv_split(kv_fma2(x, n[e / 2], kv_mul2(z, c[e / 2])), b[e], b[e + 1]);
       }
     }
   };
   const bool o16 = A.qo.type == KV_F16;
   char* qo = (char*)A.qo.p + ((long long)t * A.qo.st + (long long)(y + sub * RPW) * A.qo.sh + 8 * lr) * 2;
-  weights(nq ? A.qw : A.kw);
 #pragma unroll 1
   for (int i = 0; i < nv; i++) {
     float a[8], b[8];
@@ -393,7 +397,7 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
     const int r = fr;
     fetch(i + 1);
     if (i < nq) {
-      turn(a, b);
+      turn(a, b, 0, A.qw != nullptr);
       if (r < A.heads) {
         uint32_t u[4], x[4];
         if (o16) {
@@ -414,8 +418,7 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 2 : 3) k_kv
       }
       qo += (long long)step * A.qo.sh * 2;
     } else if (i < nk) {
-      if (i == nq && nq) weights(A.kw);
-      turn(a, b);
+      turn(a, b, 1, A.kw != nullptr);
       __half da, db;
       const uint2 ca = kv_quant<false>(a, da), cb = kv_quant<false>(b, db);
       if (r < kvh && rec0) {
