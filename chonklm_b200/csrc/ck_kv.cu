@@ -203,14 +203,20 @@ cudaError_t kv_attend_launch(const KvAttn& all, const KvDev& d, cudaStream_t s, 
 #undef KV_CASE
     if (e != cudaSuccess) return e;
     if (!listed) continue;
-    // thread groups of the join: about half the partials that a unit has when all are alike
-    const int most = 1024 / (a.pool.hd / 4);
-    int rows = a.pool.hd == 64 ? 2 : 1;
-    while (rows < most && 2 * rows * a.n * units < warps) rows *= 2;
-    const dim3 grid(a.n, a.heads), block(rows * a.pool.hd / 4);
-    if (a.pool.hd == 64) e = kv_launch(k_kv_join<64>, grid, block, 0, s, true, a, warps);
-    else if (a.pool.hd == 128) e = kv_launch(k_kv_join<128>, grid, block, 0, s, true, a, warps);
-    else e = kv_launch(k_kv_join<256>, grid, block, 0, s, true, a, warps);
+    // a head's CTAs in the join (each some of its dims) while there are fewer
+    // than SMs; thread groups: about half the partials that a unit has when all
+    // are alike
+    int z = 1;
+    while (a.pool.hd / 4 / (2 * z) >= 8 && 2LL * z * a.n * a.heads <= d.sms) z *= 2;
+    const int l = a.pool.hd / 4 / z, most = 1024 / l;
+    int rows = l < 32 ? 32 / l : 1;
+    while (rows < most && 2LL * rows * a.n * units < warps) rows *= 2;
+    const dim3 grid(a.n, a.heads, z), block(rows * l);
+    e = cudaErrorInvalidValue;
+#define KV_JOIN(HD, L) if (a.pool.hd == HD && l == L) e = kv_launch(k_kv_join<HD, L>, grid, block, 0, s, true, a, warps);
+    KV_JOIN(64, 16) KV_JOIN(64, 8) KV_JOIN(128, 32) KV_JOIN(128, 16) KV_JOIN(128, 8) KV_JOIN(256, 64) KV_JOIN(256, 32)
+    KV_JOIN(256, 16) KV_JOIN(256, 8)
+#undef KV_JOIN
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;

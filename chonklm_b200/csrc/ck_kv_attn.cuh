@@ -638,16 +638,18 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : HD == 64 ? 24 
   }
 }
 
-// Join: one CTA per (query, head) adds the partial outputs of its unit's
-// shares; zeros where a query sees nothing.  HD / 4 threads read one partial's
-// row (a float4 each), the CTA's other thread groups the next partials.
+// Join: one CTA per (query, head), or several with L float4s of its dims each,
+// adds the partial outputs of its unit's shares; zeros where a query sees
+// nothing.  L threads read one partial's row, the CTA's other thread groups
+// the next partials.
 // Bound by latency: one sequence of 71 MB (8 units) leaves some 220 partials a
-// unit; weighing and adding them takes 11 us beside k_kv_token's 20.  Joined by
-// the last warp to arrive instead (fences and atomics), a short call took
-// 10.1 us where the two launches take 8.7.
-template <int HD>
+// unit; weighing and adding them takes 8.5 us beside k_kv_token's 20, 11 with a
+// CTA a head, 16 with 256 threads.  Joined by the last warp to arrive instead
+// (fences and atomics), a short call took 10.1 us where the two launches take
+// 8.7.
+template <int HD, int L>
 __global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
-  constexpr int L = HD / 4, MAXW = 4096;
+  constexpr int MAXW = 4096;
   __shared__ float4 acc[1024];
   __shared__ float wgt[MAXW];                // weights of the partials (shares are at most the device's warps)
   __shared__ float red[64];
@@ -663,8 +665,8 @@ __global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
   const long long p0 = gpre[i], all = gpre[i + 1] - p0, total = gpre[n];
   const long long tiles = all >> 32 ? all / U : (uint32_t)all / (uint32_t)U;
   const long long per = total >> 32 ? kv_share(total, warps) : ((uint32_t)total + warps - 1) / (uint32_t)warps;
-  const int x = tid % L, y = tid / L;
-  const size_t off = (size_t)i * A.o.st + (size_t)h * A.o.sh + 4 * x;
+  const int x = tid % L, y = tid / L, dim = 4 * (blockIdx.z * L + x);
+  const size_t off = (size_t)i * A.o.st + (size_t)h * A.o.sh + dim;
   if (tiles == 0) {
     if (y == 0) kv_st4(A.o, off, make_float4(0.f, 0.f, 0.f, 0.f), kv_vec4(A.o));
     return;
@@ -698,16 +700,24 @@ __global__ void __launch_bounds__(1024) k_kv_join(KvAttn A, int warps) {
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
   for (int k = y; k < S.cnt; k += rows) {
-    const float4 v = *(const float4*)(A.part + ((size_t)S.slot(k) * 8 + row) * HD + 4 * x);
+    const float4 v = *(const float4*)(A.part + ((size_t)S.slot(k) * 8 + row) * HD + dim);
     const float w = wgt[k];
     o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
   }
-  acc[tid] = o;
+#pragma unroll
+  for (int e = L; e < 32; e <<= 1) {         // a warp's rows
+    o.x += __shfl_xor_sync(0xffffffffu, o.x, e);
+    o.y += __shfl_xor_sync(0xffffffffu, o.y, e);
+    o.z += __shfl_xor_sync(0xffffffffu, o.z, e);
+    o.w += __shfl_xor_sync(0xffffffffu, o.w, e);
+  }
+  const int groups = L < 32 ? blockDim.x / 32 : rows;
+  if (L >= 32 || (tid & 31) < L) acc[L < 32 ? (tid >> 5) * L + x : tid] = o;
   __syncthreads();
   if (y == 0) {
     l = 0.f;
     for (int w = 0; w < (int)blockDim.x / 32; w++) l += red[32 + w];
-    for (int k = 1; k < rows; k++) {
+    for (int k = 1; k < groups; k++) {
       const float4 v = acc[k * L + x];
       o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
     }
