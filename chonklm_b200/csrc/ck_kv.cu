@@ -56,7 +56,8 @@ size_t kv_pool_bytes(const KvPool& p) {
 
 #define KV_STORE_WARPS 4096  // warps that a write spreads its tokens over, a token's rows among up to 8
 #define KVP_SPLIT_TILES 8    // position tiles of a CTA, at least, where a prompt's cached positions are split
-#define KV_UNIT_PAIRS 64     // pairs of records of a CTA, at most, for one-token attention by unit
+#define KV_UNIT_PAIRS 256    // pairs of records of a unit, at most, for one-token attention by unit
+#define KV_CTA_PAIRS 64      // and of each of its CTAs
 
 #define KV_EACH(X) X(64, 8) X(64, 4) X(128, 8) X(128, 4) X(256, 8) X(256, 4)
 
@@ -121,20 +122,21 @@ struct KvForms {
   }
   // pairs: most pairs of records that a unit can have.  *listed: whether the
   // list was taken (its parts want joining).  By unit costs one launch instead
-  // of two, by list balances; a CTA of a unit may have up to KV_UNIT_PAIRS
-  // pairs.  Measured at head_dim 128 (us by unit, by list), lengths from a
-  // third of the longest up: 16 queries of 2 units over up to 2000 positions 9
-  // and 15, over 8000 18 and 22, over 16000 30 and 28; 64 of 8 units over 1040
-  // 28 and 29, over 2000 49 and 47, over 8000 157 and 135.  Clusters that do
-  // not all run at once make a second wave: 16 of 8 CTAs, where 15 fit, 12.4,
-  // in clusters of 4 8.0
+  // of two, by list balances.  Measured (us by unit, by list), lengths from a
+  // third of the longest up: at head_dim 128 one query of 2 units over up to
+  // 4000 positions 9.8 and 11.2, over 8000 12.8 and 11.8; 16 of 2 units (4 CTAs
+  // each) over 4000 12.4 and 17.8, over 8000 18.5 and 21.9; 64 of 8 units (a CTA
+  // each) over 1040 29.3 and 29.6, over 2000 48.4 and 48.1, over 8000 153 and
+  // 134; at head_dim 256 64 of one unit over 2000 17.6 and 28.0.  Clusters that
+  // do not all run at once make a second wave: 16 of 8 CTAs, where 15 fit, took
+  // 12.4, in clusters of 4 8.0
   static cudaError_t launch(const KvAttn& a, int units, long long pairs, const KvDev& d, cudaStream_t s, bool pdl,
                             bool* listed) {
     const long long n = (long long)a.n * units;
     int lc = 0;   // log2 of a unit's CTAs: more while SMs are idle and a warp has more than one pair
     while (lc < 3 && (n << (lc + 1)) <= d.sms && n <= d.clusters[lc + 1] && (8 << lc) < pairs) lc++;
     const int cs = 1 << lc;
-    *listed = pairs > (long long)KV_UNIT_PAIRS * cs;
+    *listed = pairs > KV_UNIT_PAIRS || pairs > KV_CTA_PAIRS * cs;
     if (*listed) return kv_launch(list, dim3(d.sms), dim3(C::WARPS * 32), C::SMEM, s, pdl, a, 1);
     if (n >= 2 * d.sms) return kv_launch(unit4, dim3((unsigned)n), dim3(128), SMEM4, s, pdl, a, 1);
     return kv_launch_cluster(unit8, dim3((unsigned)(n * cs)), dim3(256), SMEM8, cs, s, pdl, a, cs);
