@@ -34,7 +34,7 @@
 // -128 2^-24 sum(q) is where the sum begins, and each group's sum is
 // multiplied by its scale in 32 bits.  A value's byte becomes fp16 by
 // 0x6400 | byte = 1024 + byte.  Rounded to 16 bits: p = exp(s - m)
-// (11 bits; l sums the unrounded p) and a value code * scale (11 bits, as an
+// (11 bits; l sums the rounded p, so that weights still add up to one) and a value code * scale (11 bits, as an
 // fp16 cache would hold it).
 #pragma once
 #include "ck_kv.cuh"
@@ -479,10 +479,11 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : HD == 64 ? 24 
       for (int k = 0; k < 2; k++)
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-          const float x = kv_ex2(s[k][2 * j] - mb[0]), y = kv_ex2(s[k][2 * j + 1] - mb[1]);
-          l[0] += x;
-          l[1] += y;
-          pb[k][j] = kv_transpose(kv_pack2(x, y));
+          const __half2 p = __floats2half2_rn(kv_ex2(s[k][2 * j] - mb[0]), kv_ex2(s[k][2 * j + 1] - mb[1]));
+          const float2 f = __half22float2(p);
+          l[0] += f.x;
+          l[1] += f.y;
+          pb[k][j] = kv_transpose(*(const uint32_t*)&p);
         }
       // O^T += V^T P^T
 #pragma unroll
