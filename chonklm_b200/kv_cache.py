@@ -12,8 +12,9 @@ fp16 scale for each 32 values of a head.  The caller keeps the block table
 
 Every call enqueues its kernel on `stream` (a cudaStream_t as an integer) or,
 by default, on torch's current stream of the cache's device, and returns
-without waiting; calls on one cache have to be ordered among themselves.  A
-tensor that is used on another stream than its own is the caller's to keep
+without waiting; calls on one cache have to be ordered among themselves.  An
+output that a call makes itself is memory of the stream that the call runs on.
+A tensor that is used on another stream than its own is the caller's to keep
 alive (`Tensor.record_stream`).  A wrong argument raises ValueError or
 CkError; what only the device can see (a sequence, position or block out of
 range) is skipped there and raised by `check()`.  There is no CPU fallback.
@@ -94,6 +95,14 @@ class QuantKvCache:
     def _stream(self, stream: Optional[int]) -> int:
         return _raw_stream(self.device) if stream is None else stream
 
+    def _make(self, stream: Optional[int], empty, *args, **kw):
+        """An output in memory of the stream that writes it: what is still pending elsewhere does not write there."""
+        if stream is None or stream == _raw_stream(self.device):
+            return empty(*args, **kw)
+        s = torch.cuda.ExternalStream(stream, self._dev) if stream else torch.cuda.default_stream(self._dev)
+        with torch.cuda.stream(s):
+            return empty(*args, **kw)
+
     def _check(self, rc: int) -> None:
         if rc:
             raise _lib.CkError(rc, (self._L.ck_kv_last_error(self.h) or b"").decode("utf-8", "replace"))
@@ -108,7 +117,7 @@ class QuantKvCache:
         n = k.shape[0]
         if q is not None:
             if out is None:
-                out = torch.empty_like(q, dtype=torch.float16) if q.dtype is torch.float32 else torch.empty_like(q)
+                out = self._make(stream, torch.empty_like, q, dtype=torch.float16 if q.dtype is torch.float32 else q.dtype)
             qa, oa = self._rows("q", q, n, self.heads), self._rows("out", out, n, self.heads, False)
         else:
             if out is not None:
@@ -125,8 +134,8 @@ class QuantKvCache:
         """(k, v) [n, kv_heads, head_dim] of the tokens (seq[i], pos[i]) as the cache holds them."""
         n = seq.shape[0]
         if out is None:
-            first = torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self._dev)
-            out = first, torch.empty_like(first)
+            shape = n, self.kv_heads, self.head_dim
+            out = tuple(self._make(stream, torch.empty, shape, dtype=dtype, device=self._dev) for _ in range(2))
         a = _LOAD.pack(*self._rows("k", out[0], n, self.kv_heads), *self._rows("v", out[1], n, self.kv_heads),
                        *self._table(table), self._ints("seq", seq, n), self._ints("pos", pos, n), n, 0)
         self._check(self._L.ck_kv_load(self.h, a, self._stream(stream)))
@@ -138,7 +147,7 @@ class QuantKvCache:
         cached positions, the new one among them; sequence i of the table, or seq[i].  scale: 1 / sqrt(head_dim)."""
         n = q.shape[0]
         if out is None:
-            out = torch.empty_like(q)
+            out = self._make(stream, torch.empty_like, q)
         a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
                          *self._table(table), self._ints("length", length, n), 0 if seq is None else self._ints("seq", seq, n),
                          n, window, self._scale if scale is None else scale, 0)
@@ -151,7 +160,7 @@ class QuantKvCache:
         sequence i's length[i] cached positions (row i of the table)."""
         n = q.shape[0]
         if out is None:
-            out = torch.empty_like(q)
+            out = self._make(stream, torch.empty_like, q)
         s = cu.numel() - 1
         if s < 0:
             raise ValueError("cu: expected one entry more than sequences")
