@@ -77,6 +77,15 @@ __device__ __forceinline__ uint8_t* kv_record(const KvPool& P, const KvTable& T,
          ((((size_t)b * P.kvh + head) << (lb - 4)) + ((pos & (P.block - 1)) >> 4)) * (size_t)rec_bytes;
 }
 
+// Waits, a bounded time each, for the copies `from` .. `to` - 1 of a ring: a
+// kernel that gives up must not leave while one of them can still write to its
+// shared memory.
+__device__ __forceinline__ void kv_drain(uint64_t* bar, int from, int to, int stages) {
+#pragma unroll 1
+  for (int i = from; i < to; i++)
+    for (unsigned spins = 0; !mbar_try_wait(bar + i % stages, kv_ring_parity(i, stages)) && spins < (1u << 20); spins++) {}
+}
+
 // ---- eight neighbouring elements of a row ----------------------------------
 // they may move as 16-byte vectors: base and strides are multiples of that
 __host__ __device__ inline bool kv_vec8(const KvRows& r) {

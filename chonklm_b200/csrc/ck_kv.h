@@ -12,6 +12,20 @@
 
 enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
 
+#ifdef __CUDACC__
+#define KV_HD __host__ __device__
+#else
+#define KV_HD
+#endif
+// Copies through a ring of `stages` buffers, a barrier each: copy i (counted
+// from 0) lies in buffer i % stages and ends phase i / stages of its barrier,
+// so a wait for it asks for this parity.  (The other parity is that of the
+// phase before, which has ended: asking for either waits for nothing.)
+KV_HD inline unsigned kv_ring_parity(int i, int stages) { return (unsigned)(i / stages) & 1u; }
+// The first copy that can still be in flight when `issued` have been issued:
+// a buffer is filled again only once its copy has landed.
+KV_HD inline int kv_ring_first(int issued, int stages) { return issued > stages ? issued - stages : 0; }
+
 // One layer's pages: records of 16 positions of one kv head, [block][kv head]
 // [16-position tile of the block] (record layout in ck_kv.cuh).
 struct KvPool {

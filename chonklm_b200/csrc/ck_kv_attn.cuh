@@ -411,6 +411,7 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : HD == 64 ? 24 
         while (!mbar_try_wait(bar + cstage, parity) && ++spins < (1u << 22)) {}
         if (__any_sync(0xffffffffu, spins >= (1u << 22))) {
           if (lane == 0) atomicOr(A.pool.err, KV_ERR_WAIT);
+          kv_drain(bar, at, fetched, ST);
           gave_up = true;
           break;
         }
