@@ -330,9 +330,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     mbar_arrive(&b_q);
   }
 
+  int issued = 0;                              // tiles whose copies are on their way or have landed (copy warp)
   if (warp == C::W_COPY) {
     // ---- copies: lane i fetches record i of the tile ----
-    for (int j = jb; j < je; j++) {
+    for (int j = jb; j < je; j++, issued++) {
       const int it = j - jb, s = it % C::STAGES;
       if (it >= C::STAGES && !kvp_wait(&b_empty[s], (it / C::STAGES - 1) & 1, &s_fail, A.pool.err)) break;
       const int tile = j * C::RECS + lane;     // record of the sequence
@@ -359,9 +360,6 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         bulk_g2s(dst, A.pool.base + (((size_t)id * A.pool.kvh + kvh) * bpt + tile % bpt) * R::BYTES, R::BYTES,
                  &b_full[s]);
     }
-    if (s_fail)                                // no copy may land after the CTA has gone
-      for (int s = 0; s < min(C::STAGES, je - jb); s++)
-        for (unsigned spins = 0; !mbar_try_wait(&b_full[s], 0) && !mbar_try_wait(&b_full[s], 1) && spins < (1u << 20); spins++) {}
   } else if (warp == C::W_S || warp == C::W_O) {
     // ---- products ----
     // The whole warp runs the loop and one elected lane issues: operands that
@@ -684,8 +682,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
             make_float2(m, l);
     }
   }
-  // no CTA leaves, or frees its tensor memory, with a product in flight
+  // no CTA leaves with a copy in flight (any role may have given up, after the
+  // last copy was issued too), and none frees its tensor memory under a product
   __syncthreads();
+  if (warp == C::W_COPY && s_fail) kv_drain(b_full, kv_ring_first(issued, C::STAGES), issued, C::STAGES);
   if ((warp == C::W_S || warp == C::W_O) && elect_one()) umma_commit(&b_end);
   if (warp == 2) {
     unsigned spins = 0;
