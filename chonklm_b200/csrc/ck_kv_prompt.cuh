@@ -102,6 +102,11 @@ __device__ __forceinline__ bool kvp_bad(uint32_t d) {
   return (d & 0x7fffu) > (VB == 8 ? 0x6007u : 0x6fffu);      // 515.5 (x 127) and 8188 (x 8)
 }
 
+// The first position that the token at position pos sees (pos < 0: a row
+// before its sequence, which sees nothing; no sum here passes 32 bits, however
+// wide the window).
+__device__ __forceinline__ int kvp_low(int pos, int window) { return window > 0 && pos >= window ? pos + 1 - window : 0; }
+
 // A whole warp waits for a phase of bar (all lanes get the same answer); gives
 // up (false) after a bounded number of polls or when another role of the CTA
 // has given up.
@@ -229,8 +234,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     const int first = (128 * w) / gs, last = min(ntok, (128 * w + 127) / gs + 1) - 1;   // tokens with a row in it
     if (first > last) { beg = end = 0; return; }
     const int plo = pos0 + first, phi = pos0 + last;
-    const int lo = A.window > 0 ? max(0, plo + 1 - A.window) : 0;
-    beg = lo / C::PT;
+    beg = kvp_low(plo, A.window) / C::PT;
     end = len > 0 && phi >= 0 ? phi / C::PT + 1 : beg;
     if (end < beg) end = beg;
   };
@@ -556,7 +560,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     kvp_wait(&b_q, 0, &s_fail, A.pool.err);
     const float sc = s_scale[rr];
     const int rpos = pos0 + rtok;                                 // position of the row's token
-    const int rlo = A.window > 0 ? max(0, rpos + 1 - A.window) : 0;
+    const int rlo = kvp_low(rpos, A.window);
     float m = -INFINITY, l = 0.f;
     const uint32_t tO = tmem + C::TO + wq * HD + lanes;
     bool ok = true;

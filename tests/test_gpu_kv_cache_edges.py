@@ -43,3 +43,18 @@ def test_default_outputs_belong_to_the_given_stream():
         for t in got:
             t.record_stream(torch.cuda.current_stream())
     c.check()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 20])
+def test_a_window_wider_than_any_sequence_is_none(window):
+    """Rows that lie before their sequence among them."""
+    for H, K, hd in ((4, 2, 64), (4, 1, 256)):
+        c, table, k, v, g = _filled(H, K, hd, [3, 20], 16, 8)
+        q = torch.randn(9 + 4, H, hd, generator=g).half().cuda()
+        cu, ln = _cu([9, 4]), _i32([3, 20])
+        got = c.attend_prompt(q, cu, ln, table, window=window)
+        assert torch.equal(got, c.attend_prompt(q, cu, ln, table))
+        want, mag, top = _ref_attention(q, k, v, [3, 20], [9, 4], 1 / math.sqrt(hd), 0)
+        _close(got, want, mag, top, 2.0 ** -11)
+        assert torch.equal(c.attend(q[:2], ln, table, window=window), c.attend(q[:2], ln, table))
+        c.check()
