@@ -22,7 +22,12 @@
 //             tensor memory once and writes P over them as the second
 //             product's operand.  The exponentials are taken against a
 //             reference maximum that is moved (and O and l rescaled) only
-//             where a score passes it by 2^8, and for the first tile
+//             where a score passes it by 2^7, and for the first tile.  P is
+//             rounded to 11 bits as the operand and kept times 2^8, so that
+//             it is a normal fp16 number down to 2^-22 of the reference and
+//             not lost above 2^-33; l sums the rounded P, so that the weights
+//             still add up to one (fresh prompts, below: 190.3 us, 189.4 with
+//             the unrounded sum)
 // A CTA holds 256 query rows (two tiles, whose products and softmaxes take
 // turns; the K and V tiles serve both) or, at head_dim 256, 128.  A query row
 // is a (token, head of the kv head's group) pair, so the group shares K and V.
@@ -45,7 +50,8 @@
 #include "ck_kv_attn.cuh"
 
 #define KVP_MAXS 1024        // sequences of one launch
-#define KVP_SLACK 8.f
+#define KVP_SLACK 7.f        // log2 that a score may exceed the reference maximum before O is rescaled
+#define KVP_BOOST 8.f        // p is kept times 2^8 (cancelled by l): at most 2^15 as an operand, and normal down to 2^-22
 
 template <int HD, int VB>
 struct KvPr {
@@ -93,6 +99,8 @@ __device__ __forceinline__ float kvp_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// a plus the fp16 number h, in 32 bits
+__device__ __forceinline__ void kvp_add16(float& a, unsigned short h) { asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(a) : "h"(h)); }
 // A value scale that is NaN, or so large that code * scale would pass fp16,
 // must not meet a masked p = 0 in the second product (0 * inf): its values
 // count as zero there, and the position's key becomes NaN, so that exactly the
@@ -621,9 +629,9 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           }
         }
       }
-      uint64_t sum2 = kv_two(0.f, 0.f), sum3 = sum2;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
       {
-        const float mb = m == -INFINITY ? 0.f : m;
+        const float mb = (m == -INFINITY ? 0.f : m) - KVP_BOOST;
         const uint64_t sc2 = kv_two(sc, sc), mb2 = kv_two(-mb, -mb);
         uint32_t y[32];
 #pragma unroll
@@ -632,18 +640,13 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           kv_split(kv_fma2(kv_two(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), sc2, mb2), p, q);
           p = kv_ex2(p);
           q = kv_ex2(q);
-          if (e & 2) sum3 = kv_add2(sum3, kv_two(p, q));
-          else sum2 = kv_add2(sum2, kv_two(p, q));
           y[e / 2] = kv_pack2(p, q);
+          kvp_add16(sum[(e / 2 & 1) * 2], (unsigned short)y[e / 2]);   // l sums what the product takes
+          kvp_add16(sum[(e / 2 & 1) * 2 + 1], (unsigned short)(y[e / 2] >> 16));
         }
         tmem_st32(tS, y);
       }
-      sum2 = kv_add2(sum2, sum3);
-      {
-        float s0, s1;
-        kv_split(sum2, s0, s1);
-        l += s0 + s1;
-      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
       mbar_arrive(&b_p[wq][buf]);

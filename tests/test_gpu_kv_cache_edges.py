@@ -58,3 +58,38 @@ def test_a_window_wider_than_any_sequence_is_none(window):
         _close(got, want, mag, top, 2.0 ** -11)
         assert torch.equal(c.attend(q[:2], ln, table, window=window), c.attend(q[:2], ln, table))
         c.check()
+
+
+@pytest.mark.parametrize("queries", [80, 1])
+@pytest.mark.parametrize("lowest", [60, 100])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_small_probabilities_beside_a_large_one(hd, lowest, queries):
+    """131072 positions some 20 to 26 octaves (lowest 100: 25 to 26) below the first one's, whose value is zero: the
+    output is what the small probabilities add up to.  Key codes, scales (2^-3) and q are chosen so that code * scale and
+    the scores are exact.  A probability is rounded to 11 bits, or to half a step of the smallest fp16 numbers: 2^-25,
+    kept times 2^8, of the reference maximum, which may lie 2^7 above the largest probability; so 2^-33 each, in the
+    outputs' sum and in the sum that divides it.  80 queries of one sequence are not split over its positions, 1 is."""
+    n, block = 131072, 128
+    g = torch.Generator().manual_seed(hd + lowest)
+    k = torch.zeros(n, 1, hd)
+    k[:, 0, 1::32] = 127 / 8                     # each group's largest value: scale 1 / 8, where q is zero
+    k[:, 0, 0] = -torch.randint(lowest, 108, (n,), generator=g) / 8
+    k[0, 0, 0] = 100 / 8
+    v = 0.5 + 0.5 * torch.rand(n, 1, hd, generator=g)
+    v[0] = 0
+    table, nb = _tables([n], block, g)
+    seq, pos = _tokens([n])
+    c = _cache(1, 1, hd, nb, block)
+    c.store(None, k.cuda(), v.cuda(), seq, pos, table)
+    kk, vv = c.load(seq, pos, table, dtype=F32)
+    assert torch.equal(kk.cpu(), k)
+    q = torch.zeros(queries, 1, hd, dtype=F16, device="cuda")
+    q[:, 0, 0] = 1
+    scale = float(np.float32(math.log(2)))       # a score is its exponent of two
+    want, mag, top = _ref_attention(q[:1], [kk], [vv], [n], [1], scale, 0)
+    table = table.expand(queries, -1).contiguous()
+    ln = _i32([n] * queries)
+    for got in (c.attend_prompt(q, _cu([1] * queries), ln, table, scale=scale), c.attend(q, ln, table, scale=scale)):
+        tol = (2 * 2.0 ** -11 + 2 * 2.0 ** -20 * top) * mag + 2 * n * 2.0 ** -33 * vv.abs().max().item() + EPS[F16] * want.abs()
+        assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() - tol).max()
+    c.check()
