@@ -378,8 +378,11 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : HD == 64 ? 24 
       int e = (int)(__float_as_uint(top) >> 23) - 127;
       e = e > 127 ? 8 : max(e, -100);
       const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-      // 2^24: the codes' fp16 numbers
-      const float scr = A.scale * 1.4426950408889634f * 16777216.f * __uint_as_float((uint32_t)(127 + e - 8) << 23);
+      // 2^24: the codes' fp16 numbers.  Above 2^100 the factor is cut: no sum
+      // that it multiplies passes 2^16, so that scores stay finite, and two
+      // that differ do so by 2^-72 at least, so that the softmax is the same
+      const float scr = fminf(fmaxf(A.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + e) << 23) * 65536.f,
+                                    -0x1p100f), 0x1p100f);
       sc[0] = __shfl_sync(0xffffffffu, scr, 8 * t);
       sc[1] = __shfl_sync(0xffffffffu, scr, 8 * t + 4);
 #pragma unroll

@@ -93,3 +93,41 @@ def test_many_small_probabilities_beside_a_large_one(hd, lowest, queries):
         tol = (2 * 2.0 ** -11 + 2 * 2.0 ** -20 * top) * mag + 2 * n * 2.0 ** -33 * vv.abs().max().item() + EPS[F16] * want.abs()
         assert ((got.double() - want).abs() <= tol).all(), ((got.double() - want).abs() - tol).max()
     c.check()
+
+
+def _far_apart(hd, gain):
+    """A cache of 200 positions and a bf16 query whose scores are so large, and so far from each other (2^-9 of the
+    magnitudes they sum, which 16-bit operands cannot turn round), that the softmax is one position's."""
+    n = 200
+    g = torch.Generator().manual_seed(hd)
+    table, nb = _tables([n], 16, g)
+    seq, pos = _tokens([n])
+    k, v = (torch.randn(n, 1, hd, generator=g).mul_(0.01).cuda() for _ in range(2))
+    c = _cache(2, 1, hd, nb, 16)
+    c.store(None, k, v, seq, pos, table)
+    kk, vv = c.load(seq, pos, table, dtype=F32)
+    q = (torch.randn(1, 2, hd, generator=g) * gain).to(BF16).cuda()
+    s = torch.einsum("nhd,pkd->hp", q.double(), kk.double())
+    first, second = s.topk(2).values.unbind(1)
+    size = torch.einsum("nhd,pkd->hp", q.double().abs(), kk.double().abs()).amax(1)
+    assert ((first - second) > 2.0 ** -9 * size).all() and ((first - second) * 0.05 > 64).all()
+    return c, table, q, _i32([n]), vv[s.argmax(1), 0].double()[None]
+
+
+def _one_value(got, want):
+    """A value rounded to 11 bits as an operand, then to the output's type."""
+    assert ((got.double() - want).abs() <= (EPS[BF16] + 2.0 ** -10) * want.abs() + 1e-6).all()
+
+
+GAINS = [2.0 ** 24, 2.0 ** 40, 2.0 ** 100, 2.0 ** 114, 2.0 ** 124]
+
+
+@pytest.mark.parametrize("gain", GAINS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_very_large_queries_of_one_token(hd, gain):
+    c, table, q, ln, want = _far_apart(hd, gain)
+    _one_value(c.attend(q, ln, table, scale=0.05), want)
+    wide = torch.zeros(1, 40000, dtype=torch.int32, device="cuda")       # by list
+    wide[:, : table.shape[1]] = table
+    _one_value(c.attend(q, ln, wide, scale=0.05), want)
+    c.check()
