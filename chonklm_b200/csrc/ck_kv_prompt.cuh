@@ -47,6 +47,8 @@
 // then split over several CTAs, which leave unnormalised partial rows for
 // k_kv_prompt_join.
 #pragma once
+#include <float.h>
+
 #include "ck_kv_attn.cuh"
 
 #define KVP_MAXS 1024        // sequences of one launch
@@ -335,8 +337,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
           for (int p = 0; p < 4; p++)
             *place(row, p) = make_uint4(u[p][0] ^ flip, u[p][1] ^ flip, u[p][2] ^ flip, u[p][3] ^ flip);
       }
-      // (a scale of 0 counts as one too small to show: masked scores are -inf times it)
-      if (x == 0 && row < ROWS) s_scale[row] = fmaxf(back, 1e-37f);
+      // (a scale of 0 counts as one too small to show: masked scores are -inf
+      // times it; and past 2^100 no softmax changes: scores that differ do so
+      // by 2^-48 at least, the smallest product of two fp16 numbers)
+      if (x == 0 && row < ROWS) s_scale[row] = fminf(fmaxf(back, 1e-37f), 0x1p100f);
     }
     proxy_fence_smem();
     mbar_arrive(&b_q);
@@ -569,10 +573,17 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     const float sc = s_scale[rr];
     const int rpos = pos0 + rtok;                                 // position of the row's token
     const int rlo = kvp_low(rpos, A.window);
-    float m = -INFINITY, l = 0.f;
+    // The reference before (raw) and after the factor sc (m), and less the
+    // boost (mb).  wide: some lane's is so large that 32 bits round it to 2^-4
+    // of an octave or worse, past 2^28 to whole ones, by which all of the row's
+    // p would be off.  Such a tile's scores have the reference taken off in
+    // tensor memory and are read again (less) for the exponentials: a branch
+    // around the other path's registers cost all prompts 2.5 %.
+    float raw = -INFINITY, m = -INFINITY, mb = -KVP_BOOST, l = 0.f;
+    bool wide = false, less = false;
     const uint32_t tO = tmem + C::TO + wq * HD + lanes;
     bool ok = true;
-    for (int j = beg[wq]; ok && j < end[wq]; j++) {
+    for (int j = beg[wq]; ok && j < end[wq];) {
       const int it = j - jb, buf = it & 1;
       // uses of this buffer by this query tile before: its tiles of the same parity
       const int use = (it >> 1) - ((beg[wq] - jb + 1 - buf) >> 1);
@@ -609,11 +620,14 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
         my = kvp_max3(my, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
       }
       mx = fmaxf(mx, my);
-      mx = mx == -INFINITY ? mx : mx * sc;
-      if (__any_sync(0xffffffffu, mx > m + KVP_SLACK)) {          // move the reference
-        const float mn = fmaxf(m, mx), a = m == -INFINITY ? 0.f : kv_ex2(m - mn);
-        m = mn;
+      const float ms = mx == -INFINITY ? mx : mx * sc;
+      if (!less && __any_sync(0xffffffffu, wide || ms > m + KVP_SLACK)) {   // move the reference
+        const float rn = fmaxf(raw, mx), a = raw == -INFINITY ? 0.f : kv_ex2((raw - rn) * sc);
+        raw = rn;
+        m = rn == -INFINITY ? rn : rn * sc;
         l *= a;
+        mb = (m == -INFINITY ? 0.f : m) - KVP_BOOST;
+        wide = __any_sync(0xffffffffu, fabsf(mb) >= 0x1p20f);
         if (j > beg[wq]) {
           ok = kvp_wait(&b_pv[(it - 1) & 1], ((it - 1) >> 1) & 1, &s_fail, A.pool.err);   // O holds the tiles before
           if (!ok) break;
@@ -628,10 +642,24 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
             tmem_st32(tO + d, y);
           }
         }
+        if (wide) {
+#pragma unroll 1
+          for (int d = 0; d < C::PT; d += 32) {
+            uint32_t y[32];
+            tmem_ld32_nowait(tS + d, y);
+            tmem_ld_wait(y);
+#pragma unroll
+            for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) - (raw == -INFINITY ? 0.f : raw));
+            tmem_st32(tS + d, y);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          mb = -KVP_BOOST;
+          less = true;
+          continue;
+        }
       }
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
       {
-        const float mb = (m == -INFINITY ? 0.f : m) - KVP_BOOST;
         const uint64_t sc2 = kv_two(sc, sc), mb2 = kv_two(-mb, -mb);
         uint32_t y[32];
 #pragma unroll
@@ -650,6 +678,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       asm volatile("tcgen05.fence::before_thread_sync;");
       mbar_arrive(&b_p[wq][buf]);
+      less = false;
+      j++;
     }
     // O / l, or this CTA's part of it
     if (ok && beg[wq] < end[wq]) ok = kvp_wait(&b_o, 0, &s_fail, A.pool.err);
@@ -686,7 +716,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       }
       if (splits > 1)
         ((float2*)((long long*)A.ml + KV_PRE))[((size_t)(b * units + unit) * splits + z) * (128 * C::NQ) + rr] =
-            make_float2(m, l);
+            make_float2(raw == -INFINITY ? raw : fminf(fmaxf(m, -FLT_MAX), FLT_MAX), l);
     }
   }
   // no CTA leaves with a copy in flight (any role may have given up, after the

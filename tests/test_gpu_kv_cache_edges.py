@@ -131,3 +131,38 @@ def test_very_large_queries_of_one_token(hd, gain):
     wide[:, : table.shape[1]] = table
     _one_value(c.attend(q, ln, wide, scale=0.05), want)
     c.check()
+
+
+@pytest.mark.parametrize("gain", GAINS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_very_large_queries_in_prompts(hd, gain):
+    """With a row that lies before the sequence beside the live one, and with the positions split over CTAs (a table wide
+    enough for it)."""
+    c, table, q, ln, want = _far_apart(hd, gain)
+    _one_value(c.attend_prompt(q, _i32([0, 1]), ln, table, scale=0.05), want)
+    wide = torch.zeros(1, 40000, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    _one_value(c.attend_prompt(q, _i32([0, 1]), ln, wide, scale=0.05), want)
+    many = q.expand(201, -1, -1).contiguous()
+    got = c.attend_prompt(many, _i32([0, 201]), ln, table, scale=0.05)
+    assert not got[0].any()
+    _one_value(got[-1:], want)
+    assert torch.isfinite(got).all()
+    c.check()
+
+
+@pytest.mark.parametrize("gain", [2.0 ** 10, 2.0 ** 20] + GAINS)
+def test_equal_scores_of_any_size_weigh_alike(gain):
+    n, hd = 300, 128
+    g = torch.Generator().manual_seed(1)
+    table, nb = _tables([n], 16, g)
+    seq, pos = _tokens([n])
+    k, v = torch.randn(1, 1, hd, generator=g).expand(n, -1, -1).cuda(), torch.randn(n, 1, hd, generator=g).cuda()
+    c = _cache(2, 1, hd, nb, 16)
+    c.store(None, k, v, seq, pos, table)
+    _, vv = c.load(seq, pos, table, dtype=F32)
+    q = (torch.randn(1, 2, hd, generator=g) * gain).to(BF16).cuda()
+    want, mag = vv.double().mean(0, keepdim=True), vv.double().abs().mean(0, keepdim=True)
+    for got in (c.attend(q, _i32([n]), table), c.attend_prompt(q, _i32([0, 1]), _i32([n]), table)):
+        assert ((got.double() - want).abs() <= 2.0 ** -10 * mag + EPS[BF16] * want.abs() + 1e-6).all()
+    c.check()
