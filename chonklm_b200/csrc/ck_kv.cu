@@ -244,11 +244,12 @@ cudaError_t kv_prompt_launch(const KvAttn& all, int sms, cudaStream_t s) {
     if (splits < 1) splits = 1;
     if (ctas * splits > 0x7fffffffLL) return cudaErrorInvalidValue;
     const dim3 grid((unsigned)(ctas * splits));
+    const int ends = (i0 == 0 ? 1 : 0) | (i0 + a.n == all.n ? 2 : 0);
     cudaError_t e = cudaErrorInvalidValue;
 #define KV_CASE(HD, VB)                                                                                            \
   if (a.pool.hd == HD && a.pool.vbits == VB)                                                                       \
     e = kv_launch(k_kv_prompt<HD, VB>, grid, dim3(KvPr<HD, VB>::THREADS), KvPr<HD, VB>::SMEM, s, false, a, units, gs, \
-                  (int)splits);
+                  (int)splits, ends);
     KV_EACH(KV_CASE)
 #undef KV_CASE
     if (e != cudaSuccess) return e;
@@ -544,9 +545,10 @@ int ck_kv_check(ck_kv* h, void* stream) {
   if (!bits) return CK_OK;
   KVC(cudaMemsetAsync(h->pool.err, 0, sizeof bits, s));
   KVC(cudaStreamSynchronize(s));
-  return h->fail(CK_EDEVICE, "%s%s%s%s", bits & KV_ERR_SEQ ? "sequence outside the block table; " : "",
+  return h->fail(CK_EDEVICE, "%s%s%s%s%s", bits & KV_ERR_SEQ ? "sequence outside the block table; " : "",
                  bits & KV_ERR_POS ? "position or length outside the block table; " : "",
                  bits & KV_ERR_BLOCK ? "block table entry outside the pool; " : "",
+                 bits & KV_ERR_ROWS ? "prompt's sequence outside the query rows; " : "",
                  bits & KV_ERR_WAIT ? "device wait timed out; " : "");
 }
 

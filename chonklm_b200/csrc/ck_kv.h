@@ -9,6 +9,7 @@
 #define KV_ERR_POS 2       // position or length outside the block table
 #define KV_ERR_BLOCK 4     // block table entry outside the pool
 #define KV_ERR_WAIT 8      // a device wait gave up
+#define KV_ERR_ROWS 16     // prompt: a sequence's rows leave the query rows, or go back
 
 enum { KV_F32 = 0, KV_F16 = 1, KV_BF16 = 2 };
 

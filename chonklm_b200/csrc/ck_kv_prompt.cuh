@@ -138,14 +138,64 @@ __device__ __forceinline__ bool kvp_wait(uint64_t* bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, ok);
 }
 
+// Whether a sequence's rows lie among the query rows.
+__device__ __forceinline__ bool kvp_rows_ok(const KvAttn& A, int c0, int c1) { return c0 >= 0 && c0 <= c1 && c1 <= A.rows; }
+
+// One warp: the rows that lie in no sequence, [0] .. [1] and [2] .. [3] of
+// gaps; whether the row list goes back.  Out of line, as is kvp_zero_rows: a
+// CTA's start is bound by fetching code, and with these two in its path fresh
+// prompts took 193.0 us for 191.1 (190.4 without looking for such rows).
+__device__ __noinline__ bool kvp_gaps(const KvAttn& A, int ends, int* gaps) {
+  const int lane = threadIdx.x & 31;
+  bool bad = false, back = false;
+  int v0 = 0x7fffffff, v1 = -1;                // rows of the sequences that are not refused
+  for (int s = lane; s < A.n; s += 32) {
+    const int x = A.cu[s], y = A.cu[s + 1];
+    back = back || y < x;
+    if (kvp_rows_ok(A, x, y)) { v0 = min(v0, x); v1 = max(v1, y); }
+    else bad = true;
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  back = __any_sync(0xffffffffu, back);
+  v0 = __reduce_min_sync(0xffffffffu, v0);
+  v1 = __reduce_max_sync(0xffffffffu, v1);
+  const int r0 = ends & 1 ? 0 : min(max(A.cu[0], 0), A.rows), r1 = ends & 2 ? A.rows : min(max(A.cu[A.n], 0), A.rows);
+  if (back || v0 > v1) v0 = v1 = r1;
+  if (lane == 0) {
+    gaps[0] = r0;
+    gaps[1] = max(v0, r0);
+    gaps[2] = v1;
+    gaps[3] = max(r1, v1);
+    if (bad && blockIdx.x == 0) atomicOr(A.pool.err, KV_ERR_ROWS);
+  }
+  return back;
+}
+// All CTAs, a row in turn.
+__device__ __noinline__ void kvp_zero_rows(const KvAttn& A, int hd, const int* gaps) {
+  const int before = gaps[1] - gaps[0], n = before + gaps[3] - gaps[2], pieces = hd / 8;
+  const uint32_t zero[4] = {0u, 0u, 0u, 0u};
+  const bool vec = kv_vec8(A.o);
+  for (int r = blockIdx.x; r < n; r += gridDim.x) {
+    const size_t row = r < before ? gaps[0] + r : gaps[2] + (r - before);
+    for (int e = threadIdx.x; e < A.heads * pieces; e += blockDim.x)
+      kv_put8(A.o.p, row * A.o.st + (size_t)(e / pieces) * A.o.sh + 8 * (e % pieces), zero, vec);
+  }
+}
+
+// ends: 1, this launch has the call's first sequences; 2, its last.  Query rows
+// that lie in no sequence are written as zeros:
+// those before the first and after the last one, and those of a sequence that
+// is refused because it leaves the rows; a row list that goes back is refused
+// as a whole.
 template <int HD, int VB>
-__global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A, int units, int gs, int splits) {
+__global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __grid_constant__ KvAttn A, int units, int gs, int splits, int ends) {
   using C = KvPr<HD, VB>;
   using R = KvRec<HD, VB>;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ uint32_t s_tmem;
   __shared__ volatile int s_fail;
   __shared__ int s_seq, s_tile, s_cu0, s_cu1, s_len;
+  __shared__ int s_gap, s_gaps[4];             // whether rows lie in no sequence: [0] .. [1] and [2] .. [3]
   __shared__ float s_scale[128 * C::NQ];       // factor of each query row's scores
   __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_v[C::BUF], b_kf[2],
       b_s[C::NQ][2], b_p[C::NQ][2], b_pv[2], b_o, b_end;
@@ -156,7 +206,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
 
   if (warp == 0) {
     // tile b, deepest first: D with f(D + 1) <= b < f(D), f(D) = tiles at depth >= D
-    auto depth = [&](int c0, int c1) { return c1 > c0 ? (c1 - c0 + bt - 1) / bt : 0; };
+    auto depth = [&](int c0, int c1) { return kvp_rows_ok(A, c0, c1) ? (c1 - c0 + bt - 1) / bt : 0; };
+    auto odd = [&](int s, int c0, int c1) {    // refused, or rows beside it
+      return !kvp_rows_ok(A, c0, c1) || (s == 0 && (ends & 1) && c0 != 0) || (s == A.n - 1 && (ends & 2) && c1 != A.rows);
+    };
     // up to 32 sequences' rows stay in registers
     const bool in = lane < A.n;
     const int c0 = in ? A.cu[lane] : 0, c1 = in ? A.cu[lane + 1] : 0, ln = in ? A.len[lane] : 0;
@@ -167,9 +220,17 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       return __reduce_add_sync(0xffffffffu, c);
     };
     int lo = 0, seq = -1, most = mine;         // f(lo) > b >= f(hi)
-    for (int s = lane + 32; s < A.n; s += 32) most = max(most, depth(A.cu[s], A.cu[s + 1]));
+    bool gap = in && odd(lane, c0, c1), back = false;
+    for (int s = lane + 32; s < A.n; s += 32) {
+      most = max(most, depth(A.cu[s], A.cu[s + 1]));
+      gap = gap || odd(s, A.cu[s], A.cu[s + 1]);
+    }
     int hi = __reduce_max_sync(0xffffffffu, most);
-    if (above(0) > b) {
+    gap = __any_sync(0xffffffffu, gap);
+    if (gap) {
+      back = kvp_gaps(A, ends, s_gaps);
+    }
+    if (!back && above(0) > b) {
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (above(mid) > b) lo = mid; else hi = mid;
@@ -189,6 +250,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
       s_cu0 = seq >= 32 ? A.cu[seq] : c0;
       s_cu1 = seq >= 32 ? A.cu[seq + 1] : c1;
       s_len = seq >= 32 ? A.len[seq] : ln;
+      s_gap = gap;
       s_fail = 0;
     }
   } else if (warp == 1 && lane == 0) {
@@ -219,6 +281,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;");
+  if (s_gap) kvp_zero_rows(A, HD, s_gaps);
   const int seq = s_seq;
   int4* desc = (int4*)A.ml + b * units + unit;      // splits: what k_kv_prompt_join joins
   if (seq < 0) {
@@ -227,10 +290,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(KvAttn A
     return;
   }
   const int n_new = s_cu1 - s_cu0, q0 = s_cu0 + s_tile * bt;
-  int ntok = min(bt, s_cu1 - q0), len = max(s_len, 0);
-  if (s_cu0 < 0 || s_cu1 > A.rows || len > A.tab.max_blocks * A.pool.block) {
+  const int ntok = min(bt, s_cu1 - q0);
+  int len = max(s_len, 0);
+  if (len > A.tab.max_blocks * A.pool.block) {
     if (tid == 0) atomicOr(A.pool.err, KV_ERR_POS);
-    if (s_cu0 < 0 || s_cu1 > A.rows) ntok = 0;
     len = 0;
   }
   const int pos0 = len - n_new + s_tile * bt;  // cached position of the CTA's first token (may be negative)

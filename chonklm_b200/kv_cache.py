@@ -16,8 +16,8 @@ without waiting; calls on one cache have to be ordered among themselves.  An
 output that a call makes itself is memory of the stream that the call runs on.
 A tensor that is used on another stream than its own is the caller's to keep
 alive (`Tensor.record_stream`).  A wrong argument raises ValueError or
-CkError; what only the device can see (a sequence, position or block out of
-range) is skipped there and raised by `check()`.  There is no CPU fallback.
+CkError; what only the device can see (a sequence, position, block or row out
+of range) is skipped there and raised by `check()`.  There is no CPU fallback.
 """
 from __future__ import annotations
 
@@ -157,7 +157,7 @@ class QuantKvCache:
     def attend_prompt(self, q, cu, length, table, scale: Optional[float] = None, window: int = 0, out=None,
                       stream: Optional[int] = None):
         """Causal attention of several new tokens per sequence: rows cu[i] .. cu[i + 1] of q are the last tokens of
-        sequence i's length[i] cached positions (row i of the table)."""
+        sequence i's length[i] cached positions (row i of the table).  Rows of no sequence are zero."""
         n = q.shape[0]
         if out is None:
             out = self._make(stream, torch.empty_like, q)
@@ -172,7 +172,7 @@ class QuantKvCache:
         return out
 
     def check(self, stream: Optional[int] = None) -> None:
-        """Wait for the stream; raise if a kernel met a sequence, position or block out of range."""
+        """Wait for the stream; raise if a kernel met a sequence, position, block or row out of range."""
         self._check(self._L.ck_kv_check(self.h, self._stream(stream)))
 
     @property

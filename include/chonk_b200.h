@@ -263,7 +263,7 @@ int ck_batch_destroy(ck_batch* b);
  * so they may be captured into a CUDA graph.  All pointers in their arguments
  * are device pointers, read when the kernels run; calls on one handle have to
  * be ordered on one stream or by events (ck_kv_attend shares the handle's
- * workspace).  What only the device can see (a sequence, position or block
+ * workspace).  What only the device can see (a sequence, position, block or row
  * out of range) is skipped there and reported by ck_kv_check. */
 typedef struct ck_kv ck_kv;
 
@@ -342,7 +342,10 @@ int ck_kv_load(ck_kv* h, const ck_kv_load_args* a, void* stream);
 int ck_kv_attend(ck_kv* h, const ck_kv_attend_args* a, void* stream);
 /* Several new tokens per sequence: rows cu[i] .. cu[i + 1] of q ([rows] in
  * all) are the last tokens of sequence i's len[i] cached positions, each
- * seeing the positions up to its own. */
+ * seeing the positions up to its own.  Rows of no sequence (before cu[0], from
+ * cu[n] on) are zero.  A sequence whose rows leave [0, rows] is skipped, and a
+ * cu that goes back is refused, 1024 sequences at a time: ck_kv_check reports
+ * both, and their rows are zero. */
 int ck_kv_attend_prompt(ck_kv* h, const ck_kv_attend_args* a, const int32_t* cu, int rows, void* stream);
 /* Waits for `stream`; CK_EDEVICE when a kernel since the last check met a
  * sequence, position or block out of range. */

@@ -166,3 +166,62 @@ def test_equal_scores_of_any_size_weigh_alike(gain):
     for got in (c.attend(q, _i32([n]), table), c.attend_prompt(q, _i32([0, 1]), _i32([n]), table)):
         assert ((got.double() - want).abs() <= 2.0 ** -10 * mag + EPS[BF16] * want.abs() + 1e-6).all()
     c.check()
+
+
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+@pytest.mark.parametrize("long", [False, True])
+def test_prompt_rows_of_no_sequence_are_zero(layout, long):
+    """Rows before the first and after the last sequence's, without (short) and with a split of the positions."""
+    H, K, hd = layout
+    lens = [2000, 1030] if long else [20, 30]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=3)
+    q = torch.randn(400, H, hd, generator=g).half().cuda()
+    fill = lambda: torch.full_like(q, 7.0)
+    for cu in ([3, 20, 33], [0, 17, 30], [370, 387, 400], [0, 0, 400], [399, 399, 400], [0, 0, 0], [5, 5, 5], [400, 400, 400]):
+        a, b = cu[0], cu[-1]
+        got = c.attend_prompt(q, _i32(cu), _i32(lens), table, out=fill())
+        assert not got[:a].any() and not got[b:].any()
+        want, mag, top = _ref_attention(q[a:b], k, v, lens, [cu[1] - a, b - cu[1]], 1 / math.sqrt(hd), 0) if b > a else (None,) * 3
+        if b > a:
+            _close(got[a:b], want, mag, top, 2.0 ** -11)
+    c.check()
+
+
+def test_prompt_rows_of_refused_sequences_are_zero():
+    """Row lists that leave the rows or go back: what they name is zero and reported, the other sequences are right."""
+    from chonklm_b200 import _lib
+    lens = [20, 30, 25]
+    c, table, k, v, g = _filled(4, 2, 64, lens, 16, 8)
+    q = torch.randn(40, 4, 64, generator=g).half().cuda()
+    big = 2 ** 31 - 1
+    for cu, live in [([0, 10, 30, 41], (0, 30)), ([-1, 10, 30, 40], (10, 40)), ([-big - 1, 10, 30, 40], (10, 40)), ([0, 10, 30, big], (0, 30)),
+                     ([41, 42, 43, 44], (0, 0)), ([-5, -4, -3, -2], (0, 0)), ([-5, 50, 60, 70], (0, 0)), ([0, 30, 10, 40], (0, 0)),
+                     ([big, 0, 0, 0], (0, 0)), ([0, big, -big, 40], (0, 0))]:
+        got = c.attend_prompt(q, _i32(cu), _i32(lens), table, out=torch.full_like(q, 7.0))
+        with pytest.raises(_lib.CkError, match="rows"):
+            c.check()
+        a, b = live
+        assert not got[:a].any() and not got[b:].any(), cu
+        at = a
+        for i in range(3):
+            if at == cu[i] and at < cu[i + 1] <= b:
+                want, mag, top = _ref_attention(q[at: cu[i + 1]], k[i: i + 1], v[i: i + 1], lens[i: i + 1], [cu[i + 1] - at], 0.125, 0)
+                _close(got[at: cu[i + 1]], want, mag, top, 2.0 ** -11)
+                at = cu[i + 1]
+        assert at == b
+    c.attend_prompt(q, _i32([0, 10, 30, 40]), _i32(lens), table)
+    c.check()
+
+
+def test_prompt_rows_of_no_sequence_in_several_launches():
+    H, K, hd, S = 4, 2, 64, 1100
+    lens, news = [1 + i % 37 for i in range(S)], [1 + i % 3 for i in range(S)]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=12)
+    n = sum(news)
+    q = torch.randn(n, H, hd, generator=g).half().cuda()
+    want = c.attend_prompt(q, _cu(news), _i32(lens), table)
+    wide = torch.zeros(n + 12, H, hd, dtype=F16, device="cuda")
+    wide[5: n + 5] = q
+    got = c.attend_prompt(wide, _cu(news) + 5, _i32(lens), table, out=torch.full_like(wide, 7.0))
+    c.check()
+    assert torch.equal(got[5: n + 5], want) and not got[:5].any() and not got[n + 5:].any()
