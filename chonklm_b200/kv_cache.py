@@ -16,8 +16,10 @@ without waiting; calls on one cache have to be ordered among themselves.  An
 output that a call makes itself is memory of the stream that the call runs on.
 A tensor that is used on another stream than its own is the caller's to keep
 alive (`Tensor.record_stream`).  A wrong argument raises ValueError or
-CkError; what only the device can see (a sequence, position, block or row out
-of range) is skipped there and raised by `check()`.  There is no CPU fallback.
+CkError, and so does a tensor that requires a gradient while gradients are
+recorded (there is no backward); what only the device can see (a sequence,
+position, block or row out of range) is skipped there and raised by `check()`.
+There is no CPU fallback.
 """
 from __future__ import annotations
 
@@ -73,6 +75,8 @@ class QuantKvCache:
         st, sh, sd = t.stride()
         if sd != 1:
             raise ValueError(f"{name}: the elements of a head are not contiguous")
+        if t.requires_grad:
+            self._no_grad(name)
         return t.data_ptr(), st, sh, dt, 0
 
     def _ints(self, name: str, t, n: int) -> int:
@@ -90,7 +94,15 @@ class QuantKvCache:
             return 0
         if t.dtype is not torch.float32 or t.shape != (n,) or t.get_device() != self.device or not t.is_contiguous():
             raise ValueError(f"{name}: expected a contiguous float32 vector of {n} on {self._dev}")
+        if t.requires_grad:
+            self._no_grad(name)
         return t.data_ptr()
+
+    @staticmethod
+    def _no_grad(name: str) -> None:
+        if torch.is_grad_enabled():
+            raise ValueError(f"{name} requires a gradient, and the cache's operators have none: call them under "
+                             "torch.no_grad() or on detached tensors")
 
     def _stream(self, stream: Optional[int]) -> int:
         return _raw_stream(self.device) if stream is None else stream

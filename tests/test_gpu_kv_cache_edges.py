@@ -225,3 +225,23 @@ def test_prompt_rows_of_no_sequence_in_several_launches():
     got = c.attend_prompt(wide, _cu(news) + 5, _i32(lens), table, out=torch.full_like(wide, 7.0))
     c.check()
     assert torch.equal(got[5: n + 5], want) and not got[:5].any() and not got[n + 5:].any()
+
+
+def test_refuses_to_drop_a_gradient():
+    """There is no backward: a tensor that asks for one is refused while gradients are recorded, taken otherwise."""
+    c, table, k, v, g = _filled(4, 2, 64, [5], 16, 8)
+    seq, pos = _tokens([1])
+    q, kn = torch.randn(1, 4, 64).half().cuda(), torch.randn(1, 2, 64).half().cuda()
+    w = torch.ones(64, device="cuda")
+    asks = lambda t: t.clone().requires_grad_()
+    calls = [lambda f: c.store(f(q), kn, kn, seq, pos, table), lambda f: c.store(q, f(kn), kn, seq, pos, table),
+             lambda f: c.store(q, kn, f(kn), seq, pos, table), lambda f: c.store(q, kn, kn, seq, pos, table, q_norm=f(w)),
+             lambda f: c.store(q, kn, kn, seq, pos, table, k_norm=f(w)), lambda f: c.attend(f(q), _i32([5]), table),
+             lambda f: c.attend_prompt(f(q), _i32([0, 1]), _i32([5]), table)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call(asks)
+        want = call(lambda t: t)
+        with torch.no_grad():
+            assert torch.equal(call(asks), want)
+    c.check()
