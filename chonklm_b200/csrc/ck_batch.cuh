@@ -1561,7 +1561,8 @@ int ck_batch_stats(ck_batch* b, uint64_t* steps, uint64_t* tokens_fed, uint64_t*
 }
 
 // Cached keys and values of a running sequence in one layer, as the quantised
-// pages hold them.
+// pages hold them.  A sequence with positions has its device table's row from
+// the step that fed the first of them; one added since has none to read.
 int ck_batch_read_kv(ck_batch* b, int seq_id, int layer, float* k, float* v, int cap, int* n_out) {
   if (!b || !n_out || cap < 0 || (cap > 0 && (!k || !v))) return set_global(CK_EINVAL, "ck_batch_read_kv: bad argument");
   const ck_model_cfg& c = b->h->cfg;
@@ -1574,7 +1575,6 @@ int ck_batch_read_kv(ck_batch* b, int seq_id, int layer, float* k, float* v, int
   *n_out = b->seqs[slot].pos;
   const int n = *n_out < cap ? *n_out : cap;
   if (n == 0) return CK_OK;
-  if (b->btab_dirty) return b->fail(CK_ESTATE, "ck_batch_read_kv: no step since the last change of the block tables");
   CKB(b, cudaSetDevice(b->h->device));
   const size_t rows = (size_t)n * c.kv_heads * c.head_dim * 4;
   std::vector<int> at(2 * (size_t)n, slot);

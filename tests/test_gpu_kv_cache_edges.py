@@ -245,3 +245,24 @@ def test_refuses_to_drop_a_gradient():
         with torch.no_grad():
             assert torch.equal(call(asks), want)
     c.check()
+
+
+def test_read_kv_right_after_a_new_sequence(tiny_dir):
+    """A running sequence's pages can be read whatever was added since the last step."""
+    from chonklm_b200 import _lib
+    from test_gpu_batch import _engine
+    loaded, V = _engine(tiny_model(tiny_dir, "llama", "q4_k_m"))
+    batch = _lib.Batch(loaded.engine.dev, max_seqs=3, kv="q8")
+    first = batch.add([5, 6, 7, 8], 40)
+    for _ in range(20):
+        batch.step()
+    want = batch.read_kv(first, 1)
+    new = batch.add([9, 10], 30)
+    got = batch.read_kv(first, 1)
+    assert got[0].shape[0] == 20 and all(np.array_equal(a, b) for a, b in zip(got, want))
+    assert batch.read_kv(new, 0)[0].shape[0] == 0
+    batch.step()
+    assert batch.read_kv(first, 1)[0].shape[0] == 21 and batch.read_kv(new, 0)[0].shape[0] == 1
+    assert np.array_equal(batch.read_kv(first, 1)[0][:20], want[0])
+    batch.close()
+    loaded.engine.dispose()
