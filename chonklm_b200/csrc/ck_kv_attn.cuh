@@ -300,8 +300,10 @@ __global__ void __launch_bounds__(W * 32, UNIT ? (HD == 256 ? 8 : HD == 64 ? 24 
       ids_at = f.pair;
       const int seq = A.seq ? A.seq[f.q] : f.q, rec = 2 * f.pair + lane;
       ids = rec < A.tab.max_blocks << lb ? A.tab.dev[(size_t)seq * A.tab.max_blocks + (rec >> lb)] : -1;
-      // the second record of the last pair may lie past the end: not read, masked like any place past the end
-      if (rec * KV_TILE >= kv_len(A, f.q)) ids = -2;
+      // the second record of the last pair may lie past the end, the first of the first one before the window (and its
+      // block be another's by now): not read, masked like any place that is not seen
+      const int len = kv_len(A, f.q);
+      if (rec * KV_TILE >= len || (A.window > 0 && (rec + 1) * KV_TILE <= len - A.window)) ids = -2;
     }
     // lane 0 copies the first record, lane 1 the second
     const int id = __shfl_sync(0xffffffffu, ids, 2 * (f.pair - ids_at) + (lane & 1));

@@ -412,11 +412,12 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
   int issued = 0;                              // tiles whose copies are on their way or have landed (copy warp)
   if (warp == C::W_COPY) {
     // ---- copies: lane i fetches record i of the tile ----
+    const int lowest = kvp_low(pos0, A.window);   // no row sees a position before it: its block may be another's by now
     for (int j = jb; j < je; j++, issued++) {
       const int it = j - jb, s = it % C::STAGES;
       if (it >= C::STAGES && !kvp_wait(&b_empty[s], (it / C::STAGES - 1) & 1, &s_fail, A.pool.err)) break;
       const int tile = j * C::RECS + lane;     // record of the sequence
-      bool ok = lane < C::RECS && tile * KV_TILE < len;
+      bool ok = lane < C::RECS && tile * KV_TILE < len && (tile + 1) * KV_TILE > lowest;
       int id = 0;
       if (ok) {
         id = A.tab.dev[(size_t)seq * A.tab.max_blocks + tile / bpt];
@@ -425,8 +426,8 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
       }
       const uint32_t have = __ballot_sync(0xffffffffu, ok);
       uint8_t* dst = sm + C::SST + s * C::STAGE_BYTES + lane * R::BYTES;
-      // a record that does not exist: zero scales (its values meet p = 0) and
-      // a mark for the softmax
+      // a record that does not exist or is not seen: zero scales (its values
+      // meet p = 0) and a mark for the softmax
       if (lane < C::RECS && !ok) {
         for (int i = R::KS; i < R::BYTES; i += 4) *(uint32_t*)(dst + i) = 0u;
         proxy_fence_smem();

@@ -256,7 +256,9 @@ int ck_batch_destroy(ck_batch* b);
  * layer's pages: keys in 8 bits, values in 8 or 4, an fp16 scale for each 32
  * values of a head.  Sequences own blocks of `block` positions through a
  * block table in device memory ([n_seqs][max_blocks] int32) that the caller
- * keeps; entries past a sequence's last block are not read.
+ * keeps; what entries past a sequence's last block hold does not matter, nor,
+ * for attention with a window, those of blocks that end before the window of
+ * every query row.
  *
  * The four calls that work on the cache only enqueue their kernels on
  * `stream` (a cudaStream_t; NULL = the default stream) and allocate nothing,

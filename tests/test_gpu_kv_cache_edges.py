@@ -266,3 +266,33 @@ def test_read_kv_right_after_a_new_sequence(tiny_dir):
     assert np.array_equal(batch.read_kv(first, 1)[0][:20], want[0])
     batch.close()
     loaded.engine.dispose()
+
+
+@pytest.mark.parametrize("block", [16, 32])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+def test_blocks_before_the_window_may_be_gone(layout, block):
+    """A server with a sliding window hands blocks that no query sees any more to others and clears their entries, those
+    that end inside a tile which the window reaches among them."""
+    H, K, hd = layout
+    lens, news, window = [318, 95, 530], [1, 40, 5], 40
+    c, table, k, v, g = _filled(H, K, hd, lens, block, 8, seed=8)
+    q = torch.randn(sum(news), H, hd, generator=g).half().cuda()
+    ln, cu, last = _i32(lens), _cu(news), q[[0, 40, 45]].contiguous()
+
+    def gone(back, blocks):                      # entries of blocks that end before the first position seen
+        t = torch.full((3, blocks), -7, dtype=torch.int32, device="cuda")
+        t[:, : table.shape[1]] = table
+        for i, n in enumerate(lens):
+            t[i, : max(0, n - back[i] + 1 - window) // block] = -7
+        return t
+
+    want, one = c.attend_prompt(q, cu, ln, table, window=window), c.attend(last, ln, table, window=window)
+    c.check()
+    for blocks in (table.shape[1], 40000):       # short tables, and wide ones
+        got = c.attend(last, ln, gone([1, 1, 1], blocks), window=window)
+        c.check()
+        assert torch.equal(got, one)
+        got = c.attend_prompt(q, cu, ln, gone(news, blocks), window=window)
+        c.check()
+        _close(got, *_ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), window), 2.0 ** -11)
+        assert blocks > 1000 or torch.equal(got, want)
