@@ -107,13 +107,14 @@ class QuantKvCache:
     def _stream(self, stream: Optional[int]) -> int:
         return _raw_stream(self.device) if stream is None else stream
 
-    def _make(self, stream: Optional[int], empty, *args, **kw):
+    def _make(self, stream: int, empty, *args, **kw):
         """An output in memory of the stream that writes it: what is still pending elsewhere does not write there."""
-        if stream is None or stream == _raw_stream(self.device):
-            return empty(*args, **kw)
         s = torch.cuda.ExternalStream(stream, self._dev) if stream else torch.cuda.default_stream(self._dev)
         with torch.cuda.stream(s):
             return empty(*args, **kw)
+
+    def _like(self, t, stream: Optional[int]):
+        return torch.empty_like(t) if stream is None else self._make(stream, torch.empty_like, t)
 
     def _check(self, rc: int) -> None:
         if rc:
@@ -129,7 +130,12 @@ class QuantKvCache:
         n = k.shape[0]
         if q is not None:
             if out is None:
-                out = self._make(stream, torch.empty_like, q, dtype=torch.float16 if q.dtype is torch.float32 else q.dtype)
+                if q.dtype is not torch.float32:
+                    out = self._like(q, stream)
+                elif stream is None:
+                    out = torch.empty_like(q, dtype=torch.float16)
+                else:
+                    out = self._make(stream, torch.empty_like, q, dtype=torch.float16)
             qa, oa = self._rows("q", q, n, self.heads), self._rows("out", out, n, self.heads, False)
         else:
             if out is not None:
@@ -147,7 +153,11 @@ class QuantKvCache:
         n = seq.shape[0]
         if out is None:
             shape = n, self.kv_heads, self.head_dim
-            out = tuple(self._make(stream, torch.empty, shape, dtype=dtype, device=self._dev) for _ in range(2))
+            if stream is None:
+                first = torch.empty(shape, dtype=dtype, device=self._dev)
+            else:
+                first = self._make(stream, torch.empty, shape, dtype=dtype, device=self._dev)
+            out = first, self._like(first, stream)
         a = _LOAD.pack(*self._rows("k", out[0], n, self.kv_heads), *self._rows("v", out[1], n, self.kv_heads),
                        *self._table(table), self._ints("seq", seq, n), self._ints("pos", pos, n), n, 0)
         self._check(self._L.ck_kv_load(self.h, a, self._stream(stream)))
@@ -159,7 +169,7 @@ class QuantKvCache:
         cached positions, the new one among them; sequence i of the table, or seq[i].  scale: 1 / sqrt(head_dim)."""
         n = q.shape[0]
         if out is None:
-            out = self._make(stream, torch.empty_like, q)
+            out = self._like(q, stream)
         a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
                          *self._table(table), self._ints("length", length, n), 0 if seq is None else self._ints("seq", seq, n),
                          n, window, self._scale if scale is None else scale, 0)
@@ -172,7 +182,7 @@ class QuantKvCache:
         sequence i's length[i] cached positions (row i of the table).  Rows of no sequence are zero."""
         n = q.shape[0]
         if out is None:
-            out = self._make(stream, torch.empty_like, q)
+            out = self._like(q, stream)
         s = cu.numel() - 1
         if s < 0:
             raise ValueError("cu: expected one entry more than sequences")
