@@ -443,7 +443,7 @@ int ck_kv_store(ck_kv* h, const ck_kv_store_args* a, void* stream) {
   }
   if (a->k.dtype != a->v.dtype || (a->q.dev && a->q.dtype != a->k.dtype))
     return h->fail(CK_EINVAL, "ck_kv_store: q, k and v have to be of one type");
-  if (!(a->eps >= 0.f) && (a->q_norm || a->k_norm)) return h->fail(CK_EINVAL, "ck_kv_store: eps %g", a->eps);
+  if (!(a->eps >= 0.f && a->eps < INFINITY) && (a->q_norm || a->k_norm)) return h->fail(CK_EINVAL, "ck_kv_store: eps %g", a->eps);
   p.pool = h->pool;
   p.seq = a->seq;
   p.pos = a->pos;

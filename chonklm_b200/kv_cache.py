@@ -44,6 +44,7 @@ _STORE = struct.Struct("@" + 4 * _ROWS + _TABLE + "PPPPPfiii")
 _LOAD = struct.Struct("@" + 2 * _ROWS + _TABLE + "PPii")
 _ATTEND = struct.Struct("@" + 2 * _ROWS + _TABLE + "PPiifi")
 _NO_ROWS = (0, 0, 0, 1, 0)
+_NO_NUMBER = (struct.error, OverflowError)   # a window, scale or eps that its field cannot hold
 
 
 class QuantKvCache:
@@ -141,10 +142,13 @@ class QuantKvCache:
             if out is not None:
                 raise ValueError("out without q")
             qa = oa = _NO_ROWS
-        a = _STORE.pack(*qa, *self._rows("k", k, n, self.kv_heads), *self._rows("v", v, n, self.kv_heads), *oa,
-                        *self._table(table), self._ints("seq", seq, n), self._ints("pos", pos, n),
-                        self._vector("q_norm", q_norm, self.head_dim), self._vector("k_norm", k_norm, self.head_dim),
-                        self._vector("inv_freq", inv_freq, self.head_dim // 2), eps, 1 if interleaved else 0, n, 0)
+        try:
+            a = _STORE.pack(*qa, *self._rows("k", k, n, self.kv_heads), *self._rows("v", v, n, self.kv_heads), *oa,
+                            *self._table(table), self._ints("seq", seq, n), self._ints("pos", pos, n),
+                            self._vector("q_norm", q_norm, self.head_dim), self._vector("k_norm", k_norm, self.head_dim),
+                            self._vector("inv_freq", inv_freq, self.head_dim // 2), eps, 1 if interleaved else 0, n, 0)
+        except _NO_NUMBER as e:
+            raise ValueError(str(e)) from None
         self._check(self._L.ck_kv_store(self.h, a, self._stream(stream)))
         return out
 
@@ -170,9 +174,12 @@ class QuantKvCache:
         n = q.shape[0]
         if out is None:
             out = self._like(q, stream)
-        a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
-                         *self._table(table), self._ints("length", length, n), 0 if seq is None else self._ints("seq", seq, n),
-                         n, window, self._scale if scale is None else scale, 0)
+        try:
+            a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
+                             *self._table(table), self._ints("length", length, n), 0 if seq is None else self._ints("seq", seq, n),
+                             n, window, self._scale if scale is None else scale, 0)
+        except _NO_NUMBER as e:
+            raise ValueError(str(e)) from None
         self._check(self._L.ck_kv_attend(self.h, a, self._stream(stream)))
         return out
 
@@ -187,9 +194,12 @@ class QuantKvCache:
         if s < 0:
             raise ValueError("cu: expected one entry more than sequences")
         cua = self._ints("cu", cu, s + 1)
-        a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
-                         *self._table(table), self._ints("length", length, s), 0, s, window,
-                         self._scale if scale is None else scale, 0)
+        try:
+            a = _ATTEND.pack(*self._rows("q", q, n, self.heads, False), *self._rows("out", out, n, self.heads, False),
+                             *self._table(table), self._ints("length", length, s), 0, s, window,
+                             self._scale if scale is None else scale, 0)
+        except _NO_NUMBER as e:
+            raise ValueError(str(e)) from None
         self._check(self._L.ck_kv_attend_prompt(self.h, a, cua, n, self._stream(stream)))
         return out
 

@@ -296,3 +296,22 @@ def test_blocks_before_the_window_may_be_gone(layout, block):
         c.check()
         _close(got, *_ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), window), 2.0 ** -11)
         assert blocks > 1000 or torch.equal(got, want)
+
+
+def test_numbers_that_no_argument_holds_are_refused():
+    """A window of more than 32 bits or of no whole number, a scale or eps of no finite one."""
+    from chonklm_b200 import _lib
+    c = _cache(4, 2, 64, 4)
+    table, one = _i32([[0, 1]]), _i32([1])
+    q, k = torch.zeros(1, 4, 64, dtype=F16, device="cuda"), torch.zeros(1, 2, 64, dtype=F16, device="cuda")
+    w = torch.ones(64, device="cuda")
+    for f in (lambda: c.attend(q, one, table, window=1 << 40), lambda: c.attend(q, one, table, window=0.5),
+              lambda: c.attend(q, one, table, scale="1"), lambda: c.attend_prompt(q, _i32([0, 1]), one, table, window=1 << 31),
+              lambda: c.attend_prompt(q, _i32([0, 1]), one, table, scale=1j), lambda: c.store(q, k, k, one, one, table, eps="1")):
+        with pytest.raises(ValueError):
+            f()
+    for f in (lambda: c.attend(q, one, table, scale=1e300), lambda: c.attend_prompt(q, _i32([0, 1]), one, table, scale=-1e39),
+              lambda: c.store(q, k, k, one, one, table, q_norm=w, eps=1e300), lambda: c.store(q, k, k, one, one, table, k_norm=w, eps=math.inf)):
+        with pytest.raises((ValueError, _lib.CkError), match="scale|eps|float"):
+            f()
+    c.check()
