@@ -1311,7 +1311,7 @@ int ck_batch_create_kv(ck_engine* h, int max_seqs, int kv_blocks, int kv_kind, c
   if (!h->finalized) return h->fail(CK_ESTATE, "engine not finalized");
   const ck_model_cfg& c = h->cfg;
   if (c.arch != CK_ARCH_LLAMA) return h->fail(CK_EINVAL, "batched decode supports the llama / qwen3 architectures");
-  if (max_seqs < 1 || max_seqs > 1024) return h->fail(CK_EINVAL, "max_seqs %d outside [1, 1024]", max_seqs);
+  if (max_seqs < 1 || max_seqs > KV_MAXQ) return h->fail(CK_EINVAL, "max_seqs %d outside [1, %d]", max_seqs, KV_MAXQ);
   const int max_blocks = (c.context_length + CK_BLK - 1) / CK_BLK;
   if (max_blocks > 256) return h->fail(CK_EINVAL, "batched decode handles contexts up to %d", 256 * CK_BLK);
   if (c.hidden % 32 || c.intermediate % 32 || c.hidden > CK_KMAX || c.intermediate > CK_KMAX)

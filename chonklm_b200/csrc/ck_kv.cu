@@ -185,6 +185,7 @@ cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s) {
 }
 
 cudaError_t kv_attend_launch(const KvAttn& all, const KvDev& d, cudaStream_t s, bool pdl) {
+  if (all.n_dev && all.n > KV_MAXQ) return cudaErrorInvalidValue;
   const int warps = d.sms * kv_token_warps(all.pool.hd, all.pool.vbits), units = kv_units(all.heads, all.pool.kvh);
   for (int i0 = 0; i0 < all.n; i0 += KV_MAXQ) {
     KvAttn a = all;

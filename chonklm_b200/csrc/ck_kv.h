@@ -66,13 +66,17 @@ struct KvLoad {
   KvRows k, v;
 };
 
+// queries of a launch of one-token attention; more take several launches, but
+// not where their number is known only on the device
+#define KV_MAXQ 1024
+
 struct KvAttn {
   KvPool pool;
   KvTable tab;
   const int* seq;            // token form: table row of each query (null: query i reads row i)
   const int* len;            // cached positions of each sequence (len_add is added)
   int len_add;
-  const int* n_dev;          // token form: queries, read on the device when not null
+  const int* n_dev;          // token form: queries, read on the device when not null (n <= KV_MAXQ then)
   const int* cu;             // prompt form: first query row of each sequence, [n + 1]
   int n;                     // token form: queries; prompt form: sequences
   int rows;                  // prompt form: query rows in all

@@ -39,8 +39,8 @@
 #pragma once
 #include "ck_kv.cuh"
 
-#define KV_MAXQ 1024         // queries of one launch (their prefix sums sit in shared memory)
-#define KV_PRE (KV_MAXQ + 2) // their place in the workspace (keeps what follows 16-byte aligned)
+// prefix sums of a launch's queries sit in shared memory, and in the workspace
+#define KV_PRE (KV_MAXQ + 2) // (keeps what follows 16-byte aligned)
 #define KV_PAIR 32           // positions of a pair of records
 #define KV_SLACK 6.f         // log2 that a score may exceed the reference maximum before o is rescaled
 #define KV_BOOST 8.f         // p is kept times 2^8 (cancelled by l), so that small p stay normal fp16 numbers
