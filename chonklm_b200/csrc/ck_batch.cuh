@@ -109,13 +109,6 @@ struct BAttn {
   float eps, scale;
 };
 
-// Programmatic dependent launch: the step's kernels are launched with
-// programmatic stream serialization, so a kernel's CTAs may start while its
-// predecessor is still running.  Each kernel waits (griddepcontrol.wait:
-// the predecessor grid has completed and its writes are visible) before it
-// reads or writes anything the step's kernels share, then lets its own
-// successor launch.  Without the launch attribute both are no-ops.
-
 // ---------------------------------------------------------------------------
 // Embedding of every active entry's token (GGUF_*_EMBEDDING_WGSL, :2615-2866).
 __global__ void __launch_bounds__(256) k_bembed(const uint8_t* w, Lay L, float scale, BStep st, float* x, int H,
@@ -1248,28 +1241,28 @@ int batch_enqueue(ck_batch* b, cudaStream_t s) {
     if (b->kv_kind != CK_BATCH_KV_F16) {
       if ((rc = kvq_enqueue(b, s, i))) return rc;
     } else {
-    BAttn a;
-    a.q = b->q; a.k = b->k; a.v = b->v;
-    a.qw = c.qk_norm ? W.q_norm : nullptr;
-    a.kw = c.qk_norm ? W.k_norm : nullptr;
-    a.kc = b->kv + (size_t)(2 * i) * pool;
-    a.vc = b->kv + (size_t)(2 * i + 1) * pool;
-    a.inv_freq = h->inv_freq + (size_t)i * (hd / 2);
-    a.xo = b->xh;
-    a.heads = c.heads; a.kvh = c.kv_heads; a.hd = hd; a.interleaved = c.rope_interleaved;
-    a.window = (int)c.layer_window[i];
-    a.eps = c.qk_norm_eps;
-    a.scale = (float)(1.0 / sqrt((double)hd));   // ATTN_SCALE (:1711)
-    const int grid = b->max_seqs * c.kv_heads, G = c.heads / c.kv_heads;
-    if (hd == 64 && G == 3 && b->battn_nt == 256)
-      CKB(b, launch_pdl(k_battn_g<2, 3, 256>, dim3(grid), dim3(256), s, a, bstep(b)));
-    else if (hd == 64 && G == 2 && b->battn_nt == 256)
-      CKB(b, launch_pdl(k_battn_g<2, 2, 256>, dim3(grid), dim3(256), s, a, bstep(b)));
-    else if (hd == 64 && G == 3) CKB(b, launch_pdl(k_battn_g<2, 3>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
-    else if (hd == 64 && G == 2) CKB(b, launch_pdl(k_battn_g<2, 2>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
-    else if (hd == 64) CKB(b, launch_pdl(k_battn<2>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
-    else if (hd == 128) CKB(b, launch_pdl(k_battn<4>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
-    else CKB(b, launch_pdl(k_battn<8>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
+      BAttn a;
+      a.q = b->q; a.k = b->k; a.v = b->v;
+      a.qw = c.qk_norm ? W.q_norm : nullptr;
+      a.kw = c.qk_norm ? W.k_norm : nullptr;
+      a.kc = b->kv + (size_t)(2 * i) * pool;
+      a.vc = b->kv + (size_t)(2 * i + 1) * pool;
+      a.inv_freq = h->inv_freq + (size_t)i * (hd / 2);
+      a.xo = b->xh;
+      a.heads = c.heads; a.kvh = c.kv_heads; a.hd = hd; a.interleaved = c.rope_interleaved;
+      a.window = (int)c.layer_window[i];
+      a.eps = c.qk_norm_eps;
+      a.scale = (float)(1.0 / sqrt((double)hd));   // ATTN_SCALE (:1711)
+      const int grid = b->max_seqs * c.kv_heads, G = c.heads / c.kv_heads;
+      if (hd == 64 && G == 3 && b->battn_nt == 256)
+        CKB(b, launch_pdl(k_battn_g<2, 3, 256>, dim3(grid), dim3(256), s, a, bstep(b)));
+      else if (hd == 64 && G == 2 && b->battn_nt == 256)
+        CKB(b, launch_pdl(k_battn_g<2, 2, 256>, dim3(grid), dim3(256), s, a, bstep(b)));
+      else if (hd == 64 && G == 3) CKB(b, launch_pdl(k_battn_g<2, 3>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
+      else if (hd == 64 && G == 2) CKB(b, launch_pdl(k_battn_g<2, 2>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
+      else if (hd == 64) CKB(b, launch_pdl(k_battn<2>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
+      else if (hd == 128) CKB(b, launch_pdl(k_battn<4>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
+      else CKB(b, launch_pdl(k_battn<8>, dim3(grid), dim3(CK_THREADS), s, a, bstep(b)));
     }
     if ((rc = bgemm_launch(b, s, qd, {bseg(W.o, wt[3], b->x, b->x, H)}, b->xh, W.post_norm))) return rc;
     if (b->glu) {   // silu(gate) * up straight into the down projection's tiles (xh.xs stays 1)
@@ -1350,13 +1343,13 @@ int ck_batch_create_kv(ck_engine* h, int max_seqs, int kv_blocks, int kv_kind, c
     size_t pb = 0, mb = 0;
     if (kv_setup(p, h->device, &b->kvdev) != cudaSuccess)
       return bail(b->fail(CK_ECUDA, "quantised cache set-up"));
-    kv_workspace(p, c.heads, b->kvdev.sms, &pb, &mb);
+    kv_workspace(p, b->kvdev.sms, &pb, &mb);
     if ((rc = balloc(b, &p.base, (size_t)c.layers * kv_pool_bytes(p))) || (rc = balloc(b, &b->kv_part, pb)) ||
         (rc = balloc(b, &b->kv_ml, mb)) || (rc = balloc(b, &b->q16, S * qd * 2)) ||
         (rc = balloc(b, &b->o16, S * qd * 2)))
       return bail(rc);
   }
-  if ( (rc = balloc(b, &b->d_tok, S * 4)) ||
+  if ((rc = balloc(b, &b->d_tok, S * 4)) ||
       (rc = balloc(b, &b->d_slot, S * 4)) || (rc = balloc(b, &b->d_pos, S * 4)) ||
       (rc = balloc(b, &b->d_nact, 16)) || (rc = balloc(b, &b->d_btab, S * max_blocks * 4)) ||
       (rc = balloc(b, &b->d_err, 16)) || (rc = balloc(b, &b->d_ids, S * 4)) ||

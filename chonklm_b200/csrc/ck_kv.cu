@@ -75,11 +75,10 @@ static int kv_token_warps(int hd, int vb) {
 // as many rows (16 x sms x 128 for 128 and 256 wide heads, twice that at 64 of
 // which a CTA needs 256), a descriptor of 16 bytes a CTA in the place of the
 // prefix sums.
-int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes) {
+void kv_workspace(const KvPool& p, int sms, size_t* part_bytes, size_t* ml_bytes) {
   const size_t slots = (size_t)sms * (p.hd == 256 ? 16 : 32);
   *part_bytes = slots * 8 * p.hd * sizeof(float);
   *ml_bytes = KV_PRE * sizeof(long long) + slots * 8 * sizeof(float2);
-  return 0;
 }
 
 // the forms of k_kv_token
@@ -311,7 +310,7 @@ int kv_global(int code, const char* fmt, ...) {
 int type_bytes(int t) { return t == CK_DT_F32 ? 4 : 2; }
 
 // token rows: present, of a known type, aligned to their elements
-int check_rows(ck_kv* h, const char* call, const char* name, const ck_kv_rows& r, int n, int heads, bool f32, KvRows* out) {
+int check_rows(ck_kv* h, const char* call, const char* name, const ck_kv_rows& r, int n, bool f32, KvRows* out) {
   if (!r.dev && n > 0) return h->fail(CK_EINVAL, "%s: %s is null", call, name);
   if (r.dtype != CK_DT_F16 && r.dtype != CK_DT_BF16 && !(f32 && r.dtype == CK_DT_F32))
     return h->fail(CK_EINVAL, "%s: %s has type %d, expected %s", call, name, r.dtype, f32 ? "f32, f16 or bf16" : "f16 or bf16");
@@ -392,8 +391,7 @@ int ck_kv_create(const ck_kv_cfg* cfg, int device, ck_kv** out) {
   cudaError_t e = kv_setup(p, device, &h->dev);
   if (e != cudaSuccess) return bail(CK_ECUDA, "set-up", e);
   size_t pb = 0, mb = 0;
-  kv_workspace(p, cfg->heads, h->dev.sms, &pb, &mb);
-
+  kv_workspace(p, h->dev.sms, &pb, &mb);
   if ((e = cudaMalloc(&p.base, kv_pool_bytes(p))) != cudaSuccess || (e = cudaMalloc(&p.err, 16)) != cudaSuccess ||
       (e = cudaMalloc(&h->part, pb)) != cudaSuccess || (e = cudaMalloc(&h->ml, mb)) != cudaSuccess)
     return bail(CK_ENOMEM, "cudaMalloc", e);
@@ -427,15 +425,15 @@ int ck_kv_store(ck_kv* h, const ck_kv_store_args* a, void* stream) {
   if (a->n < 0 || (a->n > 0 && (!a->seq || !a->pos))) return h->fail(CK_EINVAL, "ck_kv_store: bad token list");
   KvStore p;
   memset(&p, 0, sizeof p);
-  const int H = h->cfg.heads, K = h->cfg.kv_heads;
+  const int H = h->cfg.heads;
   int rc;
-  if ((rc = check_rows(h, "ck_kv_store", "k", a->k, a->n, K, true, &p.k)) ||
-      (rc = check_rows(h, "ck_kv_store", "v", a->v, a->n, K, true, &p.v)) ||
+  if ((rc = check_rows(h, "ck_kv_store", "k", a->k, a->n, true, &p.k)) ||
+      (rc = check_rows(h, "ck_kv_store", "v", a->v, a->n, true, &p.v)) ||
       (rc = check_table(h, "ck_kv_store", a->table, &p.tab)))
     return rc;
   if (a->q.dev) {
-    if ((rc = check_rows(h, "ck_kv_store", "q", a->q, a->n, H, true, &p.q)) ||
-        (rc = check_rows(h, "ck_kv_store", "q_out", a->q_out, a->n, H, false, &p.qo)) ||
+    if ((rc = check_rows(h, "ck_kv_store", "q", a->q, a->n, true, &p.q)) ||
+        (rc = check_rows(h, "ck_kv_store", "q_out", a->q_out, a->n, false, &p.qo)) ||
         (rc = check_out(h, "ck_kv_store", "q_out", a->q_out, a->n, H)))
       return rc;
     p.heads = H;
@@ -467,8 +465,8 @@ int ck_kv_load(ck_kv* h, const ck_kv_load_args* a, void* stream) {
   memset(&p, 0, sizeof p);
   const int K = h->cfg.kv_heads;
   int rc;
-  if ((rc = check_rows(h, "ck_kv_load", "k", a->k, a->n, K, true, &p.k)) ||
-      (rc = check_rows(h, "ck_kv_load", "v", a->v, a->n, K, true, &p.v)) ||
+  if ((rc = check_rows(h, "ck_kv_load", "k", a->k, a->n, true, &p.k)) ||
+      (rc = check_rows(h, "ck_kv_load", "v", a->v, a->n, true, &p.v)) ||
       (rc = check_out(h, "ck_kv_load", "k", a->k, a->n, K)) || (rc = check_out(h, "ck_kv_load", "v", a->v, a->n, K)) ||
       (rc = check_table(h, "ck_kv_load", a->table, &p.tab)))
     return rc;
@@ -489,8 +487,8 @@ static int attn_args(ck_kv* h, const char* call, const ck_kv_attend_args* a, int
   if (a->window < 0) return h->fail(CK_EINVAL, "%s: window %d", call, a->window);
   if (!(a->scale > -INFINITY && a->scale < INFINITY)) return h->fail(CK_EINVAL, "%s: scale is not finite", call);
   int rc;
-  if ((rc = check_rows(h, call, "q", a->q, rows, h->cfg.heads, false, &p->q)) ||
-      (rc = check_rows(h, call, "out", a->out, rows, h->cfg.heads, false, &p->o)) ||
+  if ((rc = check_rows(h, call, "q", a->q, rows, false, &p->q)) ||
+      (rc = check_rows(h, call, "out", a->out, rows, false, &p->o)) ||
       (rc = check_out(h, call, "out", a->out, rows, h->cfg.heads)) || (rc = check_table(h, call, a->table, &p->tab)))
     return rc;
   p->pool = h->pool;

@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(KV_STORE_THREADS, TYPE == KV_F32 ? 3 : 4) k_kv
     }
   };
   fetch(0);
-  const int seq = A.seq[t], pos = A.pos[t] + A.pos_add;
+  const int seq = A.seq[t], pos = A.pos[t];
   const bool rope = A.inv_freq != nullptr, inter = A.interleaved;
   if (rope) {
     for (int i = lane; i < HD / 2; i += 32) {

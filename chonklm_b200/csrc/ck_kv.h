@@ -48,7 +48,6 @@ struct KvStore {
   KvPool pool;
   KvTable tab;
   const int *seq, *pos;      // sequence and position of each token (seq < 0: padding, skipped)
-  int pos_add;
   const int* n_dev;          // tokens, read on the device when not null
   int n, heads;              // heads 0: only k and v
   KvRows q, k, v, qo;
@@ -92,7 +91,7 @@ struct KvDev {
   int clusters[4];           // clusters of 1, 2, 4 and 8 CTAs of k_kv_token by unit that run at once
 };
 
-int kv_workspace(const KvPool& p, int heads, int sms, size_t* part_bytes, size_t* ml_bytes);
+void kv_workspace(const KvPool& p, int sms, size_t* part_bytes, size_t* ml_bytes);
 cudaError_t kv_setup(const KvPool& p, int device, KvDev* d);   // kernel attributes too; not inside a stream capture
 cudaError_t kv_store_launch(const KvStore& a, cudaStream_t s, bool pdl);
 cudaError_t kv_load_launch(const KvLoad& a, cudaStream_t s);

@@ -104,7 +104,10 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 }
 __device__ __forceinline__ void proxy_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// Waits for the grid before this one and lets the next one start; no-ops
-// without the launch attribute.
+// Programmatic dependent launch: a kernel that is launched with programmatic
+// stream serialization may start while its predecessor still runs.  It waits
+// (the predecessor's grid has completed and its writes are visible) before it
+// reads or writes anything that they share, then lets its own successor
+// launch.  Without the launch attribute both are no-ops.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
