@@ -315,3 +315,176 @@ def test_numbers_that_no_argument_holds_are_refused():
         with pytest.raises((ValueError, _lib.CkError), match="scale|eps|float"):
             f()
     c.check()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("heads", [128, 129, 130, 300])
+def test_prompt_groups_of_many_heads(heads, hd):
+    """A kv head's query heads in several units where a CTA's rows do not hold them."""
+    lens, news = [70, 33], [9, 33]
+    c, table, k, v, g = _filled(heads, 1, hd, lens, 16, 8, seed=heads)
+    q = torch.randn(sum(news), heads, hd, generator=g).mul_(2).half().cuda()
+    got = c.attend_prompt(q, _cu(news), _i32(lens), table, window=50)
+    c.check()
+    want, mag, top = _ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), 50)
+    _close(got, want, mag, top, 2.0 ** -11)
+    one = c.attend(q[:2].contiguous(), _i32(lens), table)
+    c.check()
+    _close(one, *_ref_attention(q[:2], k, v, lens, [1, 1], 1 / math.sqrt(hd), 0), 0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+def test_prompt_split_with_4_bit_values(layout, dtype):
+    H, K, hd = layout
+    lens, news = [3000, 17, 0, 1500, 5], [33, 17, 2, 1, 9]
+    c, table, k, v, g = _filled(H, K, hd, lens, 32, 4, seed=6)
+    q = torch.randn(sum(news), H, hd, generator=g).mul_(2).to(dtype).cuda()
+    got = c.attend_prompt(q, _cu(news), _i32(lens), table, window=900)
+    c.check()
+    _close(got, *_ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), 900), 2.0 ** -11)
+
+
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("layout", [(9, 3, 64), (4, 1, 256), (24, 2, 64)])
+def test_bf16_prompts(layout, v_bits):
+    """Rows of very different sizes, all-zero ones among them: each is brought to its own power of two."""
+    H, K, hd = layout
+    lens, news = [150, 290], [150, 77]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, v_bits, seed=4)
+    q = (torch.randn(sum(news), H, hd, generator=g) * torch.exp(3 * torch.randn(sum(news), H, 1, generator=g) - 4)).to(BF16).cuda()
+    q[3], q[200, 1] = 0, 0
+    got = c.attend_prompt(q, _cu(news), _i32(lens), table)
+    c.check()
+    _close(got, *_ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), 0), 2.0 ** -11)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0, -0.0, 1e-30])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+def test_scales_of_either_sign_and_zero(layout, dtype, scale):
+    H, K, hd = layout
+    lens, news = [150, 1, 77], [20, 1, 77]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=14)
+    q = torch.randn(sum(news), H, hd, generator=g).mul_(2).to(dtype).cuda()
+    got = c.attend_prompt(q, _cu(news), _i32(lens), table, scale=scale, window=60)
+    c.check()
+    _close(got, *_ref_attention(q, k, v, lens, news, scale, 60), 2.0 ** -11)
+    one = c.attend(q[:3].contiguous(), _i32(lens), table, scale=scale, window=60)
+    c.check()
+    _close(one, *_ref_attention(q[:3], k, v, lens, [1, 1, 1], scale, 60), 0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+def test_attention_rows_off_the_vector_alignment(layout, dtype):
+    """q and out at odd elements with odd strides: the same bits as aligned rows, nothing beside them written; the rows of
+    q may be the output's."""
+    H, K, hd = layout
+    lens, news = [150, 2500], [150, 31]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, 8, seed=15)
+    n, ln, cu = sum(news), _i32(lens), _cu(news)
+    q = torch.randn(n, H, hd, generator=g).mul_(2).to(dtype).cuda()
+
+    def odd(m):
+        base = torch.full((m * (H * hd + 3) + 1,), 7.0, dtype=dtype, device="cuda")
+        return base, base.as_strided((m, H, hd), (H * hd + 3, hd, 1), 1)
+
+    for call, m in ((lambda x, o: c.attend_prompt(x, cu, ln, table, out=o), n), (lambda x, o: c.attend(x, ln, table, out=o), 2)):
+        want = call(q[:m].contiguous(), None)
+        (_, x), (base, o) = odd(m), odd(m)
+        x.copy_(q[:m])
+        assert call(x, o) is o and torch.equal(o, want)
+        o.fill_(7.0)
+        assert (base == 7).all()
+        same = q[:m].clone()
+        assert torch.equal(call(same, same), want)
+    c.check()
+
+
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("layout", [(6, 2, 64), (16, 8, 128), (4, 1, 256)])
+@pytest.mark.parametrize("bad", ["k", "v"])
+def test_a_visible_nan_reaches_the_rows_that_see_it(layout, bad, v_bits):
+    """Prompts: exactly the rows that see the position, all of their dims.  One token: all dims for a key, its group's for
+    a value."""
+    H, K, hd = layout
+    n, at, window = 200, 90, 64
+    c, table, k, v, g = _filled(H, K, hd, [n], 16, v_bits, seed=16)
+    x = torch.randn(1, K, hd, generator=g).cuda()
+    y = x.clone()
+    y[0, 0, 33] = float("nan")                   # kv head 0, group 1
+    c.store(None, *((y, x) if bad == "k" else (x, y)), _i32([0]), _i32([at]), table)
+    q = torch.randn(n, H, hd, generator=g).half().cuda()
+    got = c.attend_prompt(q, _i32([0, n]), _i32([n]), table, window=window)
+    sees = torch.zeros(n, H, 1, dtype=torch.bool, device="cuda")
+    sees[at: at + window, : H // K] = True
+    assert torch.equal(torch.isnan(got), sees.expand_as(got))
+    one = torch.isnan(c.attend(q[:1], _i32([at + 5]), table))
+    assert one[0, : H // K, 32:64].all() and not one[0, H // K:].any()
+    assert one[0, : H // K].all() if bad == "k" else not one[0, : H // K, :32].any() and not one[0, : H // K, 64:].any()
+    assert not torch.isnan(c.attend(q[:1], _i32([at]), table)).any()
+    c.check()
+
+
+def test_replayed_writes_go_where_the_inputs_say():
+    """A captured decode step replayed on other tokens at other positions: the pages hold them, and the outputs are those
+    of a second cache that takes the same calls one by one."""
+    H, K, hd, block = 4, 2, 64, 16
+    c, table, _, _, g = _filled(H, K, hd, [96, 96], block, 8)
+    other, table2, _, _, _ = _filled(H, K, hd, [96, 96], block, 8)
+    assert torch.equal(table, table2)
+    q, kn, vn = (torch.randn(2, h, hd, generator=g).half().cuda() for h in (H, K, K))
+    seq, pos, length = _i32([0, 1]), _i32([4, 89]), _i32([5, 90])
+    f = torch.rand(hd // 2, generator=g).cuda()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c.attend(c.store(q, kn, vn, seq, pos, table, inv_freq=f), length, table)
+    torch.cuda.current_stream().wait_stream(s)
+    other.store(q, kn, vn, seq, pos, table, inv_freq=f)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turned = c.store(q, kn, vn, seq, pos, table, inv_freq=f)
+        out = c.attend(turned, length, table)
+    every = _tokens([96, 96])
+    for _ in range(4):
+        for t in (q, kn, vn):
+            t.copy_(torch.randn(t.shape, generator=g))
+        pos.add_(1)
+        length.add_(1)
+        graph.replay()
+        want = other.store(q, kn, vn, seq, pos, table, inv_freq=f)
+        assert torch.equal(turned, want) and torch.equal(out, other.attend(want, length, table))
+        for a, b in zip(c.load(*every, table), other.load(*every, table)):
+            assert torch.equal(a, b)
+    c.check()
+    other.check()
+
+
+def test_batch_by_list_follows_the_plain_model(tiny_dir):
+    """Contexts past 2048 and more slots than fill the device by unit: the attention's list form and its join, with the
+    number of queries on the device (5 or fewer of 40)."""
+    from chonklm_b200 import _lib
+    from chonklm_b200.registry import ModelDef
+    from chonklm_b200.runtime import loadLlamaWgslModel
+    from test_gpu_batch import _run
+    from test_gpu_batch_quantised import TOL, PlainModel
+    path = tiny_model(tiny_dir, "llama", "q4_k_m", context_length=4096)
+    V = 1000
+    loaded = loadLlamaWgslModel(ModelDef(id="t", label="t", vocab=V, maxContext=4096, gguf=path, eosIds=[]))
+    rng = np.random.default_rng(3)
+    pending = [(rng.integers(0, V, size=n).tolist(), m, ()) for n, m in ((3, 20), (40, 12), (1, 30), (90, 5), (170, 9))]
+    batch = _lib.Batch(loaded.engine.dev, max_seqs=40, kv="q8")
+    got = _run(batch, pending)
+    batch.close()
+    for (prompt, _, _), ids in zip(pending, got):
+        plain = PlainModel(path, loaded, 8)
+        for t in prompt[:-1]:
+            plain.step(t)
+        t = prompt[-1]
+        for want in ids:
+            logits = plain.step(t)
+            assert logits[want] >= logits.max() - 2 * TOL * np.abs(logits).max(), (len(prompt), want)
+            t = want
+    loaded.engine.dispose()
