@@ -97,7 +97,9 @@ struct KvForms {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit4, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM4);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit8, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM8);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB>::SMEM);
+      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB, true>::SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB, false>::SMEM);
     return e == cudaSuccess ? fit(d) : e;
   }
   // clusters of unit8 that run at once: they lie within a GPC, so fewer than SMs / size
@@ -246,11 +248,14 @@ cudaError_t kv_prompt_launch(const KvAttn& all, int sms, cudaStream_t s) {
     const dim3 grid((unsigned)(ctas * splits));
     const int ends = (i0 == 0 ? 1 : 0) | (i0 + a.n == all.n ? 2 : 0);
     cudaError_t e = cudaErrorInvalidValue;
-#define KV_CASE(HD, VB)                                                                                            \
-  if (a.pool.hd == HD && a.pool.vbits == VB)                                                                       \
-    e = kv_launch(k_kv_prompt<HD, VB>, grid, dim3(KvPr<HD, VB>::THREADS), KvPr<HD, VB>::SMEM, s, false, a, units, gs, \
-                  (int)splits, ends);
+#define KV_PROMPT(HD, VB, FINE)                                                                                          \
+  kv_launch(k_kv_prompt<HD, VB, FINE>, grid, dim3(KvPr<HD, VB, FINE>::THREADS), KvPr<HD, VB, FINE>::SMEM, s, false, a, \
+            units, gs, (int)splits, ends)
+#define KV_CASE(HD, VB)                      \
+  if (a.pool.hd == HD && a.pool.vbits == VB) \
+    e = a.o.type == KV_F16 ? KV_PROMPT(HD, VB, true) : KV_PROMPT(HD, VB, false);
     KV_EACH(KV_CASE)
+#undef KV_PROMPT
 #undef KV_CASE
     if (e != cudaSuccess) return e;
     if (splits > 1) {

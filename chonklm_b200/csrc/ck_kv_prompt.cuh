@@ -2,8 +2,9 @@
 // paged cache, on tcgen05.
 //
 //   S = scale Q K^T,  P = exp(S - m) under the causal and window mask,
-//   O = P V / sum P;  K and V = code * scale, rounded to 16 bits (an fp16
-//   cache's values), sums in 32 bits in tensor memory.
+//   O = P V / sum P;  K and V = code * scale, V and (but for fp16 outputs, see
+//   FINE) K rounded to 16 bits (an fp16 cache's values), sums in 32 bits in
+//   tensor memory.
 //
 // Bound by arithmetic once a sequence has some hundred tokens: per 128 x 128
 // tile of scores at head_dim 128 the two products take 1024 cycles of an SM's
@@ -55,7 +56,17 @@
 #define KVP_SLACK 7.f        // log2 that a score may exceed the reference maximum before O is rescaled
 #define KVP_BOOST 8.f        // p is kept times 2^8 (cancelled by l): at most 2^15 as an operand, and normal down to 2^-22
 
-template <int HD, int VB>
+// FINE: keys as two operand tiles.  code * scale has 18 bits, and as one fp16
+// number loses 7 of them: 2^-12 of the magnitudes that a score sums, on average.
+// Split into its scale's upper 4 bits (their product with a 7-bit code is exact)
+// and the rest (rounded to 11 bits: 2^-14 of a key), the scores are two
+// products.  Taken where the output is fp16, whose own rounding is small enough
+// for it to show: a short prompt on 240 positions was off by 3.6 times what the
+// same in 32 bits is, and is by 1.7 times; with bf16 outputs one product is off
+// by 1.08 times.  Time (us) with one product and with two: 133 GFLOP of fresh
+// prompts at head_dim 128 180 and 210; the same lengths at 64 94 and 103; chunks
+// at 256 47 and 57, with 8-bit values 57 and 57.
+template <int HD, int VB, bool FINE>
 struct KvPr {
   using R = KvRec<HD, VB>;
   static constexpr int NQ = HD == 256 ? 1 : 2;            // 128-row query tiles
@@ -66,14 +77,19 @@ struct KvPr {
   static constexpr int W_COPY = SOFT + DEQ, W_S = W_COPY + 1, W_O = W_COPY + 2;   // the single warps
   static constexpr int RECS = PT / KV_TILE;
   static constexpr int STAGE_BYTES = RECS * R::BYTES;
-  static constexpr int STAGES = HD == 256 ? (VB == 8 ? 2 : 3) : 4;   // what fits
-  static constexpr int QB = 128 * HD * 2, KB = PT * HD * 2;
-  static constexpr int SQ = 0, SK = NQ * QB, SV = SK + BUF * KB, SST = SV + BUF * KB;
+  static constexpr int QB = 128 * HD * 2, KB = PT * HD * 2, KT = FINE ? 2 * KB : KB;
+  // Q goes to tensor memory where its shared memory is wanted for K's second
+  // tile (head_dim 256): it is laid out in K's place first
+  static constexpr bool QT = FINE && HD == 256;
+  static constexpr int SQ = 0, SK = QT ? 0 : NQ * QB, SV = SK + BUF * KT, SST = SV + BUF * KB;
+  static constexpr int FIT = (226 * 1024 - SST) / STAGE_BYTES, STAGES = FIT > 4 ? 4 : FIT;
   // at least 120 KB, so that an SM holds one CTA (each takes all of its tensor memory)
   static constexpr int NEED = SST + STAGES * STAGE_BYTES;
   static constexpr int SMEM = NEED < 120 * 1024 ? 120 * 1024 : NEED;
-  static constexpr int TO = NQ * 2 * PT;                  // tensor memory: two score buffers a query tile, then O
-  static_assert(TO + NQ * HD <= 512, "tensor memory");
+  static constexpr int TO = NQ * 2 * PT;                  // tensor memory: two score buffers a query tile, O, Q
+  static constexpr int TQ = TO + NQ * HD;
+  static_assert(TQ + (QT ? HD / 2 : 0) <= 512 && (!QT || NQ * QB <= BUF * KT), "tensor memory, and Q in K's place");
+  static_assert(STAGES >= 2, "K is made a tile ahead of V");
   static_assert(SMEM <= 227 * 1024 - 1024, "shared memory");
 };
 
@@ -187,9 +203,9 @@ __device__ __noinline__ void kvp_zero_rows(const KvAttn& A, int hd, const int* g
 // those before the first and after the last one, and those of a sequence that
 // is refused because it leaves the rows; a row list that goes back is refused
 // as a whole.
-template <int HD, int VB>
-__global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __grid_constant__ KvAttn A, int units, int gs, int splits, int ends) {
-  using C = KvPr<HD, VB>;
+template <int HD, int VB, bool FINE>
+__global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(const __grid_constant__ KvAttn A, int units, int gs, int splits, int ends) {
+  using C = KvPr<HD, VB, FINE>;
   using R = KvRec<HD, VB>;
   extern __shared__ __align__(1024) uint8_t sm[];
   __shared__ uint32_t s_tmem;
@@ -198,7 +214,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
   __shared__ int s_gap, s_gaps[4];             // whether rows lie in no sequence: [0] .. [1] and [2] .. [3]
   __shared__ float s_scale[128 * C::NQ];       // factor of each query row's scores
   __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_v[C::BUF], b_kf[2],
-      b_s[C::NQ][2], b_p[C::NQ][2], b_pv[2], b_o, b_end;
+      b_s[C::NQ][2], b_p[C::NQ][2], b_pv[2], b_o, b_end, b_qt;
   __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 5 ahead)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bt = 128 * C::NQ / gs;             // tokens of a CTA
@@ -272,6 +288,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
       mbar_init(&b_pv[i], 1);
     }
     mbar_init(&b_o, 1);
+    if (C::QT) mbar_init(&b_qt, 1);
     mbar_init(&b_end, 2);
     mbar_fence_init();
   } else if (warp == 2) {
@@ -461,6 +478,16 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
       const uint32_t idS = (1u << 4) | ((uint32_t)(C::PT >> 3) << 17) | (8u << 24);
       const uint64_t dq = umma_desc(smem_u32(sm + C::SQ), 128, 256), dk = umma_desc(smem_u32(sm + C::SK), 128, 256);
       ok = n <= 0 || kvp_wait(&b_q, 0, &s_fail, A.pool.err);
+      if (C::QT && ok && n > 0) {              // 16 of a row's elements a copy: 8 columns
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        if (leader) {
+#pragma unroll 1
+          for (int k = 0; k < HD / 16; k++)
+            asm volatile("tcgen05.cp.cta_group::1.128x256b [%0], %1;" ::"r"(tm + C::TQ + 8 * k), "l"(dq + k * 4096 / 16) : "memory");
+          umma_commit(&b_qt);
+        }
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int it = 0; ok && it < n; it++) {
         const int kb = it & (C::BUF - 1);
@@ -474,9 +501,12 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
           for (int w = 0; w < C::NQ; w++)
             if (it >= from[w] && it < to[w]) {
 #pragma unroll
-              for (int k = 0; k < HD / 16; k++)
-                umma_f16(tm + (2 * w + (it & 1)) * C::PT, dq + (w * C::QB + k * 4096) / 16,
-                         dk + kb * (C::KB / 16) + k * C::PT * 32 / 16, idS, k > 0 ? 1u : 0u);
+              for (int k = 0; k < (FINE ? 2 : 1) * HD / 16; k++) {   // (the second tile of K follows the first)
+                const uint32_t to = tm + (2 * w + (it & 1)) * C::PT;
+                const uint64_t from_k = dk + kb * (C::KT / 16) + k * C::PT * 32 / 16;
+                if (C::QT) umma_f16_ts(to, tm + C::TQ + 8 * (k % (HD / 16)), from_k, idS, k > 0 ? 1u : 0u);
+                else umma_f16(to, dq + (w * C::QB + k % (HD / 16) * 4096) / 16, from_k, idS, k > 0 ? 1u : 0u);
+              }
               umma_commit(&b_s[w][it & 1]);
             }
           umma_commit(&b_kf[it & 1]);
@@ -553,18 +583,30 @@ __global__ void __launch_bounds__(KvPr<HD, VB>::THREADS, 1) k_kv_prompt(const __
           if (kvp_bad<VB>(*(const unsigned short*)(rec + R::VS + kscl))) d[k] = 0x7fffu;
           d[k] |= d[k] << 16;
         }
+        if (C::QT && k0 == 0 && it == 0) ok = kvp_wait(&b_qt, 0, &s_fail, A.pool.err);   // Q has left K's place
         if (k0 == 0 && it >= C::BUF)           // the scores of the tile that was there before are done
           ok = kvp_wait(&b_kf[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < KB; k++) {
-          uint8_t* dst = sm + kdst + kb * C::KB + (kr + (k0 + k) * KW) * 512;
-          *(uint4*)dst =
-              make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c[k].x), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].x), d[k]),
-                         kv_hmul2(kv_half2<0x4140, 128>(c[k].y), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].y), d[k]));
-          *(uint4*)(dst + 128) =
-              make_uint4(kv_hmul2(kv_half2<0x4140, 128>(c[k].z), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].z), d[k]),
-                         kv_hmul2(kv_half2<0x4140, 128>(c[k].w), d[k]), kv_hmul2(kv_half2<0x4342, 128>(c[k].w), d[k]));
+          uint8_t* dst = sm + kdst + kb * C::KT + (kr + (k0 + k) * KW) * 512;
+          const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
+          const uint32_t top = FINE ? d[k] & 0xff80ff80u : d[k];
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            h[2 * e] = kv_half2<0x4140, 128>(w[e]);
+            h[2 * e + 1] = kv_half2<0x4342, 128>(w[e]);
+          }
+          auto put = [&](uint8_t* to, uint32_t by) {
+            *(uint4*)to = make_uint4(kv_hmul2(h[0], by), kv_hmul2(h[1], by), kv_hmul2(h[2], by), kv_hmul2(h[3], by));
+            *(uint4*)(to + 128) = make_uint4(kv_hmul2(h[4], by), kv_hmul2(h[5], by), kv_hmul2(h[6], by), kv_hmul2(h[7], by));
+          };
+          put(dst, top);
+          if (FINE) {
+            const __half2 low = __hsub2(*(const __half2*)&d[k], *(const __half2*)&top);
+            put(dst + C::KB, *(const uint32_t*)&low);
+          }
         }
       }
       proxy_fence_smem();

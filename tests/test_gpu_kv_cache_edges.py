@@ -488,3 +488,54 @@ def test_batch_by_list_follows_the_plain_model(tiny_dir):
             assert logits[want] >= logits.max() - 2 * TOL * np.abs(logits).max(), (len(prompt), want)
             t = want
     loaded.engine.dispose()
+
+
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("length", [2, 700])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_fp16_prompts_keep_the_bits_of_keys(hd, length, v_bits):
+    """Two kinds of key whose code * scale lies at the middle between two fp16 numbers, one rounded up and one down in
+    every dim that the query looks at, and scores of 50: keys as single fp16 numbers move the two kinds' probabilities by
+    several times what is left when the scale's upper 4 bits are a product of their own.  Its rest is below 2^-3 of the
+    scale and rounded to 11 bits: 2^-14 of a key."""
+    d, codes = 1406 * 2.0 ** -14, (95, 96)
+    rel = [(float(np.float16(d * x)) - d * x) / (d * x) for x in codes]
+    assert abs(rel[0] - rel[1]) > 2.0 ** -10.1
+    g = torch.Generator().manual_seed(hd)
+    table, nb = _tables([length], 16, g)
+    seq, pos = _tokens([length])
+    k = torch.empty(length, 1, hd)
+    k[0::2], k[1::2] = codes[0] * d, codes[1] * d
+    k[:, 0, 1::32] = 127 * d                     # the groups' largest values, which the query does not look at
+    v = torch.ones(length, 1, hd)
+    v[1::2] = -1
+    c = _cache(1, 1, hd, nb, 16, v_bits)
+    c.store(None, k.cuda(), v.cuda(), seq, pos, table)
+    kk, vv = c.load(seq, pos, table, dtype=F32)
+    assert torch.equal(kk.cpu(), k)
+    q = torch.ones(1, 1, hd, dtype=F16, device="cuda")
+    q[0, 0, 1::32] = 0
+    scale = 50 / (hd * 31 / 32 * codes[0] * d)
+    want, mag, top = _ref_attention(q, [kk], [vv], [length], [1], scale, 0)
+    for rows, blocks in ((1, table.shape[1]), (1, 1000), (100, table.shape[1])):   # whole, split, on many CTAs
+        wide = torch.zeros(rows, blocks, dtype=torch.int32, device="cuda")
+        wide[:, : table.shape[1]] = table
+        got = c.attend_prompt(q.expand(rows, -1, -1).contiguous(), _cu([1] * rows), _i32([length] * rows), wide, scale=scale)
+        c.check()
+        _close(got, want.expand_as(got), mag, top, 2.0 ** -14)
+
+
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("layout", [(9, 3, 64), (16, 8, 128), (4, 1, 256)])
+def test_fp16_prompts_to_14_bits_of_a_key(layout, v_bits):
+    """Many position tiles and CTAs, ragged, with a window and without."""
+    H, K, hd = layout
+    lens, news = [700, 65, 1300, 64, 129], [700, 65, 300, 1, 129]
+    c, table, k, v, g = _filled(H, K, hd, lens, 16, v_bits, seed=31)
+    q = torch.randn(sum(news), H, hd, generator=g).mul_(2).half().cuda()
+    for window in (0, 150):
+        got = c.attend_prompt(q, _cu(news), _i32(lens), table, window=window)
+        c.check()
+        _close(got, *_ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), window), 2.0 ** -14)
+        for _ in range(50):
+            assert torch.equal(got, c.attend_prompt(q, _cu(news), _i32(lens), table, window=window))
