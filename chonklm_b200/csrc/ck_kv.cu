@@ -82,14 +82,14 @@ void kv_workspace(const KvPool& p, int sms, size_t* part_bytes, size_t* ml_bytes
 }
 
 // the forms of k_kv_token
-template <int HD, int VB>
+template <int HD, int VB, bool FINE>
 struct KvForms {
   using C = KvTok<HD, VB>;
-  static constexpr auto list = k_kv_token<HD, VB, false, C::WARPS, C::STAGES>;
+  static constexpr auto list = k_kv_token<HD, VB, false, C::WARPS, C::STAGES, FINE>;
   // by unit: 4 warps where the units fill the device, else 8 in up to 8 CTAs
   static constexpr int ST4 = HD == 256 ? 1 : 2, ST8 = HD == 256 ? 1 : 2;
-  static constexpr auto unit4 = k_kv_token<HD, VB, true, 4, ST4>;
-  static constexpr auto unit8 = k_kv_token<HD, VB, true, 8, ST8>;
+  static constexpr auto unit4 = k_kv_token<HD, VB, true, 4, ST4, FINE>;
+  static constexpr auto unit8 = k_kv_token<HD, VB, true, 8, ST8, FINE>;
   static constexpr int SUM = 8 * HD * 4;   // a CTA's sum
   static constexpr int SMEM4 = 4 * ST4 * C::PAIR_BYTES + SUM, SMEM8 = 8 * ST8 * C::PAIR_BYTES + SUM;
   static cudaError_t setup(KvDev* d) {
@@ -97,9 +97,7 @@ struct KvForms {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit4, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM4);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(unit8, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM8);
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB, true>::SMEM);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB, false>::SMEM);
+      e = cudaFuncSetAttribute(k_kv_prompt<HD, VB, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, KvPr<HD, VB, FINE>::SMEM);
     return e == cudaSuccess ? fit(d) : e;
   }
   // clusters of unit8 that run at once: they lie within a GPC, so fewer than SMs / size
@@ -147,7 +145,12 @@ struct KvForms {
 cudaError_t kv_setup(const KvPool& p, int device, KvDev* d) {
   const cudaError_t e = cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return e;
-#define KV_CASE(HD, VB) if (p.hd == HD && p.vbits == VB) return KvForms<HD, VB>::setup(d);
+  // (both kinds of a form have the same bounds and shared memory: one answer for their clusters)
+#define KV_CASE(HD, VB)                              \
+  if (p.hd == HD && p.vbits == VB) {                 \
+    const cudaError_t f = KvForms<HD, VB, true>::setup(d); \
+    return f != cudaSuccess ? f : KvForms<HD, VB, false>::setup(d); \
+  }
   KV_EACH(KV_CASE)
 #undef KV_CASE
   return cudaErrorInvalidValue;
@@ -201,8 +204,10 @@ cudaError_t kv_attend_launch(const KvAttn& all, const KvDev& d, cudaStream_t s, 
     if (a.window > 0 && pairs > a.window / KV_PAIR + 2) pairs = a.window / KV_PAIR + 2;
     bool listed = false;
     cudaError_t e = cudaErrorInvalidValue;
-#define KV_CASE(HD, VB) \
-  if (a.pool.hd == HD && a.pool.vbits == VB) e = KvForms<HD, VB>::launch(a, units, pairs, d, s, pdl, &listed);
+#define KV_CASE(HD, VB)                                                                                  \
+  if (a.pool.hd == HD && a.pool.vbits == VB)                                                             \
+    e = a.o.type == KV_F16 ? KvForms<HD, VB, true>::launch(a, units, pairs, d, s, pdl, &listed)          \
+                           : KvForms<HD, VB, false>::launch(a, units, pairs, d, s, pdl, &listed);
     KV_EACH(KV_CASE)
 #undef KV_CASE
     if (e != cudaSuccess) return e;

@@ -86,6 +86,15 @@ __device__ __forceinline__ void kv_drain(uint64_t* bar, int from, int to, int st
     for (unsigned spins = 0; !mbar_try_wait(bar + i % stages, kv_ring_parity(i, stages)) && spins < (1u << 20); spins++) {}
 }
 
+// The upper bits of two fp16 scales, whose product with a code is exact in fp16:
+// 4 bits and a 7-bit code, or 8 and one of 3 bits (or -8).
+#define KV_TOP(BITS) ((BITS) == 8 ? 0xff80ff80u : 0xfff8fff8u)
+// and the rest
+__device__ __forceinline__ uint32_t kv_rest(uint32_t d, uint32_t top) {
+  const __half2 y = __hsub2(*(const __half2*)&d, *(const __half2*)&top);
+  return *(const uint32_t*)&y;
+}
+
 // ---- eight neighbouring elements of a row ----------------------------------
 // they may move as 16-byte vectors: base and strides are multiples of that
 __host__ __device__ inline bool kv_vec8(const KvRows& r) {

@@ -539,3 +539,38 @@ def test_fp16_prompts_to_14_bits_of_a_key(layout, v_bits):
         _close(got, *_ref_attention(q, k, v, lens, news, 1 / math.sqrt(hd), window), 2.0 ** -14)
         for _ in range(50):
             assert torch.equal(got, c.attend_prompt(q, _cu(news), _i32(lens), table, window=window))
+
+
+def _half_and_half(hd, length, v_bits):
+    """Two kinds of value in turn, equally likely: their mean is small beside them, and code * scale of each lies near the
+    middle between two fp16 numbers.  8 bits: 95 d and -96 d; 4 bits: 7 d and -6 d (and -8 d, the groups' largest)."""
+    d, a, b, top = (1406 * 2.0 ** -14, 95, -96, 127) if v_bits == 8 else (1404 * 2.0 ** -14, 7, -6, -8)
+    g = torch.Generator().manual_seed(hd)
+    table, nb = _tables([length], 16, g)
+    seq, pos = _tokens([length])
+    v = torch.empty(length, 1, hd)
+    v[0::2], v[1::2] = a * d, b * d
+    v[:, 0, 1::32] = top * d
+    c = _cache(1, 1, hd, nb, 16, v_bits)
+    c.store(None, torch.ones(length, 1, hd, device="cuda"), v.cuda(), seq, pos, table)
+    _, vv = c.load(seq, pos, table, dtype=F32)
+    assert torch.equal(vv.cpu(), v)
+    want, mag = v.double().mean(0)[0].cuda(), v.double().abs().mean(0)[0].cuda()
+    # the probabilities are equal, powers of two, and exact; the scale's rest below 2^-3 of it is rounded to 11 bits, or
+    # (4 bits) not at all
+    tol = (2.0 ** -14 if v_bits == 8 else 2.0 ** -20) * mag + EPS[F16] * want.abs() + 1e-6
+    wide = torch.zeros(1, 40000, dtype=torch.int32, device="cuda")
+    wide[:, : table.shape[1]] = table
+    return c, table, wide, want, tol
+
+
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("length", [2, 100, 2000])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_fp16_outputs_of_one_token_keep_the_bits_of_values(hd, length, v_bits):
+    c, table, wide, want, tol = _half_and_half(hd, length, v_bits)
+    q = torch.ones(400, 1, hd, dtype=F16, device="cuda")
+    for n, t in ((1, table), (1, wide), (400, table)):       # in clusters, by list, a CTA each
+        got = c.attend(q[:n], _i32([length] * n), t.expand(n, -1).contiguous())
+        assert ((got.double() - want).abs() <= tol).all()
+    c.check()
