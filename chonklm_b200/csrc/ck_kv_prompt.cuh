@@ -2,9 +2,9 @@
 // paged cache, on tcgen05.
 //
 //   S = scale Q K^T,  P = exp(S - m) under the causal and window mask,
-//   O = P V / sum P;  K and V = code * scale, V and (but for fp16 outputs, see
-//   FINE) K rounded to 16 bits (an fp16 cache's values), sums in 32 bits in
-//   tensor memory.
+//   O = P V / sum P;  K and V = code * scale, but for fp16 outputs (FINE)
+//   rounded to 16 bits (an fp16 cache's values), sums in 32 bits in tensor
+//   memory.
 //
 // Bound by arithmetic once a sequence has some hundred tokens: per 128 x 128
 // tile of scores at head_dim 128 the two products take 1024 cycles of an SM's
@@ -56,22 +56,28 @@
 #define KVP_SLACK 7.f        // log2 that a score may exceed the reference maximum before O is rescaled
 #define KVP_BOOST 8.f        // p is kept times 2^8 (cancelled by l): at most 2^15 as an operand, and normal down to 2^-22
 
-// FINE: keys as two operand tiles.  code * scale has 18 bits, and as one fp16
-// number loses 7 of them: 2^-12 of the magnitudes that a score sums, on average.
-// Split into its scale's upper 4 bits (their product with a 7-bit code is exact)
-// and the rest (rounded to 11 bits: 2^-14 of a key), the scores are two
-// products.  Taken where the output is fp16, whose own rounding is small enough
-// for it to show: a short prompt on 240 positions was off by 3.6 times what the
-// same in 32 bits is, and is by 1.7 times; with bf16 outputs one product is off
-// by 1.08 times.  Time (us) with one product and with two: 133 GFLOP of fresh
-// prompts at head_dim 128 180 and 210; the same lengths at 64 94 and 103; chunks
-// at 256 47 and 57, with 8-bit values 57 and 57.
+// FINE: keys and values as two operand tiles each.  code * scale has 18 bits,
+// and as one fp16 number loses 7 of them: 2^-12 of it, on average.  Split into
+// its scale's upper bits (their product with a code is exact, KV_TOP) and the
+// rest (rounded to 11 bits: 2^-14 of a key or value; 4-bit values are exact),
+// the scores and the outputs are two products each.  Taken where the output is
+// fp16, whose own rounding is small enough for it to show: a short prompt on
+// 240 positions is off by 1.07 to 1.21 times what the same in 32 bits is, with
+// one product each by 2 to 3.6 times, with two for the scores alone by 1.3 to
+// 1.7 times; with bf16 outputs one product each is off by 1.08 times.  Time (us)
+// with one and with two: fresh prompts of 133 GFLOP at head_dim 128 180 and 250
+// (the scores' alone 210); the same lengths at 64 94 and 108; chunks at 256 47
+// and 57, with 8-bit values 57 and 68.  Half of that is the products, the rest
+// the memory of the tiles: fewer staging buffers, one V tile at head_dim 128
+// (two, with two staging buffers, took 280), Q in tensor memory at 256 (in
+// shared memory, with two staging buffers, 63 for 57).
 template <int HD, int VB, bool FINE>
 struct KvPr {
   using R = KvRec<HD, VB>;
   static constexpr int NQ = HD == 256 ? 1 : 2;            // 128-row query tiles
   static constexpr int PT = 64;                           // positions of a K / V tile
   static constexpr int BUF = HD == 256 ? 1 : 2;           // K and V tiles
+  static constexpr int VBUF = FINE && HD == 128 ? 1 : BUF;
   static constexpr int SOFT = 4 * NQ, DEQ = 12 - SOFT;    // warps
   static constexpr int THREADS = (SOFT + DEQ + 3) * 32;
   static constexpr int W_COPY = SOFT + DEQ, W_S = W_COPY + 1, W_O = W_COPY + 2;   // the single warps
@@ -81,7 +87,7 @@ struct KvPr {
   // Q goes to tensor memory where its shared memory is wanted for K's second
   // tile (head_dim 256): it is laid out in K's place first
   static constexpr bool QT = FINE && HD == 256;
-  static constexpr int SQ = 0, SK = QT ? 0 : NQ * QB, SV = SK + BUF * KT, SST = SV + BUF * KB;
+  static constexpr int SQ = 0, SK = QT ? 0 : NQ * QB, SV = SK + BUF * KT, SST = SV + VBUF * KT;
   static constexpr int FIT = (226 * 1024 - SST) / STAGE_BYTES, STAGES = FIT > 4 ? 4 : FIT;
   // at least 120 KB, so that an SM holds one CTA (each takes all of its tensor memory)
   static constexpr int NEED = SST + STAGES * STAGE_BYTES;
@@ -116,6 +122,11 @@ __device__ __forceinline__ float kvp_max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+// 16 codes, neighbours in pairs, times a scale, into an operand tile
+__device__ __forceinline__ void kvp_put(uint8_t* to, const uint32_t (&h)[8], uint32_t by) {
+  *(uint4*)to = make_uint4(kv_hmul2(h[0], by), kv_hmul2(h[1], by), kv_hmul2(h[2], by), kv_hmul2(h[3], by));
+  *(uint4*)(to + 128) = make_uint4(kv_hmul2(h[4], by), kv_hmul2(h[5], by), kv_hmul2(h[6], by), kv_hmul2(h[7], by));
 }
 // a plus the fp16 number h, in 32 bits
 __device__ __forceinline__ void kvp_add16(float& a, unsigned short h) { asm("add.rn.f32.f16 %0, %1, %0;" : "+f"(a) : "h"(h)); }
@@ -212,7 +223,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
   __shared__ volatile int s_fail;
   __shared__ int s_seq, s_tile, s_cu0, s_cu1, s_len;
   __shared__ int s_gap, s_gaps[4];             // whether rows lie in no sequence: [0] .. [1] and [2] .. [3]
-  __shared__ float s_scale[128 * C::NQ];       // factor of each query row's scores
+  __shared__ signed char s_exp[128 * C::NQ];   // each query row's products want 2^(this - 8) times the scale
   __shared__ __align__(8) uint64_t b_full[C::STAGES], b_empty[C::STAGES], b_q, b_k[C::BUF], b_v[C::BUF], b_kf[2],
       b_s[C::NQ][2], b_p[C::NQ][2], b_pv[2], b_o, b_end, b_qt;
   __shared__ uint32_t s_miss[8];               // records of a tile that do not exist, by tile & 7 (copies run at most 5 ahead)
@@ -381,11 +392,10 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");           // each lane goes on with what it copied itself
-    const float fac = fabsf(A.scale) * 1.4426950408889634f;
     const uint32_t flip = A.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll 1
     for (int row = warp * RW + y; row - y < ROWS; row += NWQ * RW) {
-      float back = fac;
+      int e = 8;
       if (A.q.type != KV_F16 || flip) {
         uint32_t u[4][4];
 #pragma unroll
@@ -402,10 +412,9 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
           m[0] = max(m[0] & 0xffffu, m[0] >> 16);
 #pragma unroll
           for (int o = 1; o < L; o <<= 1) m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
-          int e = (int)(m[0] >> 7) - 127;
+          e = (int)(m[0] >> 7) - 127;
           e = e > 127 ? 8 : max(e, -100);
           const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-          back *= __uint_as_float((uint32_t)(127 + e - 8) << 23);
 #pragma unroll
           for (int p = 0; p < 4; p++)
 #pragma unroll
@@ -417,10 +426,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
           for (int p = 0; p < 4; p++)
             *place(row, p) = make_uint4(u[p][0] ^ flip, u[p][1] ^ flip, u[p][2] ^ flip, u[p][3] ^ flip);
       }
-      // (a scale of 0 counts as one too small to show: masked scores are -inf
-      // times it; and past 2^100 no softmax changes: scores that differ do so
-      // by 2^-48 at least, the smallest product of two fp16 numbers)
-      if (x == 0 && row < ROWS) s_scale[row] = fminf(fmaxf(back, 1e-37f), 0x1p100f);
+      if (x == 0 && row < ROWS) s_exp[row] = (signed char)e;
     }
     proxy_fence_smem();
     mbar_arrive(&b_q);
@@ -518,7 +524,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
       const uint64_t dv = umma_desc(smem_u32(sm + C::SV), HD * 16, 128);
 #pragma unroll 1
       for (int it = 0; ok && it < n; it++) {
-        const int vb = it & (C::BUF - 1);
+        const int vb = it & (C::VBUF - 1);
         // two buffers: this V is announced with the next K
         if (C::BUF == 1) ok = kvp_wait(&b_v[0], it & 1, &s_fail, A.pool.err);
         else ok = kvp_wait(&b_k[(it + 1) & 1], ((it + 1) >> 1) & 1, &s_fail, A.pool.err);
@@ -529,9 +535,9 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
             asm volatile("tcgen05.fence::after_thread_sync;");
             if (ok && leader) {
 #pragma unroll
-              for (int k = 0; k < C::PT / 16; k++)
-                umma_f16_ts(tm + C::TO + w * HD, tm + (2 * w + (it & 1)) * C::PT + 8 * k,
-                            dv + vb * (C::KB / 16) + k * 2 * HD * 16 / 16, idO, it == from[w] && k == 0 ? 0u : 1u);
+              for (int k = 0; k < (FINE ? 2 : 1) * C::PT / 16; k++)
+                umma_f16_ts(tm + C::TO + w * HD, tm + (2 * w + (it & 1)) * C::PT + 8 * (k % (C::PT / 16)),
+                            dv + vb * (C::KT / 16) + k * 2 * HD * 16 / 16, idO, it == from[w] && k == 0 ? 0u : 1u);
             }
             __syncwarp();
           }
@@ -591,22 +597,15 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
         for (int k = 0; k < KB; k++) {
           uint8_t* dst = sm + kdst + kb * C::KT + (kr + (k0 + k) * KW) * 512;
           const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
-          const uint32_t top = FINE ? d[k] & 0xff80ff80u : d[k];
+          const uint32_t top = FINE ? d[k] & KV_TOP(8) : d[k];
           uint32_t h[8];
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             h[2 * e] = kv_half2<0x4140, 128>(w[e]);
             h[2 * e + 1] = kv_half2<0x4342, 128>(w[e]);
           }
-          auto put = [&](uint8_t* to, uint32_t by) {
-            *(uint4*)to = make_uint4(kv_hmul2(h[0], by), kv_hmul2(h[1], by), kv_hmul2(h[2], by), kv_hmul2(h[3], by));
-            *(uint4*)(to + 128) = make_uint4(kv_hmul2(h[4], by), kv_hmul2(h[5], by), kv_hmul2(h[6], by), kv_hmul2(h[7], by));
-          };
-          put(dst, top);
-          if (FINE) {
-            const __half2 low = __hsub2(*(const __half2*)&d[k], *(const __half2*)&top);
-            put(dst + C::KB, *(const uint32_t*)&low);
-          }
+          kvp_put(dst, h, top);
+          if (FINE) kvp_put(dst + C::KB, h, kv_rest(d[k], top));
         }
       }
       proxy_fence_smem();
@@ -615,7 +614,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
       return true;
     };
     auto make_v = [&](int it) {
-      const int s = it % C::STAGES, vb = it % C::BUF, j = jb + it;
+      const int s = it % C::STAGES, vb = it % C::VBUF, j = jb + it;
       const uint8_t* stg = sm + C::SST + s * C::STAGE_BYTES;
       bool ok = true;
 #pragma unroll
@@ -633,24 +632,25 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
             d[k][nib] = e | (e << 16);
           }
         }
-        if (k0 == 0 && it >= C::BUF)           // and so is its output
-          ok = kvp_wait(&b_pv[(it - C::BUF) & 1], ((it - C::BUF) >> 1) & 1, &s_fail, A.pool.err);
+        if (k0 == 0 && it >= C::VBUF)          // and so is its output
+          ok = kvp_wait(&b_pv[(it - C::VBUF) & 1], ((it - C::VBUF) >> 1) & 1, &s_fail, A.pool.err);
         if (!ok) return false;
 #pragma unroll
         for (int k = 0; k < VB4; k++) {
-          uint8_t* dst = sm + vdst + vb * C::KB + (vr + (k0 + k) * VW) * (HD * 32);
+          uint8_t* dst = sm + vdst + vb * C::KT + (vr + (k0 + k) * VW) * (HD * 32);
           const uint32_t w[4] = {c[k].x, c[k].y, c[k].z, c[k].w};
 #pragma unroll
           for (int nib = 0; nib < (VB == 8 ? 1 : 2); nib++) {
-            uint32_t o[8];
+            uint32_t h[8];
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-              o[2 * e] = kv_hmul2(kv_code2<VB>(__byte_perm(w[e], 0x64646464u, 0x4140), nib), d[k][nib]);
-              o[2 * e + 1] = kv_hmul2(kv_code2<VB>(__byte_perm(w[e], 0x64646464u, 0x4342), nib), d[k][nib]);
+              h[2 * e] = kv_code2<VB>(__byte_perm(w[e], 0x64646464u, 0x4140), nib);
+              h[2 * e + 1] = kv_code2<VB>(__byte_perm(w[e], 0x64646464u, 0x4342), nib);
             }
             // the other group of a 4-bit chunk: 32 dims on
-            *(uint4*)(dst + nib * 512) = make_uint4(o[0], o[1], o[2], o[3]);
-            *(uint4*)(dst + nib * 512 + 128) = make_uint4(o[4], o[5], o[6], o[7]);
+            const uint32_t top = FINE ? d[k][nib] & KV_TOP(VB) : d[k][nib];
+            kvp_put(dst + nib * 512, h, top);
+            if (FINE) kvp_put(dst + nib * 512 + C::KB, h, kv_rest(d[k][nib], top));
           }
         }
       }
@@ -676,7 +676,12 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
     const int rr = 128 * wq + rl, rtok = rr / gs, rhead = rr % gs;
     const bool rlive = rtok < ntok && rhead < nh;
     kvp_wait(&b_q, 0, &s_fail, A.pool.err);
-    const float sc = s_scale[rr];
+    // the factor of this row's scores (a scale of 0 counts as one too small to
+    // show: masked scores are -inf times it; and past 2^100 no softmax changes:
+    // scores that differ do so by 2^-48 at least, the smallest product of two
+    // fp16 numbers)
+    const float sc = fminf(fmaxf(fabsf(A.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + s_exp[rr] - 8) << 23), 1e-37f),
+                           0x1p100f);
     const int rpos = pos0 + rtok;                                 // position of the row's token
     const int rlo = kvp_low(rpos, A.window);
     // The reference before (raw) and after the factor sc (m), and less the

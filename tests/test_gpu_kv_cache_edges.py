@@ -574,3 +574,15 @@ def test_fp16_outputs_of_one_token_keep_the_bits_of_values(hd, length, v_bits):
         got = c.attend(q[:n], _i32([length] * n), t.expand(n, -1).contiguous())
         assert ((got.double() - want).abs() <= tol).all()
     c.check()
+
+
+@pytest.mark.parametrize("v_bits", [8, 4])
+@pytest.mark.parametrize("length", [2, 100, 2000])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_fp16_prompts_keep_the_bits_of_values(hd, length, v_bits):
+    c, table, wide, want, tol = _half_and_half(hd, length, v_bits)
+    q = torch.ones(400, 1, hd, dtype=F16, device="cuda")
+    for n, t in ((1, table), (1, wide), (400, table)):       # whole, split, on many CTAs
+        got = c.attend_prompt(q[:n], _cu([1] * n), _i32([length] * n), t.expand(n, -1).contiguous())
+        assert ((got.double() - want).abs() <= tol).all()
+    c.check()
