@@ -119,16 +119,18 @@ struct KvForms {
     }
     return cudaSuccess;
   }
-  // pairs: most pairs of records that a unit can have.  *listed: whether the
-  // list was taken (its parts want joining).  By unit costs one launch instead
-  // of two, by list balances.  Measured (us by unit, by list), lengths from a
-  // third of the longest up: at head_dim 128 one query of 2 units over up to
-  // 4000 positions 9.8 and 11.2, over 8000 12.8 and 11.8; 16 of 2 units (4 CTAs
-  // each) over 4000 12.4 and 17.8, over 8000 18.5 and 21.9; 64 of 8 units (a CTA
-  // each) over 1040 29.3 and 29.6, over 2000 48.4 and 48.1, over 8000 153 and
-  // 134; at head_dim 256 64 of one unit over 2000 17.6 and 28.0.  Clusters that
-  // do not all run at once make a second wave: 16 of 8 CTAs, where 15 fit, took
-  // 12.4, in clusters of 4 8.0
+  // pairs: most pairs of records that a unit can have (the block table's width
+  // and the window stand for the lengths, which only the device knows).
+  // *listed: whether the list was taken (its parts want joining).  By unit costs
+  // one launch instead of two, by list balances.  Measured (us by unit, by
+  // list), lengths from a third of the longest up: at head_dim 128 one query of
+  // 2 units over up to 4000 positions 9.8 and 11.2; 16 of 2 units (4 CTAs each)
+  // over 4000 12.4 and 17.8, over 8000 18.5 and 21.9; 64 of 8 units (a CTA each)
+  // over 1040 29.3 and 29.6, over 2000 48.4 and 48.1, over 8000 153 and 134; at
+  // head_dim 256 64 of one unit over 2000 17.6 and 28.0.  One bound serves all,
+  // and at its end it is not every call's best: one query of 2 units over 8000
+  // takes 12.8 and 11.8.  Clusters that do not all run at once make a second
+  // wave: 16 of 8 CTAs, where 15 fit, took 12.4, in clusters of 4 8.0
   static cudaError_t launch(const KvAttn& a, int units, long long pairs, const KvDev& d, cudaStream_t s, bool pdl,
                             bool* listed) {
     const long long n = (long long)a.n * units;

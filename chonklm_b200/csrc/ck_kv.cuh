@@ -191,13 +191,14 @@ __device__ __forceinline__ void kv_st4(const KvRows& r, size_t off, float4 f, bo
 // group of 32 values 4 lanes.  The cosines and sines of the token's position
 // are made once per warp and lie in shared memory with the norm weights, so
 // that four CTAs fit an SM (three for 32-bit rows).
-// Its bytes would bound it, but what does is latency, then instructions: 16
-// heads and 8 kv heads of 128 take some 2500 warp instructions a token, two
-// IEEE divisions a group among them, which the definition of scale and code
-// needs.  Ragged prompts of 214 MB take 52 us (63 % of the copy bandwidth); with
-// cosines, sines and weights in registers, three CTAs an SM, 69; with the same
-// operands one by one instead of in pairs 71; five CTAs (48 registers) 72.  For
-// 32-bit rows three CTAs take 69 us, two 79, four 73.
+// Its bytes would bound it, but what does is instructions (issue slots 74 %
+// busy), then latency: 16 heads and 8 kv heads of 128 take some 2500 warp
+// instructions a token, two IEEE divisions a group among them, which the
+// definition of scale and code needs.  Ragged prompts of 214 MB take 52 us (63 %
+// of the copy bandwidth); with cosines, sines and weights in registers, three
+// CTAs an SM, 69; with the same operands one by one instead of in pairs 71; five
+// CTAs (48 registers) 72.  For 32-bit rows three CTAs take 69 us, two 79, four
+// 73.
 
 // two 32-bit floats at once
 __device__ __forceinline__ uint64_t kv_two(float a, float b) {

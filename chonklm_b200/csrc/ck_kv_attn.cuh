@@ -20,8 +20,8 @@
 //             warps' parts added through shared memory, the CTAs' through
 //             distributed shared memory; one launch.
 // Measured at head_dim 128, 4-bit values: 64 sequences of 493 MB in all take
-// 92 us by list (5.4 TB/s, 82 % of the copy bandwidth; 375 warp instructions
-// a record, issue slots 61 % busy) and the join 9 more.  A warp a record, a
+// 92 us by list (5.4 TB/s, 82 % of the copy bandwidth; 380 warp instructions
+// a record, issue slots 62 % busy) and the join 8 more.  A warp a record, a
 // row of heads as the product's rows, took 139 us: pairs halve the fixed work
 // of a step, and the heads as columns waste none of the product's rows.  16 or
 // 8 warps an SM instead of 12 took 105 and 119 us.

@@ -233,7 +233,7 @@ int ck_batch_create(ck_engine* h, int max_seqs, int kv_blocks, ck_batch** out);
 int ck_batch_create_kv(ck_engine* h, int max_seqs, int kv_blocks, int kv_kind, ck_batch** out);
 /* Keys and values [n][kv_heads][head_dim] of a running sequence's first
  * min(n, cap) positions in one layer, as a quantised batch's pages hold them
- * (host fp32); *n = its cached positions. */
+ * (host fp32); *n = its cached positions (0 before its first step). */
 int ck_batch_read_kv(ck_batch* b, int seq_id, int layer, float* k, float* v, int cap, int* n);
 /* Queue a sequence: prompt of n >= 1 ids, up to max_new >= 1 generated ids
  * (capped at the context left, as generateLlamaWgsl does), stopping after
@@ -339,8 +339,9 @@ int ck_kv_load(ck_kv* h, const ck_kv_load_args* a, void* stream);
 /* One new token per query, whose own key and value are stored already:
  * out = softmax(scale q k) v over the last `window` of its len positions, zero
  * where len is 0.  The cached length is split over the device and joined.
- * Products run on 16-bit operands with 32-bit sums: cached values of more
- * than 65504 in magnitude are out of range. */
+ * Products run on 16-bit operands with 32-bit sums; with f16 outputs a cached
+ * number is two operands (14 bits or more).  Cached values of more than 65504
+ * in magnitude are out of range: rows that see one are NaN or infinite. */
 int ck_kv_attend(ck_kv* h, const ck_kv_attend_args* a, void* stream);
 /* Several new tokens per sequence: rows cu[i] .. cu[i + 1] of q ([rows] in
  * all) are the last tokens of sequence i's len[i] cached positions, each
