@@ -27,17 +27,16 @@
 //             rounded to 11 bits as the operand and kept times 2^8, so that
 //             it is a normal fp16 number down to 2^-22 of the reference and
 //             not lost above 2^-33; l sums the rounded P, so that the weights
-//             still add up to one (fresh prompts, below: 190.3 us, 189.4 with
-//             the unrounded sum)
+//             still add up to one (0.5 % of the fresh prompts' time, below)
 // A CTA holds 256 query rows (two tiles, whose products and softmaxes take
 // turns; the K and V tiles serve both) or, at head_dim 256, 128.  A query row
 // is a (token, head of the kv head's group) pair, so the group shares K and V.
 // CTAs are numbered by depth (position of the tile within its sequence), the
 // deepest first: they take longest.
 //
-// Measured: ragged fresh prompts of 133 GFLOP at head_dim 128 take 190 us (700
-// TFLOP/s, 42 % of cuBLAS's bf16 rate), the first form with one K and V tile
-// and one warp for both products 296.  What bounds it now is the softmax's
+// Measured: ragged fresh prompts of 133 GFLOP, bf16, at head_dim 128 take 192.5
+// us (690 TFLOP/s, 42 % of cuBLAS's bf16 rate), the first form with one K and V
+// tile and one warp for both products 296.  What bounds it now is the softmax's
 // chain (scores read, maximum, exponentials, P written: some 2250 cycles for a
 // K tile against both query tiles, of which the products fill 1024) and some
 // 15000 cycles at a CTA's start, when Q is laid out and each role's code is
@@ -63,7 +62,7 @@
 // the scores and the outputs are two products each.  Taken where the output is
 // fp16, whose own rounding is small enough for it to show: a short prompt on
 // 240 positions is off by 1.07 to 1.21 times what the same in 32 bits is, with
-// one product each by 2 to 3.6 times, with two for the scores alone by 1.3 to
+// one product each by up to 3.6 times, with two for the scores alone by 1.3 to
 // 1.7 times; with bf16 outputs one product each is off by 1.08 times.  Time (us)
 // with one and with two: fresh prompts of 133 GFLOP at head_dim 128 180 and 250
 // (the scores' alone 210); the same lengths at 64 94 and 108; chunks at 256 47
@@ -210,10 +209,9 @@ __device__ __noinline__ void kvp_zero_rows(const KvAttn& A, int hd, const int* g
 }
 
 // ends: 1, this launch has the call's first sequences; 2, its last.  Query rows
-// that lie in no sequence are written as zeros:
-// those before the first and after the last one, and those of a sequence that
-// is refused because it leaves the rows; a row list that goes back is refused
-// as a whole.
+// that lie in no sequence are written as zeros: those before the first and after
+// the last one, and those of a sequence that is refused because it leaves the
+// rows; a row list that goes back is refused as a whole.
 template <int HD, int VB, bool FINE>
 __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(const __grid_constant__ KvAttn A, int units, int gs, int splits, int ends) {
   using C = KvPr<HD, VB, FINE>;
@@ -254,9 +252,7 @@ __global__ void __launch_bounds__(KvPr<HD, VB, FINE>::THREADS, 1) k_kv_prompt(co
     }
     int hi = __reduce_max_sync(0xffffffffu, most);
     gap = __any_sync(0xffffffffu, gap);
-    if (gap) {
-      back = kvp_gaps(A, ends, s_gaps);
-    }
+    if (gap) back = kvp_gaps(A, ends, s_gaps);
     if (!back && above(0) > b) {
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
